@@ -34,6 +34,15 @@ class QGemmItem(ctypes.Structure):
                 ("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("mode", ctypes.c_int32), ("opts", QGemmOpts)]
 
 
+class ResidualNorm(ctypes.Structure):
+    """include/hh.h: hh_residual_norm -- the operands of hh_residual_norm_fwd / _bwd."""
+    _fields_ = [("rows", c_i64), ("groups", c_i64), ("cols", ctypes.c_int32), ("x_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("h_dtype", ctypes.c_int32),
+                ("gate_kind", ctypes.c_int32), ("gate_tanh", ctypes.c_int32), ("rms", ctypes.c_int32), ("res_scale", c_float), ("post_eps", c_float), ("pre_eps", c_float),
+                ("gate", c_vp), ("post_gamma", c_vp), ("post_beta", c_vp), ("pre_gamma", c_vp), ("pre_beta", c_vp), ("x", c_vp), ("y", c_vp), ("x_new", c_vp), ("h", c_vp),
+                ("dx_new", c_vp), ("dh", c_vp), ("dx", c_vp), ("dy", c_vp), ("dgate", c_vp), ("dpost_gamma", c_vp), ("dpost_beta", c_vp), ("dpre_gamma", c_vp),
+                ("dpre_beta", c_vp), ("workspace", c_vp)]
+
+
 QGEMM_GROUP_MAX = 12          # include/hh.h: HH_QGEMM_GROUP_MAX
 
 
@@ -111,10 +120,21 @@ SIGNATURES = {
     "hh_adamw_step": [c_vp, c_vp, c_vp, c_vp, c_i64, c_float, c_float, c_float, c_float, c_float, c_int, c_vp],
     "hh_adamw_arena_step": [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_float, c_float, c_float, c_float,
                             c_float, c_int, c_vp],
+    "hh_embed_tokens_fwd": [c_vp, c_int, c_vp, c_int, c_vp, c_vp, c_int, c_i64, c_int, c_i64, c_int, c_float, c_vp],
+    "hh_workspace_bytes_embed_tokens_bwd": [c_i64, c_int, c_i64, c_int],
+    "hh_embed_tokens_bwd": [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_vp, c_i64, c_int, c_i64, c_int, c_float, c_i64, c_vp, c_vp],
+    "hh_residual_norm_fwd": [ctypes.POINTER(ResidualNorm), c_vp],
+    "hh_workspace_bytes_residual_norm_bwd": [c_i64, c_int, c_i64],
+    "hh_residual_norm_bwd": [ctypes.POINTER(ResidualNorm), c_vp],
+    "hh_act8_fwd": [c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_vp],
+    "hh_act8_bwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_int, c_int, c_vp],
+    "hh_workspace_bytes_gemm_tn_act8": [c_int, c_int, c_i64],
+    "hh_gemm_tn_act8": [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_int, c_i64, c_vp, c_vp],
 }
 _RESTYPES = {"hh_last_error_string": ctypes.c_char_p, "hh_call_count": c_i64, "hh_debug_space_redo_count": c_i64, "hh_prof_kernel_name": ctypes.c_char_p, "hh_workspace_bytes_gemm_splitk": c_i64, "hh_workspace_bytes_gemm_tn": c_i64, "hh_workspace_bytes_gemm_zstats": c_i64,
              "hh_workspace_bytes_xattn_bwd": c_i64, "hh_workspace_bytes_xattn_fwd": c_i64, "hh_workspace_bytes_attn_cls_partial": c_i64, "hh_workspace_bytes_egonce": c_i64,
-             "hh_workspace_bytes_mattn_fwd": c_i64, "hh_workspace_bytes_mattn_bwd": c_i64}
+             "hh_workspace_bytes_mattn_fwd": c_i64, "hh_workspace_bytes_mattn_bwd": c_i64,
+             "hh_workspace_bytes_embed_tokens_bwd": c_i64, "hh_workspace_bytes_residual_norm_bwd": c_i64, "hh_workspace_bytes_gemm_tn_act8": c_i64}
 
 _lib = None
 
@@ -132,7 +152,7 @@ def lib():
             fn = getattr(L, name)          # AttributeError if the symbol is missing
             fn.argtypes = args
             fn.restype = _RESTYPES.get(name, c_int)
-        for cname, cls in ((b"hh_gemm_epilogue", GemmEpilogue), (b"hh_qgemm_opts", QGemmOpts), (b"hh_qgemm_item", QGemmItem)):
+        for cname, cls in ((b"hh_gemm_epilogue", GemmEpilogue), (b"hh_qgemm_opts", QGemmOpts), (b"hh_qgemm_item", QGemmItem), (b"hh_residual_norm", ResidualNorm)):
             if L.hh_abi_sizeof(cname) != ctypes.sizeof(cls):
                 raise RuntimeError("libhh.so was built from another include/hh.h: sizeof(%s) is %d there, %d in this binding -- rebuild it "
                                    "(`python -m helping_hand_for_egocentric_videos_amd.build --force`)" % (cname.decode(), L.hh_abi_sizeof(cname), ctypes.sizeof(cls)))

@@ -1,0 +1,195 @@
+// Activation checkpoints in 8 bits: what a backward pass needs of a forward activation u, kept as e4m3 values q with one scale s = 2^k for
+// every 128 consecutive channels of a row, u ~ q * s.
+//
+//   forward:   a = act(u) from the exact u;  k = the smallest whole number with max|u| <= 448 * 2^k over the 128 channels (448 = 1.75 * 2^8 is
+//              the largest e4m3 value; k is held in [-117, 120], and is 0 where all are zero);  q = u / s rounded to nearest, ties to even.
+//              A power of two, because then u / s and q * s are exact in fp32, and q * s (4 significant bits) is exact in bf16 too: the matrix core
+//              takes a checkpoint without a second rounding (gemm_tn8.hip), and the only error is e4m3's own half step, 2^-4 of the value
+//              (2^-10 of s below 2^-6 of s).  k >= -117 keeps the smallest step, 2^(k - 9), a normal number.
+//              Infinities and NaN do not count for the scale; both are stored as e4m3's NaN, so that a gradient that uses them shows it.
+//   backward:  v = q * s;  du = da * act'(v), and on request act(v), the operand of the next product's weight gradient.
+//
+// Both are HBM-bound: a lane takes 8 channels (16 B of bf16), 16 lanes share a scale.
+#include "common.h"
+
+#define ACT8_GROUP 128
+
+__device__ __forceinline__ float sigmoid1702(float v) { return 1.f / (1.f + expf(-1.702f * v)); }
+__device__ __forceinline__ float act_value(float v, int act) {
+    if (act == HH_ACT_QUICKGELU) return v * sigmoid1702(v);
+    if (act == HH_ACT_RELU) return v < 0.f ? 0.f : v;             // (keeps NaN)
+    return v;
+}
+__device__ __forceinline__ float act_slope(float v, int act) {
+    if (act == HH_ACT_QUICKGELU) {
+        const float s = sigmoid1702(v);
+        return s * (1.f + 1.702f * v * (1.f - s));
+    }
+    if (act == HH_ACT_RELU) return v > 0.f ? 1.f : 0.f;
+    return 1.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool whole, int n, float (&v)[8]) {
+    if (whole) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+        } else {
+            const u32x4 t = *(const u32x4*)p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_lo_to_f32(t[j]); v[2 * j + 1] = bf16_hi_to_f32(t[j]); }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool whole, int n, const float (&v)[8]) {
+    if (whole) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+            *(f32x4*)p = a;
+            *(f32x4*)(p + 4) = b;
+        } else {
+            const u32x4 t = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+            *(u32x4*)p = t;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) p[j] = (T)v[j];
+    }
+}
+
+__device__ __forceinline__ float pow2(int k) { return __uint_as_float((unsigned)(k + 127) << 23); }
+
+template <typename T>
+__global__ __launch_bounds__(256) void act8_fwd_kernel(const T* __restrict__ u, T* __restrict__ a, unsigned char* __restrict__ q, float* __restrict__ scale, int64_t groups, int per_row,
+                                                       int cols, int act, int aligned) {
+    const int64_t g = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);     // group of 128 channels
+    if (g >= groups) return;                                             // (16 lanes at a time: the exchange below stays inside them)
+    const int64_t row = g / per_row;
+    const int c = (int)(g % per_row) * ACT8_GROUP + (threadIdx.x & 15) * 8;
+    const int n = cols - c;                                              // channels left in the row, may be <= 0
+    const bool whole = aligned && n >= 8;
+    const int64_t at = row * cols + c;
+    float v[8];
+    load8<T>(u + at, whole, n, v);
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float m = fabsf(v[j]);
+        top = fmaxf(top, m <= 3.402823466e38f ? m : 0.f);                // (false for NaN and infinity)
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    int k = 0;
+    if (top > 0.f) {
+        const unsigned b = __float_as_uint(top);
+        k = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u);     // 1.75 is the mantissa 0x600000; subnormals land below the clamp
+        k = k < -117 ? -117 : k > 120 ? 120 : k;
+    }
+    if ((threadIdx.x & 15) == 0) scale[g] = pow2(k);
+    const float inv = pow2(-k);
+    unsigned w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h] * inv, v[4 * h + 1] * inv, 0, false);
+        w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * inv, v[4 * h + 3] * inv, w[h], true);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (!(fabsf(v[4 * h + j]) <= 3.402823466e38f)) w[h] |= 0x7fu << (8 * j);
+    }
+    if (whole) {
+        const u32x2 t = {w[0], w[1]};
+        *(u32x2*)(q + at) = t;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) q[at + j] = (unsigned char)(w[j >> 2] >> (8 * (j & 3)));
+    }
+    if (a != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = act_value(v[j], act);
+        store8<T>(a + at, whole, n, v);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void act8_bwd_kernel(const unsigned char* __restrict__ q, const float* __restrict__ scale, const T* __restrict__ da, T* __restrict__ du, T* __restrict__ a,
+                                                       int64_t groups, int per_row, int cols, int act, int aligned) {
+    const int64_t g = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (g >= groups) return;
+    const int64_t row = g / per_row;
+    const int c = (int)(g % per_row) * ACT8_GROUP + (threadIdx.x & 15) * 8;
+    const int n = cols - c;
+    const bool whole = aligned && n >= 8;
+    const int64_t at = row * cols + c;
+    unsigned w[2] = {0u, 0u};
+    if (whole) {
+        const u32x2 t = *(const u32x2*)(q + at);
+        w[0] = t[0]; w[1] = t[1];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) w[j >> 2] |= (unsigned)q[at + j] << (8 * (j & 3));
+    }
+    const float s = scale[g];
+    float v[8], d[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[h], true);
+        v[4 * h] = lo[0] * s; v[4 * h + 1] = lo[1] * s;
+        v[4 * h + 2] = hi[0] * s; v[4 * h + 3] = hi[1] * s;
+    }
+    load8<T>(da + at, whole, n, d);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] *= act_slope(v[j], act);
+    store8<T>(du + at, whole, n, d);
+    if (a != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = act_value(v[j], act);
+        store8<T>(a + at, whole, n, v);
+    }
+}
+
+static bool act8_ok(int act) { return act == HH_ACT_NONE || act == HH_ACT_QUICKGELU || act == HH_ACT_RELU; }
+
+extern "C" int hh_act8_fwd(const void* u, int u_dtype, void* a, void* q, float* scale, int64_t rows, int cols, int act, hh_stream_t stream) {
+    HH_REQUIRE(rows >= 0 && cols > 0, HH_ERR_SHAPE, "hh_act8_fwd: rows=%lld cols=%d", (long long)rows, cols);
+    HH_REQUIRE(u_dtype == HH_F32 || u_dtype == HH_BF16, HH_ERR_DTYPE, "hh_act8_fwd: bad dtype");
+    HH_REQUIRE(act8_ok(act), HH_ERR_UNSUPPORTED, "hh_act8_fwd: unknown activation %d", act);
+    const int per_row = (cols + ACT8_GROUP - 1) / ACT8_GROUP;
+    const int64_t groups = rows * per_row, blocks = (groups + 15) / 16;
+    HH_REQUIRE(blocks <= 0x7fffffff, HH_ERR_SHAPE, "hh_act8_fwd: too many rows");
+    if (groups == 0) return HH_OK;
+    HH_REQUIRE(u != nullptr && q != nullptr && scale != nullptr, HH_ERR_ALIGN, "hh_act8_fwd: NULL pointer");
+    const int al = cols % 8 == 0 && HH_ALIGNED16(u) && HH_ALIGNED16(a) && (((uintptr_t)q) & 7) == 0;
+    if (u_dtype == HH_F32)
+        hipLaunchKernelGGL(act8_fwd_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const float*)u, (float*)a, (unsigned char*)q, scale, groups, per_row, cols, act, al);
+    else
+        hipLaunchKernelGGL(act8_fwd_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)u, (bf16_t*)a, (unsigned char*)q, scale, groups, per_row, cols, act, al);
+    return hh_check_launch("hh_act8_fwd");
+}
+
+extern "C" int hh_act8_bwd(const void* q, const float* scale, const void* da, void* du, void* a, int dtype, int64_t rows, int cols, int act, hh_stream_t stream) {
+    HH_REQUIRE(rows >= 0 && cols > 0, HH_ERR_SHAPE, "hh_act8_bwd: rows=%lld cols=%d", (long long)rows, cols);
+    HH_REQUIRE(dtype == HH_F32 || dtype == HH_BF16, HH_ERR_DTYPE, "hh_act8_bwd: bad dtype");
+    HH_REQUIRE(act8_ok(act), HH_ERR_UNSUPPORTED, "hh_act8_bwd: unknown activation %d", act);
+    const int per_row = (cols + ACT8_GROUP - 1) / ACT8_GROUP;
+    const int64_t groups = rows * per_row, blocks = (groups + 15) / 16;
+    HH_REQUIRE(blocks <= 0x7fffffff, HH_ERR_SHAPE, "hh_act8_bwd: too many rows");
+    if (groups == 0) return HH_OK;
+    HH_REQUIRE(q != nullptr && scale != nullptr && da != nullptr && du != nullptr, HH_ERR_ALIGN, "hh_act8_bwd: NULL pointer");
+    const int al = cols % 8 == 0 && HH_ALIGNED16(da) && HH_ALIGNED16(du) && HH_ALIGNED16(a) && (((uintptr_t)q) & 7) == 0;
+    if (dtype == HH_F32)
+        hipLaunchKernelGGL(act8_bwd_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const unsigned char*)q, scale, (const float*)da, (float*)du, (float*)a, groups, per_row, cols,
+                           act, al);
+    else
+        hipLaunchKernelGGL(act8_bwd_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const unsigned char*)q, scale, (const bf16_t*)da, (bf16_t*)du, (bf16_t*)a, groups, per_row,
+                           cols, act, al);
+    return hh_check_launch("hh_act8_bwd");
+}

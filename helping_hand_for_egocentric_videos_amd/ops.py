@@ -5,11 +5,12 @@ SURVEY.md section 8b "Error conventions"), allocates outputs as torch tensors, a
 current torch stream.  Nothing here computes on the CPU: non-GPU tensors raise.
 """
 import ctypes
+from collections import namedtuple
 
 import torch
 
 from . import _lib
-from ._lib import GemmEpilogue, QGemmOpts
+from ._lib import GemmEpilogue, QGemmOpts, ResidualNorm
 
 F32, BF16 = 0, 1
 ACT_NONE, ACT_QUICKGELU, ACT_RELU = 0, 1, 2
@@ -1007,3 +1008,229 @@ def tv_accuracy(sim, text_cos, sim_v, sim_n):
     out = torch.empty(2, dtype=torch.float32, device=sim.device)
     _lib.check(_lib.lib().hh_tv_accuracy(_p(sim), sim.stride(0), _p(text_cos), _p(sim_v), _p(sim_n), Bg, _p(out), _stream()), "hh_tv_accuracy")
     return out
+
+
+# ---- training a token stream: embedding, the end of a residual block, activation checkpoints in 8 bits --------------------------------
+def _chk_here(*tensors):
+    """_chk, and every tensor on the current device: the launch goes to that device's current stream."""
+    _chk(*tensors)
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError("libhh ops run on the current device (cuda:%d), got a tensor on %s: enter torch.cuda.device(tensor.device)" % (dev, t.device))
+
+
+def _bytes(nbytes, what, device):
+    """Scratch of `nbytes` (a hh_workspace_bytes_* result); None where none is needed."""
+    if nbytes < 0:
+        raise ValueError("%s: the library does not take these sizes" % what)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _ids_of(ids, what):
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError("%s: ids must be int64 or int32, got %s" % (what, ids.dtype))
+    if ids.dim() == 0:
+        raise ValueError("%s: ids need at least one dimension" % what)
+    length = ids.shape[-1]
+    return length, (ids.numel() // length if length else 0)
+
+
+def embed_tokens(ids, weight, scale=1.0, pos=None, out_dtype=None):
+    """scale * weight[ids] + pos  (CLIP.encode_text, LaviLa.py:660-663; include/hh.h: hh_embed_tokens_fwd).
+
+    ids int64 / int32 [..., L]; weight fp32 / bf16 [V, D]; pos fp32 [P >= L, D] or None: row t is added at index t of the last dimension (a decoding step
+    at position t passes pos[t:t + 1]).  -> out_dtype (weight's by default) [..., L, D].  An id outside [0, V) gives a row of NaN (nothing
+    can be raised without waiting for the device)."""
+    _chk_here(ids, weight, pos)
+    length, seqs = _ids_of(ids, "embed_tokens")
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError("embed_tokens: weight must be [V, D], got %s" % (tuple(weight.shape),))
+    V, D = weight.shape
+    if pos is not None and (pos.dtype != torch.float32 or pos.dim() != 2 or pos.shape[1] != D or pos.shape[0] < length):
+        raise ValueError("embed_tokens: pos must be fp32 [>= %d, %d], got %s %s" % (length, D, pos.dtype, tuple(pos.shape)))
+    out = torch.empty((*ids.shape, D), dtype=weight.dtype if out_dtype is None else out_dtype, device=weight.device)
+    wd, od = _dt(weight), _dt(out)
+    if out.numel() == 0:
+        return out
+    _lib.check(_lib.lib().hh_embed_tokens_fwd(_p(ids), ids.element_size(), _p(weight), wd, _p(pos), _p(out), od, seqs, length, V, D, float(scale), _stream()),
+               "hh_embed_tokens_fwd")
+    return out
+
+
+def embed_tokens_bwd(ids, dy, num_rows, scale=1.0, skip_id=None, pos_grad=False, out=None):
+    """Gradients of embed_tokens: dweight fp32 [num_rows, D] with dweight[v] = scale * the sum of dy over the places whose id is v, and with pos_grad also
+    dpos fp32 [L, D] = dy summed over the sequences -> dweight or (dweight, dpos)   (include/hh.h: hh_embed_tokens_bwd).
+
+    ids int64 / int32 [..., L], dy fp32 / bf16 [..., L, D].  skip_id: an id without a gradient (nn.Embedding's padding_idx); ids outside [0, num_rows) have
+    none either.  out: a fp32 [num_rows, D] buffer that the gradient is ACCUMULATED into (a parameter's slice of the gradient arena), a fresh one by
+    default.  Equal inputs give equal bits (the ids are sorted, no floating-point atomics)."""
+    _chk_here(ids, dy, out)
+    length, seqs = _ids_of(ids, "embed_tokens_bwd")
+    if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] == 0:
+        raise ValueError("embed_tokens_bwd: dy must be ids' shape and a last dimension D, got %s for ids %s" % (tuple(dy.shape), tuple(ids.shape)))
+    V, D = int(num_rows), dy.shape[-1]
+    if out is not None and (out.dtype != torch.float32 or tuple(out.shape) != (V, D)):
+        raise ValueError("embed_tokens_bwd: out must be fp32 [%d, %d]" % (V, D))
+    dd = _dt(dy)
+    L = _lib.lib()
+    ws = _bytes(L.hh_workspace_bytes_embed_tokens_bwd(seqs, max(length, 1), V, D), "embed_tokens_bwd", dy.device)
+    dw = torch.empty((V, D), dtype=torch.float32, device=dy.device) if out is None else out
+    dpos = torch.empty((length, D), dtype=torch.float32, device=dy.device) if pos_grad else None
+    _lib.check(L.hh_embed_tokens_bwd(_p(ids), ids.element_size(), _p(dy), dd, _p(dw), int(out is not None), _p(dpos) if length else None, seqs, max(length, 1), V, D,
+                                     float(scale), -1 if skip_id is None else int(skip_id), _p(ws), _stream()), "hh_embed_tokens_bwd")
+    return (dw, dpos) if pos_grad else dw
+
+
+GATE_NONE, GATE_SCALAR, GATE_CHANNEL, GATE_GROUP = 0, 1, 2, 3          # include/hh.h: enum hh_gate_kind
+ResidualNormGrads = namedtuple("ResidualNormGrads", "dx dy dgate dpost_gamma dpost_beta dpre_gamma dpre_beta")
+
+
+def _residual_norm_desc(what, x, y, gate, gate_tanh, res_scale, post, pre, rms):
+    cols = x.shape[-1] if x.dim() else 0
+    if cols == 0 or y.shape != x.shape:
+        raise ValueError("%s: stream and branch must have one shape [..., cols], got %s and %s" % (what, tuple(x.shape), tuple(y.shape)))
+    d = ResidualNorm()
+    d.rows, d.groups, d.cols = x.numel() // cols, 1, cols
+    d.x_dtype, d.y_dtype, d.h_dtype = _dt(x), _dt(y), F32
+    d.rms, d.res_scale, d.gate_tanh = int(bool(rms)), float(res_scale), int(bool(gate_tanh))
+    d.y = y.data_ptr()
+    if gate is not None:
+        if gate.dtype != torch.float32:
+            raise TypeError("%s: the gate must be fp32" % what)
+        if gate.dim() == 2 and gate.shape[1] == cols:
+            d.gate_kind, d.groups = (GATE_GROUP, gate.shape[0]) if gate.shape[0] != 1 else (GATE_CHANNEL, 1)
+            if d.groups == 0 or d.rows % d.groups:
+                raise ValueError("%s: %d rows do not split into %d gate groups" % (what, d.rows, d.groups))
+        elif gate.numel() == 1:
+            d.gate_kind = GATE_SCALAR
+        elif gate.dim() == 1 and gate.numel() == cols:
+            d.gate_kind = GATE_CHANNEL
+        else:
+            raise ValueError("%s: the gate must hold one value, [cols] or [groups, cols], got %s" % (what, tuple(gate.shape)))
+        d.gate = gate.data_ptr()
+    for name, norm in (("post", post), ("pre", pre)):
+        if norm is None:
+            continue
+        gamma, beta, eps = norm
+        for v in (gamma, beta):
+            if v is not None and (v.dtype != torch.float32 or v.numel() != cols):
+                raise ValueError("%s: %s norm's gamma / beta must be fp32 [%d]" % (what, name, cols))
+        setattr(d, name + "_gamma", gamma.data_ptr())
+        setattr(d, name + "_beta", beta.data_ptr() if beta is not None else None)
+        setattr(d, name + "_eps", float(eps))
+    return d
+
+
+def _norm_tensors(post, pre):
+    return [t for n in (post, pre) if n is not None for t in n[:2]]
+
+
+def residual_norm(x, y, *, gate=None, gate_tanh=False, res_scale=1.0, post=None, pre=None, rms=False, out_dtype=torch.bfloat16, out=None):
+    """The end of a residual block in one pass (include/hh.h: hh_residual_norm_fwd):
+        x_new = res_scale * x + g * post(y),   h = pre(x_new)   ->  (x_new, h); h is None without `pre`.
+
+    x, y fp32 / bf16 [..., cols], x_new like x, h of out_dtype.  post / pre: (gamma, beta or None, eps) of a norm (fp32 [cols]) or None; rms: root-mean-square norms
+    instead of LayerNorms.  gate fp32, through tanh with gate_tanh: one value, [cols], or [groups, cols] for `groups` groups of consecutive rows (a
+    clip's, a caption's).  out: x_new's buffer, may be x itself (the stream updated in place)."""
+    _chk_here(x, y, gate, out, *_norm_tensors(post, pre))
+    d = _residual_norm_desc("residual_norm", x, y, gate, gate_tanh, res_scale, post, pre, rms)
+    if out is not None and (out.dtype != x.dtype or out.shape != x.shape):
+        raise ValueError("residual_norm: out must have x's shape and type")
+    x_new = torch.empty_like(x) if out is None else out
+    h = None
+    if pre is not None:
+        h = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        d.h_dtype, d.h = _dt(h), h.data_ptr()
+    d.x, d.x_new = x.data_ptr(), x_new.data_ptr()
+    _lib.check(_lib.lib().hh_residual_norm_fwd(ctypes.byref(d), _stream()), "hh_residual_norm_fwd")
+    return x_new, h
+
+
+def residual_norm_bwd(x_new, y, dx_new=None, dh=None, *, gate=None, gate_tanh=False, res_scale=1.0, post=None, pre=None, rms=False):
+    """Gradients of residual_norm from its x_new and y and the gradients of x_new (None: zeros) and of h (with `pre`) -> ResidualNormGrads: dx like x_new, dy like
+    y, and fp32 dgate (the gate's shape), dpost_gamma, dpost_beta, dpre_gamma, dpre_beta, None where the parameter is (include/hh.h: hh_residual_norm_bwd)."""
+    _chk_here(x_new, y, dx_new, dh, gate, *_norm_tensors(post, pre))
+    d = _residual_norm_desc("residual_norm_bwd", x_new, y, gate, gate_tanh, res_scale, post, pre, rms)
+    if (dh is None) != (pre is None):
+        raise ValueError("residual_norm_bwd: dh comes with pre")
+    if dx_new is not None and (dx_new.dtype != x_new.dtype or dx_new.shape != x_new.shape):
+        raise ValueError("residual_norm_bwd: dx_new must have x_new's shape and type")
+    if dh is not None:
+        if dh.shape != x_new.shape:
+            raise ValueError("residual_norm_bwd: dh must have x_new's shape")
+        d.h_dtype, d.dh = _dt(dh), dh.data_ptr()
+    dev = x_new.device
+    dx, dy = torch.empty_like(x_new), torch.empty_like(y)
+    grads = [None if t is None else torch.empty_like(t) for t in (gate, *(post[:2] if post is not None else (None, None)), *(pre[:2] if pre is not None else (None, None)))]
+    d.x_new, d.dx_new, d.dx, d.dy = x_new.data_ptr(), dx_new.data_ptr() if dx_new is not None else None, dx.data_ptr(), dy.data_ptr()
+    d.dgate, d.dpost_gamma, d.dpost_beta, d.dpre_gamma, d.dpre_beta = (None if t is None else t.data_ptr() for t in grads)
+    L = _lib.lib()
+    ws = _bytes(L.hh_workspace_bytes_residual_norm_bwd(d.rows, d.cols, d.groups), "residual_norm_bwd", dev)
+    d.workspace = ws.data_ptr() if ws is not None else None
+    _lib.check(L.hh_residual_norm_bwd(ctypes.byref(d), _stream()), "hh_residual_norm_bwd")
+    return ResidualNormGrads(dx, dy, *grads)
+
+
+ACT8_GROUP = 128                                                       # channels that share a scale
+
+
+def _chk_act8(q, scale, what):
+    if q.dtype != torch.float8_e4m3fn or q.dim() != 2 or q.shape[1] == 0:
+        raise TypeError("%s: q must be float8_e4m3fn [rows, cols] (act8's), got %s %s" % (what, q.dtype, tuple(q.shape)))
+    if scale.dtype != torch.float32 or tuple(scale.shape) != (q.shape[0], -(-q.shape[1] // ACT8_GROUP)):
+        raise TypeError("%s: scale must be fp32 [rows, ceil(cols / 128)] (act8's), got %s %s" % (what, scale.dtype, tuple(scale.shape)))
+
+
+def act8(u, act=ACT_NONE, want_out=True):
+    """An activation and its 8-bit checkpoint in one pass (include/hh.h: hh_act8_fwd): -> (a = act(u) like u or None, q float8_e4m3fn, scale fp32).
+    u fp32 / bf16 [rows, cols]; u ~ q * scale with one power of two for every 128 channels (q.float() * scale.repeat_interleave(128, 1)[:, :cols] has the
+    values): 1.03 bytes for an element that a backward pass would keep in 2 or 4.  want_out=False: the checkpoint alone (the input of a linear layer)."""
+    _chk_here(u)
+    if u.dim() != 2 or u.shape[1] == 0:
+        raise ValueError("act8: u must be [rows, cols], got %s" % (tuple(u.shape),))
+    dt = _dt(u)
+    rows, cols = u.shape
+    a = torch.empty_like(u) if want_out else None
+    q = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=u.device)
+    scale = torch.empty((rows, -(-cols // ACT8_GROUP)), dtype=torch.float32, device=u.device)
+    _lib.check(_lib.lib().hh_act8_fwd(_p(u), dt, _p(a), _p(q), _p(scale), rows, cols, int(act), _stream()), "hh_act8_fwd")
+    return a, q, scale
+
+
+def act8_bwd(q, scale, da, act, want_out=False):
+    """du = da * act'(v) with v = q * scale, the values of act8's checkpoint (include/hh.h: hh_act8_bwd) -> du like da; with want_out (du, act(v)): the
+    activation again, the operand of the next layer's weight gradient."""
+    _chk_here(q, scale, da)
+    _chk_act8(q, scale, "act8_bwd")
+    if da.shape != q.shape:
+        raise ValueError("act8_bwd: da must have q's shape")
+    dt = _dt(da)
+    du = torch.empty_like(da)
+    a = torch.empty_like(da) if want_out else None
+    _lib.check(_lib.lib().hh_act8_bwd(_p(q), _p(scale), _p(da), _p(du), _p(a), dt, q.shape[0], q.shape[1], int(act), _stream()), "hh_act8_bwd")
+    return (du, a) if want_out else du
+
+
+def gemm_tn_act8(dy, q, scale, colsum=False, out=None):
+    """Weight gradient from an 8-bit checkpoint: dy bf16 [K, M], (q, scale) = act8's of the layer's input [K, N] -> fp32 [M, N] = dy^T @ (q * scale), written
+    into `out` when given; colsum=True also returns sum_k dy[k, :] (fp32 [M]: the bias gradient)   (include/hh.h: hh_gemm_tn_act8).  dy and q may be
+    row-strided views with unit inner stride; any K, M, N."""
+    for t in (dy, q):
+        if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError("gemm_tn_act8: dy and q must be 2-D with unit inner stride and rows that do not overlap")
+    _chk_here(scale, out, dy[:0], q[:0])
+    _chk_act8(q, scale, "gemm_tn_act8")
+    K, M = dy.shape
+    N = q.shape[1]
+    if dy.dtype != torch.bfloat16 or q.shape[0] != K or M == 0:
+        raise ValueError("gemm_tn_act8: dy must be bf16 [%d, M], got %s %s" % (q.shape[0], dy.dtype, tuple(dy.shape)))
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.float32, device=dy.device)
+    elif out.dtype != torch.float32 or tuple(out.shape) != (M, N):
+        raise ValueError("gemm_tn_act8: out must be fp32 [%d, %d]" % (M, N))
+    db = torch.empty((M,), dtype=torch.float32, device=dy.device) if colsum else None
+    L = _lib.lib()
+    ws = _bytes(L.hh_workspace_bytes_gemm_tn_act8(M, N, K), "gemm_tn_act8", dy.device)
+    _lib.check(L.hh_gemm_tn_act8(_p(dy), dy.stride(0) if K > 1 else M, _p(q), q.stride(0) if K > 1 else N, _p(scale), _p(out), _p(db), M, N, K, _p(ws), _stream()), "hh_gemm_tn_act8")
+    return (out, db) if colsum else out

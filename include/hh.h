@@ -497,6 +497,69 @@ int hh_adamw_arena_step(float* p, float* g, float* m, float* v, int64_t n, const
                         int* seg_step, const float* seg_flag, float* seg_coef, int n_seg, float lr, float beta1, float beta2,
                         float eps, float weight_decay, int zero_grads, hh_stream_t stream);
 
+/* ---- token embedding and its gradients (CLIP.encode_text: model/LaviLa.py:660-663; the gradient is what autograd's index_add does there)
+ *   out[s,t,:] = scale * weight[ids[s,t],:] + pos[t,:]          ids [seqs, length] of id_bytes = 4 or 8; pos fp32 [length, dim] or NULL
+ *   dweight[v,:] (+)= scale * sum over ids[s,t] == v of dy[s,t,:]      dpos[t,:] = sum_s dy[s,t,:] (or NULL)
+ * An id outside [0, rows) gives a row of NaN forward and no gradient; neither does skip_id (pass -1 for none), like nn.Embedding's padding_idx.
+ * accumulate != 0: dweight is added to and untouched where no id points; 0: written whole.  The gradient sorts the ids and adds equal rows in the
+ * order of their positions, without floating-point atomics: equal inputs give equal bits.  dim and the pointers' alignment are free (dim % 4 == 0 and 16
+ * bytes take wide accesses); dim <= 2^20, seqs * length < 2^30, rows < 2^31. */
+int hh_embed_tokens_fwd(const void* ids, int id_bytes, const void* weight, int w_dtype, const float* pos, void* out, int out_dtype, int64_t seqs, int length, int64_t rows,
+                        int dim, float scale, hh_stream_t stream);
+int64_t hh_workspace_bytes_embed_tokens_bwd(int64_t seqs, int length, int64_t rows, int dim);
+int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy, int dy_dtype, float* dweight, int accumulate, float* dpos, int64_t seqs, int length, int64_t rows,
+                        int dim, float scale, int64_t skip_id, void* workspace, hh_stream_t stream);
+
+/* ---- the end of a residual block: norms before and after, gate and residual scale in one pass over the rows
+ *   p = post(y),  x_new = res_scale * x + g o p,  h = pre(x_new);   post / pre: LayerNorm (rms = 0) or root-mean-square norm with gamma and an
+ *   optional beta, or the identity (gamma NULL; without pre there is no h);  g: 1, gate[0], gate[cols], or gate[group, cols] for `groups` groups of
+ *   consecutive rows, through tanh with gate_tanh (the tanh gate of SpaceTimeBlock, model/LaviLa.py:305-390, is the scalar one).
+ * x, x_new, dx_new, dx have x_dtype, y, dy y_dtype, h, dh h_dtype; parameters and their gradients are fp32.  x_new may be x.
+ * hh_residual_norm_bwd reads x_new, y, dx_new (NULL: zeros) and dh (with pre) and writes dx, dy and the gradients of the parameters that there are
+ * (dpost_beta / dpre_beta may be NULL); dx may be dx_new.  No floating-point atomics.  cols <= 4096, any alignment (cols % 4 == 0 and 16 bytes take
+ * wide accesses); groups <= 65000 and rows % groups == 0. */
+enum hh_gate_kind { HH_GATE_NONE = 0, HH_GATE_SCALAR = 1, HH_GATE_CHANNEL = 2, HH_GATE_GROUP = 3 };
+typedef struct hh_residual_norm {
+    int64_t rows, groups;
+    int32_t cols, x_dtype, y_dtype, h_dtype, gate_kind, gate_tanh, rms;
+    float res_scale, post_eps, pre_eps;
+    const float* gate;
+    const float* post_gamma;
+    const float* post_beta;
+    const float* pre_gamma;
+    const float* pre_beta;
+    const void* x;            /* forward */
+    const void* y;
+    void* x_new;              /* forward: output; backward: input */
+    void* h;
+    const void* dx_new;       /* backward */
+    const void* dh;
+    void* dx;
+    void* dy;
+    float* dgate;
+    float* dpost_gamma;
+    float* dpost_beta;
+    float* dpre_gamma;
+    float* dpre_beta;
+    void* workspace;          /* backward: hh_workspace_bytes_residual_norm_bwd bytes */
+} hh_residual_norm;
+int hh_residual_norm_fwd(const hh_residual_norm* d, hh_stream_t stream);
+int64_t hh_workspace_bytes_residual_norm_bwd(int64_t rows, int cols, int64_t groups);
+int hh_residual_norm_bwd(const hh_residual_norm* d, hh_stream_t stream);
+
+/* ---- activation checkpoints in 8 bits
+ * hh_act8_fwd: a = act(u) (NULL: not wanted), q = e4m3(u / s) [rows, cols], scale = s = 2^k fp32 [rows, ceil(cols / 128)]: k is the smallest whole number in
+ *   [-117, 120] with max |u| <= 448 * 2^k over the 128 channels (0 where all are zero; infinities and NaN do not count and are stored as NaN).
+ * hh_act8_bwd: v = q * s, du = da * act'(v), a = act(v) (NULL: not wanted); da, du and a have `dtype`.
+ * hh_gemm_tn_act8: dw fp32 [M, N] = dy^T (q * s) and db fp32 [M] = sum_k dy[k,:] (or NULL) over K tokens, dy bf16 [K, M] (ld_dy), q [K, N] (ldq), scale
+ *   [K, ceil(N / 128)] whose entries are powers of two; q * s is exact in the matrix core's bf16, sums are fp32 and in a fixed order.  dw: 16-byte aligned.
+ * act: HH_ACT_NONE, HH_ACT_QUICKGELU, HH_ACT_RELU.  Any cols / M / N / K and alignment. */
+int hh_act8_fwd(const void* u, int u_dtype, void* a, void* q, float* scale, int64_t rows, int cols, int act, hh_stream_t stream);
+int hh_act8_bwd(const void* q, const float* scale, const void* da, void* du, void* a, int dtype, int64_t rows, int cols, int act, hh_stream_t stream);
+int64_t hh_workspace_bytes_gemm_tn_act8(int M, int N, int64_t K);
+int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int64_t ldq, const float* scale, float* dw, float* db, int M, int N, int64_t K, void* workspace,
+                    hh_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
