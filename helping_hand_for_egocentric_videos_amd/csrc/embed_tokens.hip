@@ -99,17 +99,18 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__
 }
 
 // ---- the sort: least significant digit first, stable, two launches for each digit --------------------------------------------------------
+#define SORT_THREADS 1024
 #define SORT_BLOCKS 256                              // at most: a block's share of the list grows with it
 
 struct SortPass { int shift, bits; };
-struct SortPlan { int blocks, per_block, passes; SortPass pass[4]; };
+struct SortPlan { int blocks, passes; int64_t per_block; SortPass pass[4]; };
 
 static SortPlan sort_plan(int64_t n, int64_t rows) {
     SortPlan p;
-    p.blocks = (int)((n + 1023) / 1024);
-    if (p.blocks > SORT_BLOCKS) p.blocks = SORT_BLOCKS;
-    if (p.blocks < 1) p.blocks = 1;
-    p.per_block = (int)(((n + p.blocks - 1) / p.blocks + 255) / 256 * 256);
+    int64_t blocks = (n + SORT_THREADS - 1) / SORT_THREADS;
+    if (blocks > SORT_BLOCKS) blocks = SORT_BLOCKS;
+    p.blocks = (int)(blocks < 1 ? 1 : blocks);
+    p.per_block = ((n + p.blocks - 1) / p.blocks + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;
     int bits = 1;
     while ((rows >> bits) != 0) ++bits;              // keys 0 .. rows (rows = "no row")
     p.passes = (bits + 7) / 8;
@@ -122,15 +123,31 @@ static SortPlan sort_plan(int64_t n, int64_t rows) {
     return p;
 }
 
+// A fresh gradient's zeros ride along: the sort keeps few CUs busy and waits for latencies, so that each of its launches carries, in the workgroups
+// behind its own, an equal part of the fill (152 MB for 49 408 x 768: 20 us at the card's 6.9 TB/s of a fill alone, spread over four launches here).
+struct ZeroPart { float* p; int64_t begin, end; int wide; };
+
+__device__ __forceinline__ void zero_part(const ZeroPart& z, int block, int blocks) {
+    const int64_t first = z.begin + ((int64_t)block * SORT_THREADS + threadIdx.x) * (z.wide ? 4 : 1);
+    const int64_t stride = (int64_t)blocks * SORT_THREADS * (z.wide ? 4 : 1);
+    if (z.wide) {                                    // begin, end: multiples of 4
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t i = first; i < z.end; i += stride) *(f32x4*)(z.p + i) = zero;
+    } else {
+        for (int64_t i = first; i < z.end; i += stride) z.p[i] = 0.f;
+    }
+}
+
 // counts of one digit in a block's share; the first pass also turns ids into keys (no row: `rows`, which sorts behind all others)
-__global__ __launch_bounds__(256) void sort_count_kernel(const void* __restrict__ ids, int wide, int64_t rows, int64_t skip, u32* __restrict__ keys, u32* __restrict__ hist, int n,
-                                                         int per_block, int shift, int bits) {
+__global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const void* __restrict__ ids, int wide, int64_t rows, int64_t skip, u32* __restrict__ keys, u32* __restrict__ hist, int n,
+                                                                  int64_t per_block, int shift, int bits, int sort_blocks, ZeroPart z) {
+    if ((int)blockIdx.x >= sort_blocks) { zero_part(z, blockIdx.x - sort_blocks, gridDim.x - sort_blocks); return; }
     __shared__ u32 count[256];
-    count[threadIdx.x] = 0;
+    if (threadIdx.x < 256) count[threadIdx.x] = 0;
     __syncthreads();
-    const int64_t b0 = (int64_t)blockIdx.x * per_block;
+    const int64_t b0 = blockIdx.x * per_block;
     const int64_t b1 = b0 + per_block < n ? b0 + per_block : n;
-    for (int64_t i = b0 + threadIdx.x; i < b1; i += 256) {
+    for (int64_t i = b0 + threadIdx.x; i < b1; i += SORT_THREADS) {
         u32 key;
         if (ids) {
             const int64_t id = load_id(ids, wide, i);
@@ -142,35 +159,54 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const void* __restrict_
         atomicAdd(&count[(key >> shift) & ((1u << bits) - 1)], 1u);
     }
     __syncthreads();
-    hist[(int64_t)blockIdx.x * 256 + threadIdx.x] = count[threadIdx.x];
+    if (threadIdx.x < 256) hist[(int64_t)blockIdx.x * 256 + threadIdx.x] = count[threadIdx.x];
 }
 
 // places a block's share behind the smaller digits and behind the earlier blocks' equal ones; `from`: NULL on the first pass (position i)
-__global__ __launch_bounds__(256) void sort_place_kernel(const u32* __restrict__ keys, const u32* __restrict__ from, const u32* __restrict__ hist, u32* __restrict__ keys_out,
-                                                         u32* __restrict__ from_out, int n, int per_block, int shift, int bits) {
-    __shared__ u32 base[256], wcount[4][256], part[4];
+__global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const u32* __restrict__ keys, const u32* __restrict__ from, const u32* __restrict__ hist, u32* __restrict__ keys_out,
+                                                                  u32* __restrict__ from_out, int n, int64_t per_block, int shift, int bits, int sort_blocks, ZeroPart z) {
+    if ((int)blockIdx.x >= sort_blocks) { zero_part(z, blockIdx.x - sort_blocks, gridDim.x - sort_blocks); return; }
+    __shared__ u32 base[256], wcount[16][256], sums[4][2][256], part[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    u32 before = 0, total = 0;
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-        const u32 h = hist[(int64_t)b * 256 + tid];
-        if (b < (int)blockIdx.x) before += h;
-        total += h;
-    }
-    u32 incl = total;                                // digits below `tid`: inclusive scan over the wave, then over the four waves
+    {   // digit tid & 255: its count in all blocks and in the earlier ones; four threads take every fourth block, eight loads in flight
+        const int d = tid & 255, q = tid >> 8;
+        u32 before = 0, total = 0;
+        for (int b = q; b < sort_blocks; b += 32) {
+            u32 h[8];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u32 t = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += t;
+            for (int i = 0; i < 8; ++i) h[i] = b + 4 * i < sort_blocks ? hist[(int64_t)(b + 4 * i) * 256 + d] : 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                total += h[i];
+                if (b + 4 * i < (int)blockIdx.x) before += h[i];
+            }
+        }
+        sums[q][0][d] = total;
+        sums[q][1][d] = before;
     }
-    if (lane == 63) part[wave] = incl;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) incl += part[w];
-    base[tid] = incl - total + before;
-    const int64_t b0 = (int64_t)blockIdx.x * per_block;
-    const int64_t b1 = b0 + per_block < n ? b0 + per_block : n;
-    for (int64_t r = b0; r < b1; r += 256) {
+    u32 total = 0, before = 0, incl = 0;
+    if (tid < 256) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) wcount[w][tid] = 0;
+        for (int q = 0; q < 4; ++q) { total += sums[q][0][tid]; before += sums[q][1][tid]; }
+        incl = total;                                // smaller digits: inclusive scan over the wave, then over the four waves
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const u32 t = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += t;
+        }
+        if (lane == 63) part[wave] = incl;
+    }
+    __syncthreads();
+    if (tid < 256) {
+        for (int w = 0; w < wave; ++w) incl += part[w];
+        base[tid] = incl - total + before;
+    }
+    const int64_t b0 = blockIdx.x * per_block;
+    const int64_t b1 = b0 + per_block < n ? b0 + per_block : n;
+    for (int64_t r = b0; r < b1; r += SORT_THREADS) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ((u32*)wcount)[tid + SORT_THREADS * i] = 0;
         __syncthreads();
         const int64_t i = r + tid;
         const bool valid = i < b1;
@@ -184,97 +220,178 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const u32* __restrict__
         const u32 rank = (u32)__popcll(same & ((1ull << lane) - 1));
         if (valid && rank == 0) wcount[wave][digit] = (u32)__popcll(same);
         __syncthreads();
+        if (tid < 256) {                             // counts -> places of the waves, in wave order
+            u32 at = base[tid];
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                const u32 c = wcount[w][tid];
+                wcount[w][tid] = at;
+                at += c;
+            }
+            base[tid] = at;
+        }
+        __syncthreads();
         if (valid) {
-            u32 at = base[digit] + rank;
-            for (int w = 0; w < wave; ++w) at += wcount[w][digit];
+            const u32 at = wcount[wave][digit] + rank;
             keys_out[at] = key;
             from_out[at] = from ? from[i] : (u32)i;
         }
         __syncthreads();
-        base[tid] += wcount[0][tid] + wcount[1][tid] + wcount[2][tid] + wcount[3][tid];
     }
 }
 
 // ---- the sums over runs of equal keys ----------------------------------------------------------------------------------------------------
-struct RunParams {
+enum { RUN_ENDS = 0, RUN_STARTS = 1, RUN_COVERS = 2 };   // nothing; a run that starts in the chunk; one that began before it
+struct RunList {
     const u32* keys; const u32* from;                // sorted keys and the positions they came from; keys == NULL: the list of dpos, see run_key
-    const void* dy;
     float* out;                                      // [rows, dim]
     float* part;                                     // [chunks][2][dim]: a chunk's first run where it began earlier, its last where it goes on
-    int n, chunk, dim, accumulate, aligned;
-    int length, seqs;                                // dpos: entry j is row t = j / seqs of the sequence j % seqs
+    u32* flags;                                      // [chunks]: what crosses the border behind the chunk
     int64_t rows;
+    int accumulate, aligned;
     float scale;
 };
-__device__ __forceinline__ u32 run_key(const RunParams& p, int j) { return p.keys ? p.keys[j] : (u32)(j / p.seqs); }
-__device__ __forceinline__ int64_t run_from(const RunParams& p, int j) { return p.keys ? (int64_t)p.from[j] : (int64_t)(j % p.seqs) * p.length + j / p.seqs; }
+struct RunParams {
+    RunList list[2];                                 // dweight, and dpos if there is one
+    const void* dy;
+    int n, chunk, chunks, dim, length, seqs;         // dpos: entry j is row t = j / seqs of the sequence j % seqs
+};
+__device__ __forceinline__ u32 run_key(const RunParams& p, const RunList& l, int j) { return l.keys ? l.keys[j] : (u32)(j / p.seqs); }
+__device__ __forceinline__ int64_t run_from(const RunParams& p, const RunList& l, int j) { return l.keys ? (int64_t)l.from[j] : (int64_t)(j % p.seqs) * p.length + j / p.seqs; }
 
-__device__ __forceinline__ void put_row(const RunParams& p, u32 key, int c, bool whole, fvec<4> v) {
-    float* o = p.out + (int64_t)key * p.dim + c;
+template <int E>
+__device__ __forceinline__ void put_row(const RunParams& p, const RunList& l, u32 key, int c, bool whole, fvec<E> v) {
+    float* o = l.out + (int64_t)key * p.dim + c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v.v[i] *= p.scale;
-    if (p.accumulate) {
-        const fvec<4> t = load_e<4, float>(o, whole, p.dim - c);
+    for (int i = 0; i < E; ++i) v.v[i] *= l.scale;
+    if (l.accumulate) {
+        const fvec<E> t = load_e<E, float>(o, whole, p.dim - c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v.v[i] += t.v[i];
+        for (int i = 0; i < E; ++i) v.v[i] += t.v[i];
     }
-    store_e<4, float>(o, v, whole, p.dim - c);
+    store_e<E, float>(o, v, whole, p.dim - c);
 }
 
-template <typename T>
+// blockIdx.x: a chunk of the list blockIdx.z;  eight rows are requested before the first is added (the gather's latency is what there is to hide)
+template <typename T, int E>
 __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
-    const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+    const RunList& l = p.list[blockIdx.z];
+    const int c = (blockIdx.y * 256 + threadIdx.x) * E;
     if (c >= p.dim) return;
-    const bool whole = p.aligned && c + 4 <= p.dim;
+    const bool whole = l.aligned && c + E <= p.dim;
     const int j0 = blockIdx.x * p.chunk, j1 = j0 + p.chunk < p.n ? j0 + p.chunk : p.n;
-    u32 key = run_key(p, j0);
-    bool head = j0 > 0 && run_key(p, j0 - 1) == key;  // this run began in an earlier chunk
-    fvec<4> acc = {{0.f, 0.f, 0.f, 0.f}};
-    for (int j = j0; j < j1 && (int64_t)key < p.rows; ++j) {
-        const fvec<4> v = load_e<4, T>((const T*)p.dy + run_from(p, j) * p.dim + c, whole, p.dim - c);
+    u32 key = run_key(p, l, j0);
+    bool head = j0 > 0 && run_key(p, l, j0 - 1) == key;          // this run began in an earlier chunk
+    fvec<E> acc;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc.v[i] += v.v[i];
-        const bool last = j + 1 == p.n;
-        const u32 next = last ? 0 : run_key(p, j + 1);
-        if (!last && next == key && j + 1 < j1) continue;
-        const bool goes_on = !last && next == key;
-        if (head) store_e<4, float>(p.part + ((int64_t)blockIdx.x * 2) * p.dim + c, acc, whole, p.dim - c);
-        else if (goes_on) store_e<4, float>(p.part + ((int64_t)blockIdx.x * 2 + 1) * p.dim + c, acc, whole, p.dim - c);
-        else put_row(p, key, c, whole, acc);
-        acc = fvec<4>{{0.f, 0.f, 0.f, 0.f}};
-        head = false;
-        if (!last) key = next;
+    for (int i = 0; i < E; ++i) acc.v[i] = 0.f;
+    float* part = l.part + (int64_t)blockIdx.x * 2 * p.dim + c;
+    if (c == 0) {
+        const u32 at_end = run_key(p, l, j1 - 1);
+        const bool cross = j1 < p.n && (int64_t)at_end < l.rows && run_key(p, l, j1) == at_end;
+        l.flags[blockIdx.x] = !cross ? RUN_ENDS : head && key == at_end ? RUN_COVERS : RUN_STARTS;
+    }
+    for (int j = j0; j < j1 && (int64_t)key < l.rows; j += 8) {
+        fvec<E> v[8];
+        u32 next[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = j + i < j1 ? j + i : j1 - 1;              // (behind the chunk: its last row once more, not added)
+            v[i] = load_e<E, T>((const T*)p.dy + run_from(p, l, at) * p.dim + c, whole, p.dim - c);
+            next[i] = at + 1 < p.n ? run_key(p, l, at + 1) : ~0u;   // (~0: no key is that large)
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (j + i < j1 && (int64_t)key < l.rows) {
+#pragma unroll
+                for (int k = 0; k < E; ++k) acc.v[k] += v[i].v[k];
+                if (next[i] != key || j + i + 1 == j1) {
+                    if (head) store_e<E, float>(part, acc, whole, p.dim - c);
+                    else if (next[i] == key) store_e<E, float>(part + p.dim, acc, whole, p.dim - c);
+                    else put_row<E>(p, l, key, c, whole, acc);
+#pragma unroll
+                    for (int k = 0; k < E; ++k) acc.v[k] = 0.f;
+                    head = false;
+                    key = next[i];
+                }
+            }
+        }
     }
 }
 
-// a run that starts in chunk b and goes on: its part of chunk b and of the chunks behind, added in that order
-__global__ __launch_bounds__(256) void run_join_kernel(RunParams p) {
-    const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
-    const int b = blockIdx.x;
-    const int j1 = (b + 1) * p.chunk;
-    if (c >= p.dim || j1 >= p.n) return;
-    const u32 key = run_key(p, j1);
-    if ((int64_t)key >= p.rows || run_key(p, j1 - 1) != key) return;           // nothing crosses this border
-    const int j0 = b * p.chunk;
-    if (j0 > 0 && run_key(p, j0) == key && run_key(p, j0 - 1) == key) return;   // it began before this chunk
-    const bool whole = p.aligned && c + 4 <= p.dim;
-    fvec<4> acc = load_e<4, float>(p.part + ((int64_t)b * 2 + 1) * p.dim + c, whole, p.dim - c);
-    for (int k = b + 1; (int64_t)k * p.chunk < p.n && run_key(p, k * p.chunk) == key; ++k) {
-        const fvec<4> v = load_e<4, float>(p.part + ((int64_t)k * 2) * p.dim + c, whole, p.dim - c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc.v[i] += v.v[i];
+// The runs that cross borders between chunks: for each, its part of the chunk that it starts in and of the chunks behind.  A wave takes a border (and 256
+// channels, blockIdx.y): where a run starts in its chunk and goes on into at most JOIN_LIGHT chunks, it adds them by itself, all loads in flight; longer
+// runs are left to all 16 waves of the workgroup, which take every 16th chunk each and are added in wave order.
+#define JOIN_LIGHT 8
+__global__ __launch_bounds__(1024) void run_join_kernel(RunParams p) {
+    __shared__ int heavy[16];
+    __shared__ float buf[16][256];
+    const RunList& l = p.list[blockIdx.z];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int c = (blockIdx.y * 64 + lane) * 4;
+    const bool mine = c < p.dim, whole = l.aligned && c + 4 <= p.dim;
+    const int b = blockIdx.x * 16 + wave;
+    int heads = 0;                                               // chunks b + 1 .. b + heads belong to the run that starts in chunk b
+    if (b < p.chunks && l.flags[b] == RUN_STARTS) {
+        for (int k = b + 1;; k += 64) {
+            const uint64_t g = __ballot(k + lane < p.chunks && l.flags[k + lane] == RUN_COVERS);
+            if (~g != 0) { heads += __builtin_ctzll(~g) + 1; break; }
+            heads += 64;
+        }
     }
-    put_row(p, key, c, whole, acc);
+    if (lane == 0) heavy[wave] = heads > JOIN_LIGHT ? heads : 0;
+    if (heads > 0 && heads <= JOIN_LIGHT && mine) {
+        const float* rest = l.part + ((int64_t)b + 1) * 2 * p.dim + c;
+        fvec<4> acc = load_e<4, float>(rest - p.dim, whole, p.dim - c);
+        fvec<4> v[JOIN_LIGHT];
+#pragma unroll
+        for (int u = 0; u < JOIN_LIGHT; ++u)
+            if (u < heads) v[u] = load_e<4, float>(rest + (int64_t)u * 2 * p.dim, whole, p.dim - c);
+#pragma unroll
+        for (int u = 0; u < JOIN_LIGHT; ++u)
+            if (u < heads)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc.v[e] += v[u].v[e];
+        put_row<4>(p, l, run_key(p, l, (b + 1) * p.chunk), c, whole, acc);
+    }
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) {
+        const int n = heavy[i];
+        if (n == 0) continue;                                    // (the same for the whole workgroup)
+        const int from = blockIdx.x * 16 + i;
+        const float* rest = l.part + ((int64_t)from + 1) * 2 * p.dim + c;
+        fvec<4> acc = {{0.f, 0.f, 0.f, 0.f}};
+        if (mine) {
+            if (wave == 0) acc = load_e<4, float>(rest - p.dim, whole, p.dim - c);
+            for (int k = wave; k < n; k += 128) {
+                fvec<4> v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) v[u] = load_e<4, float>(rest + (int64_t)(k + 16 * u < n ? k + 16 * u : k) * 2 * p.dim, whole, p.dim - c);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (k + 16 * u < n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc.v[e] += v[u].v[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) buf[wave][lane * 4 + e] = acc.v[e];
+        __syncthreads();
+        if (wave == 0 && mine) {
+            for (int q = 1; q < 16; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc.v[e] += buf[q][lane * 4 + e];
+            put_row<4>(p, l, run_key(p, l, (from + 1) * p.chunk), c, whole, acc);
+        }
+        __syncthreads();
+    }
 }
 
-__global__ __launch_bounds__(256) void fill_zero_kernel(float* __restrict__ p, int64_t n) {
-    const int64_t stride = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) p[i] = 0.f;
-}
+__global__ __launch_bounds__(SORT_THREADS) void zero_kernel(ZeroPart z) { zero_part(z, blockIdx.x, gridDim.x); }
 
 static int run_chunk(int64_t n) {
-    int64_t c = (n + 2047) / 2048;                   // about 2048 workgroups for a long list, and at least 32 rows for each
-    return (int)(c < 32 ? 32 : c);
+    int64_t c = (n + 4095) / 4096;                   // up to 4096 workgroups, and at least 16 rows for each
+    return (int)(c < 16 ? 16 : c);
 }
 static int64_t run_chunks(int64_t n) { return n ? (n + run_chunk(n) - 1) / run_chunk(n) : 0; }
 
@@ -315,7 +432,21 @@ static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 extern "C" int64_t hh_workspace_bytes_embed_tokens_bwd(int64_t seqs, int length, int64_t rows, int dim) {
     if (!embed_shape_ok(seqs, length, rows, dim)) return -1;
     const int64_t n = seqs * length;
-    return 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4) + align256(run_chunks(n) * 2 * (int64_t)dim * 4);
+    return 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4) + 2 * align256(4 * run_chunks(n)) + 2 * align256(run_chunks(n) * 2 * (int64_t)dim * 4);
+}
+
+// part i of `parts` of the zeros of out, and the workgroups that write it
+static ZeroPart zero_share(float* out, int64_t total, int i, int parts, int* blocks) {
+    ZeroPart z = {out, 0, 0, 0};
+    *blocks = 0;
+    if (out == nullptr) return z;
+    z.wide = HH_ALIGNED16(out) && total % 4 == 0;
+    const int64_t share = ((total + parts - 1) / parts + 3) / 4 * 4;
+    z.begin = i * share < total ? i * share : total;
+    z.end = z.begin + share < total ? z.begin + share : total;
+    const int64_t want = (z.end - z.begin + 16383) / 16384;                   // 16 values for each thread
+    *blocks = (int)(want < 1024 ? want : 1024);
+    return z;
 }
 
 extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy, int dy_dtype, float* dweight, int accumulate, float* dpos, int64_t seqs, int length, int64_t rows,
@@ -329,45 +460,41 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     const int64_t n = seqs * length;
     HH_REQUIRE(n == 0 || (ids != nullptr && dy != nullptr && workspace != nullptr && HH_ALIGNED16(workspace)), HH_ERR_ALIGN,
                "hh_embed_tokens_bwd: ids, dy and a 16-byte aligned workspace are needed");
-    if (!accumulate) {
-        const int64_t total = rows * dim, blocks = (total + 1023) / 1024;
-        hipLaunchKernelGGL(fill_zero_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, dweight, total);
-    }
+    int zb = 0;
+    float* zero = accumulate ? nullptr : dweight;
     if (n == 0) {
-        if (dpos) hipLaunchKernelGGL(fill_zero_kernel, dim3(64), dim3(256), 0, s, dpos, (int64_t)length * dim);
+        ZeroPart z = zero_share(zero, rows * dim, 0, 1, &zb);
+        if (zb) hipLaunchKernelGGL(zero_kernel, dim3(zb), dim3(SORT_THREADS), 0, s, z);
+        z = zero_share(dpos, (int64_t)length * dim, 0, 1, &zb);
+        if (zb) hipLaunchKernelGGL(zero_kernel, dim3(zb), dim3(SORT_THREADS), 0, s, z);
         return hh_check_launch("hh_embed_tokens_bwd");
     }
     char* ws = (char*)workspace;
     u32* keys[2] = {(u32*)ws, (u32*)(ws + align256(4 * n))};
     u32* from[2] = {(u32*)(ws + 2 * align256(4 * n)), (u32*)(ws + 3 * align256(4 * n))};
     u32* hist = (u32*)(ws + 4 * align256(4 * n));
-    float* part = (float*)(ws + 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4));
+    u32* flags = (u32*)((char*)hist + align256(SORT_BLOCKS * 256 * 4));
+    const int64_t flag_bytes = align256(4 * run_chunks(n)), part_bytes = align256(run_chunks(n) * 2 * (int64_t)dim * 4);
+    char* part = (char*)flags + 2 * flag_bytes;
     const SortPlan sp = sort_plan(n, rows);
     for (int i = 0; i < sp.passes; ++i) {
-        hipLaunchKernelGGL(sort_count_kernel, dim3(sp.blocks), dim3(256), 0, s, i == 0 ? ids : nullptr, id_bytes == 8, rows, skip_id, keys[i & 1], hist, (int)n, sp.per_block,
-                           sp.pass[i].shift, sp.pass[i].bits);
-        hipLaunchKernelGGL(sort_place_kernel, dim3(sp.blocks), dim3(256), 0, s, keys[i & 1], i == 0 ? nullptr : from[i & 1], hist, keys[(i + 1) & 1], from[(i + 1) & 1], (int)n,
-                           sp.per_block, sp.pass[i].shift, sp.pass[i].bits);
+        ZeroPart z = zero_share(zero, rows * dim, 2 * i, 2 * sp.passes, &zb);
+        hipLaunchKernelGGL(sort_count_kernel, dim3(sp.blocks + zb), dim3(SORT_THREADS), 0, s, i == 0 ? ids : nullptr, id_bytes == 8, rows, skip_id, keys[i & 1], hist, (int)n, sp.per_block,
+                           sp.pass[i].shift, sp.pass[i].bits, sp.blocks, z);
+        z = zero_share(zero, rows * dim, 2 * i + 1, 2 * sp.passes, &zb);
+        hipLaunchKernelGGL(sort_place_kernel, dim3(sp.blocks + zb), dim3(SORT_THREADS), 0, s, keys[i & 1], i == 0 ? nullptr : from[i & 1], hist, keys[(i + 1) & 1], from[(i + 1) & 1], (int)n,
+                           sp.per_block, sp.pass[i].shift, sp.pass[i].bits, sp.blocks, z);
     }
     RunParams p;
-    p.keys = keys[sp.passes & 1]; p.from = from[sp.passes & 1];
-    p.dy = dy; p.out = dweight; p.part = part;
-    p.n = (int)n; p.chunk = run_chunk(n); p.dim = dim; p.accumulate = accumulate != 0;
-    p.aligned = dim % 4 == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dweight);
-    p.length = length; p.seqs = (int)seqs; p.rows = rows; p.scale = scale;
-    const int need = (dim + 3) / 4;
+    p.dy = dy; p.n = (int)n; p.chunk = run_chunk(n); p.chunks = (int)run_chunks(n); p.dim = dim; p.length = length; p.seqs = (int)seqs;
+    const int e = dy_dtype == HH_F32 ? 4 : 8;
+    p.list[0] = RunList{keys[sp.passes & 1], from[sp.passes & 1], dweight, (float*)part, flags, rows, accumulate != 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dweight), scale};
+    p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), (u32*)((char*)flags + flag_bytes), length, 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dpos), 1.f};
+    const int need = (dim + e - 1) / e;
     const int threads = need >= 256 ? 256 : (need + 63) / 64 * 64;
-    const dim3 grid((unsigned)run_chunks(n), (unsigned)((need + 255) / 256));
-    for (int which = 0; which < 2; ++which) {
-        if (which == 1) {
-            if (!dpos) break;
-            p.keys = p.from = nullptr;
-            p.out = dpos; p.accumulate = 0; p.scale = 1.f; p.rows = length;
-            p.aligned = dim % 4 == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dpos);
-        }
-        if (dy_dtype == HH_F32) hipLaunchKernelGGL(run_sum_kernel<float>, grid, dim3(threads), 0, s, p);
-        else hipLaunchKernelGGL(run_sum_kernel<bf16_t>, grid, dim3(threads), 0, s, p);
-        hipLaunchKernelGGL(run_join_kernel, grid, dim3(threads), 0, s, p);
-    }
+    const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), dpos ? 2u : 1u);
+    if (e == 4) hipLaunchKernelGGL((run_sum_kernel<float, 4>), grid, dim3(threads), 0, s, p);
+    else hipLaunchKernelGGL((run_sum_kernel<bf16_t, 8>), grid, dim3(threads), 0, s, p);
+    hipLaunchKernelGGL(run_join_kernel, dim3((unsigned)((p.chunks + 15) / 16), (unsigned)((dim + 255) / 256), dpos ? 2u : 1u), dim3(1024), 0, s, p);
     return hh_check_launch("hh_embed_tokens_bwd");
 }
