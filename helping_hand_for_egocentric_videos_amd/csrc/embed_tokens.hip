@@ -14,19 +14,19 @@ typedef unsigned int u32;
 template <int E> struct fvec { float v[E]; };
 
 // E consecutive elements as fp32; `whole`: the address is aligned for one wide access and all E exist, else `n` of them one by one
-template <int E, typename T>
+template <int E, typename T, bool NT = false>
 __device__ __forceinline__ fvec<E> load_e(const T* p, bool whole, int n) {
     fvec<E> r;
     if (whole) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < E; i += 4) {
-                const f32x4 t = *(const f32x4*)(p + i);
+                const f32x4 t = NT ? __builtin_nontemporal_load((const f32x4*)(p + i)) : *(const f32x4*)(p + i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) r.v[i + j] = t[j];
             }
         } else if constexpr (E == 8) {
-            const u32x4 t = *(const u32x4*)p;
+            const u32x4 t = NT ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
 #pragma unroll
             for (int j = 0; j < 4; ++j) { r.v[2 * j] = bf16_lo_to_f32(t[j]); r.v[2 * j + 1] = bf16_hi_to_f32(t[j]); }
         } else {
@@ -40,12 +40,12 @@ __device__ __forceinline__ fvec<E> load_e(const T* p, bool whole, int n) {
     }
     return r;
 }
-template <int E, typename T>
+template <int E, typename T, bool NT = false>
 __device__ __forceinline__ void store_e(T* p, const fvec<E>& r, bool whole, int n) {
     if (whole) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < E; i += 4) { f32x4 t = {r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]}; *(f32x4*)(p + i) = t; }
+            for (int i = 0; i < E; i += 4) { f32x4 t = {r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]}; if (NT) __builtin_nontemporal_store(t, (f32x4*)(p + i)); else *(f32x4*)(p + i) = t; }
         } else if constexpr (E == 8) {
             u32x4 t = {pack_bf16(r.v[0], r.v[1]), pack_bf16(r.v[2], r.v[3]), pack_bf16(r.v[4], r.v[5]), pack_bf16(r.v[6], r.v[7])};
             *(u32x4*)p = t;
@@ -65,7 +65,7 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t i)
 }
 
 // lpr lanes (a power of two) share a row, each takes every lpr-th piece of E elements; 64 / lpr rows to a wave
-template <typename TW, typename TO, int E>
+template <typename TW, typename TO, int E, bool NT>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__ ids, int wide, const TW* __restrict__ w, const float* __restrict__ pos, TO* __restrict__ out,
                                                         int64_t n, int length, int64_t rows, int dim, float scale, int lpr_log2, int aligned) {
     const int lane = threadIdx.x & 63;
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__
 #pragma unroll
             for (int i = 0; i < E; ++i) v.v[i] = __builtin_nanf("");
         }
-        store_e<E, TO>(o + c, v, whole, dim - c);
+        store_e<E, TO, NT>(o + c, v, whole, dim - c);
     }
 }
 
@@ -273,7 +273,7 @@ __device__ __forceinline__ void put_row(const RunParams& p, const RunList& l, u3
 }
 
 // blockIdx.x: a chunk of the list blockIdx.z;  eight rows are requested before the first is added (the gather's latency is what there is to hide)
-template <typename T, int E>
+template <typename T, int E, bool NT>
 __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
     const RunList& l = p.list[blockIdx.z];
     const int c = (blockIdx.y * 256 + threadIdx.x) * E;
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int at = j + i < j1 ? j + i : j1 - 1;              // (behind the chunk: its last row once more, not added)
-            v[i] = load_e<E, T>((const T*)p.dy + run_from(p, l, at) * p.dim + c, whole, p.dim - c);
+            v[i] = load_e<E, T, NT>((const T*)p.dy + run_from(p, l, at) * p.dim + c, whole, p.dim - c);
             next[i] = at + 1 < p.n ? run_key(p, l, at + 1) : ~0u;   // (~0: no key is that large)
         }
 #pragma unroll
@@ -411,19 +411,22 @@ extern "C" int hh_embed_tokens_fwd(const void* ids, int id_bytes, const void* we
     HH_REQUIRE(ids != nullptr && weight != nullptr && out != nullptr, HH_ERR_ALIGN, "hh_embed_tokens_fwd: NULL pointer");
     hipStream_t s = (hipStream_t)stream;
     const bool al = HH_ALIGNED16(weight) && HH_ALIGNED16(out) && HH_ALIGNED16(pos);
+#define EFL(TW, TO, E, NT)                                                                                                                       \
+    hipLaunchKernelGGL((embed_fwd_kernel<TW, TO, E, NT>), dim3((unsigned)blocks), dim3(256), 0, s, ids, id_bytes == 8, (const TW*)weight, pos, (TO*)out, n, length, rows, dim, scale, l, \
+                       (int)(al && dim % E == 0))
 #define EF(TW, TO, E)                                                                                                                            \
     do {                                                                                                                                         \
         int l = 0;                                                                                                                               \
         while (l < 6 && ((int64_t)E << l) < dim) ++l;                                                                                            \
         const int64_t waves = (n + (64 >> l) - 1) / (64 >> l), blocks = (waves + 3) / 4;                                                         \
-        hipLaunchKernelGGL((embed_fwd_kernel<TW, TO, E>), dim3((unsigned)blocks), dim3(256), 0, s, ids, id_bytes == 8, (const TW*)weight, pos, (TO*)out, n, length, rows, dim, scale, l, \
-                           (int)(al && dim % E == 0));                                                                                           \
+        if (n * dim * (int64_t)sizeof(TO) > HH_STREAM_BYTES) EFL(TW, TO, E, true); else EFL(TW, TO, E, false);                                    \
     } while (0)
     if (w_dtype == HH_F32 && out_dtype == HH_F32) EF(float, float, 4);
     else if (w_dtype == HH_F32) EF(float, bf16_t, 4);
     else if (out_dtype == HH_F32) EF(bf16_t, float, 4);
     else EF(bf16_t, bf16_t, 8);
 #undef EF
+#undef EFL
     return hh_check_launch("hh_embed_tokens_fwd");
 }
 
@@ -493,8 +496,13 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     const int need = (dim + e - 1) / e;
     const int threads = need >= 256 ? 256 : (need + 63) / 64 * 64;
     const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), dpos ? 2u : 1u);
-    if (e == 4) hipLaunchKernelGGL((run_sum_kernel<float, 4>), grid, dim3(threads), 0, s, p);
-    else hipLaunchKernelGGL((run_sum_kernel<bf16_t, 8>), grid, dim3(threads), 0, s, p);
+    // dy past the caches where it is read once (64 x 2048 x 1024 bf16: 210 -> 190 us) or does not fit there; with dpos it is read twice, and 160 x 77 x 768 fp32
+    // stay in the cache between (61.5 us, 65.3 past it)
+    const bool nt = !dpos || n * dim * (e == 4 ? 4 : 2) > HH_STREAM_BYTES;
+    if (e == 4 && nt) hipLaunchKernelGGL((run_sum_kernel<float, 4, true>), grid, dim3(threads), 0, s, p);
+    else if (e == 4) hipLaunchKernelGGL((run_sum_kernel<float, 4, false>), grid, dim3(threads), 0, s, p);
+    else if (nt) hipLaunchKernelGGL((run_sum_kernel<bf16_t, 8, true>), grid, dim3(threads), 0, s, p);
+    else hipLaunchKernelGGL((run_sum_kernel<bf16_t, 8, false>), grid, dim3(threads), 0, s, p);
     hipLaunchKernelGGL(run_join_kernel, dim3((unsigned)((p.chunks + 15) / 16), (unsigned)((dim + 255) / 256), dpos ? 2u : 1u), dim3(1024), 0, s, p);
     return hh_check_launch("hh_embed_tokens_bwd");
 }

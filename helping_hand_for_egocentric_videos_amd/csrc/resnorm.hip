@@ -7,450 +7,508 @@
 // Backward, from x_new, y and the gradients dx_new, dh (statistics are taken again: both rows are in registers anyway, and nothing has to be kept):
 //     d = dx_new + pre'(dh),   dx = res_scale * d,   dgate = sum d o p (* 1 - tanh^2),   dy = post'(g o d),
 //     n'(dn) = rstd * (k - mean(k) - xh * mean(k o xh)) with k = dn o gamma and xh the normed row   (no mean(k) term for root-mean-square norms).
-// Gradients of gamma, beta and the gate are column sums: every workgroup sums its rows in registers and leaves one row of partial sums, which a
-// second launch adds in workgroup order (no atomics: equal inputs give equal bits).
+// The gate's and post's gradients all come from two column sums over the rows of a gate group, S0 = sum d and S1 = sum d o xh:
+//     dgate = (gamma o S1 + beta o S0) (* 1 - tanh^2),   dgamma += g o S1,   dbeta += g o S0,
+// so that a lane keeps four sums for a channel (with dh o xh and dh of pre) and never needs p itself.  Every workgroup sums its rows in registers and leaves
+// one row of partial sums, which a second launch adds in a fixed order (no atomics: equal inputs give equal bits).
+//
+// Layout: a row lies across the ceil(cols / 256) waves of a workgroup, 4 channels to a lane; the workgroup takes R rows at a time, so that the
+// parameters are read once for them, R rows of loads are in flight, and one exchange through LDS (one barrier) serves the sums of R rows.  A wave per row, the
+// obvious form, holds 16 channels of five sums in a lane at 1024 channels: 256 registers, one wave to a SIMD, 1168 us for the backward pass of 131 104 rows.
 #include "common.h"
 
-// cols <= WPR * NV * 256: WPR waves share a row, each lane holds NV pieces of 4 consecutive channels
-template <int NV>
-struct Row { float v[NV][4]; };
+struct Q4 { float v[4]; };
 
 struct RnParams {
     const void* x; const void* y; void* x_new; void* h;
     const void* dx_new; const void* dh; void* dx; void* dy;
     const float* gate; const float* g1; const float* b1; const float* g2; const float* b2;
-    float* part;                       // [4][blocks][cols]: dgamma / dbeta of post, of pre;  behind them [units][cols] (or [units]) of the gate
-    float* gate_part;
+    float* part;                       // [4][blocks][cols]: dgamma / dbeta of post, of pre
+    float* gate_part;                  // [units][cols], or [units] for a scalar gate
     int64_t rows, each;                // rows of one gate group (all of them without groups)
     int64_t chunk, chunks;             // rows of a unit, units of a group
     int64_t units, per_block;          // units in all, and of one workgroup
-    int cols, gate_kind, gate_tanh, rms, vec;
+    int cols, gate_kind, gate_tanh, rms;
     int x_dt, y_dt, h_dt;
     float eps1, eps2, res_scale;
 };
 
-template <int NV, int WPR>
-__device__ __forceinline__ void rn_load(Row<NV>& r, const void* base, int dt, int64_t off, int cols, int vec, int t) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * 64 * WPR + t) * 4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r.v[i][j] = 0.f;
+// four channels as they lie in memory: 4 dwords of fp32, 2 of bf16; turned into fp32 only when all loads of a step have been issued (a conversion behind
+// each load would wait for it)
+template <bool VEC>
+__device__ __forceinline__ u32x4 rn_raw(const void* base, int dt, int64_t off, int c, int cols) {
+    u32x4 r = {0u, 0u, 0u, 0u};
+    if (VEC) {
         if (c < cols) {
-            if (vec) {
-                if (dt == HH_F32) {
-                    const f32x4 q = *(const f32x4*)((const float*)base + off + c);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) r.v[i][j] = q[j];
-                } else {
-                    const u32x2 q = *(const u32x2*)((const bf16_t*)base + off + c);
-                    r.v[i][0] = bf16_lo_to_f32(q[0]); r.v[i][1] = bf16_hi_to_f32(q[0]);
-                    r.v[i][2] = bf16_lo_to_f32(q[1]); r.v[i][3] = bf16_hi_to_f32(q[1]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (c + j < cols) r.v[i][j] = dt == HH_F32 ? ((const float*)base)[off + c + j] : (float)((const bf16_t*)base)[off + c + j];
-            }
+            if (dt == HH_F32) r = *(const u32x4*)((const float*)base + off + c);
+            else { const u32x2 t = *(const u32x2*)((const bf16_t*)base + off + c); r[0] = t[0]; r[1] = t[1]; }
         }
-    }
-}
-template <int NV, int WPR>
-__device__ __forceinline__ void rn_store(const Row<NV>& r, void* base, int dt, int64_t off, int cols, int vec, int t) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * 64 * WPR + t) * 4;
-        if (c < cols) {
-            if (vec) {
-                if (dt == HH_F32) {
-                    const f32x4 q = {r.v[i][0], r.v[i][1], r.v[i][2], r.v[i][3]};
-                    *(f32x4*)((float*)base + off + c) = q;
-                } else {
-                    const u32x2 q = {pack_bf16(r.v[i][0], r.v[i][1]), pack_bf16(r.v[i][2], r.v[i][3])};
-                    *(u32x2*)((bf16_t*)base + off + c) = q;
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (c + j < cols) {
-                        if (dt == HH_F32) ((float*)base)[off + c + j] = r.v[i][j];
-                        else ((bf16_t*)base)[off + c + j] = (bf16_t)r.v[i][j];
-                    }
-            }
-        }
-    }
-}
-
-// sums of N values over the WPR waves of a row; `red` holds [4 waves][N], and the two barriers keep its uses apart
-template <int N, int WPR>
-__device__ __forceinline__ void row_sums(float (&s)[N], float* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < N; ++k) s[k] += __shfl_xor(s[k], o, 64);
-    if constexpr (WPR > 1) {
-        const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int k = 0; k < N; ++k) red[wave * N + k] = s[k];
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            s[k] = 0.f;
-#pragma unroll
-            for (int w = 0; w < WPR; ++w) s[k] += red[w * N + k];
-        }
-        __syncthreads();
-    }
-}
-
-template <int NV, int WPR>
-__device__ __forceinline__ bool rn_in(int i, int j, int t, int cols) { return (i * 64 * WPR + t) * 4 + j < cols; }
-
-// means and reciprocal standard deviations of two rows at once (one reduction tree for both)
-template <int NV, int WPR>
-__device__ __forceinline__ void rn_stats2(const Row<NV>& a, const Row<NV>& b, int cols, int rms, float eps_a, float eps_b, int t, float* red, float (&mean)[2], float (&rstd)[2]) {
-    const float inv = 1.f / (float)cols;
-    mean[0] = mean[1] = 0.f;
-    if (!rms) {
-        float s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { s[0] += a.v[i][j]; s[1] += b.v[i][j]; }
-        row_sums<2, WPR>(s, red);
-        mean[0] = s[0] * inv; mean[1] = s[1] * inv;
-    }
-    float q[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (rn_in<NV, WPR>(i, j, t, cols)) {
-                const float da = a.v[i][j] - mean[0], db = b.v[i][j] - mean[1];
-                q[0] += da * da; q[1] += db * db;
-            }
-    row_sums<2, WPR>(q, red);
-    rstd[0] = 1.f / sqrtf(q[0] * inv + eps_a);
-    rstd[1] = 1.f / sqrtf(q[1] * inv + eps_b);
-}
-template <int NV, int WPR>
-__device__ __forceinline__ void rn_stats(const Row<NV>& a, int cols, int rms, float eps, int t, float* red, float& mean, float& rstd) {
-    const float inv = 1.f / (float)cols;
-    mean = 0.f;
-    if (!rms) {
-        float s[1] = {0.f};
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[0] += a.v[i][j];
-        row_sums<1, WPR>(s, red);
-        mean = s[0] * inv;
-    }
-    float q[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (rn_in<NV, WPR>(i, j, t, cols)) { const float d = a.v[i][j] - mean; q[0] += d * d; }
-    row_sums<1, WPR>(q, red);
-    rstd = 1.f / sqrtf(q[0] * inv + eps);
-}
-
-template <int NV, int WPR>
-__device__ __forceinline__ void rn_gate(Row<NV>& g, const RnParams& p, int64_t group, int t) {
-    if (p.gate_kind == HH_GATE_NONE) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) g.v[i][j] = 1.f;
-        return;
-    }
-    if (p.gate_kind == HH_GATE_SCALAR) {
-        const float a = p.gate_tanh ? tanhf(p.gate[0]) : p.gate[0];
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) g.v[i][j] = a;
-        return;
-    }
-    rn_load<NV, WPR>(g, p.gate, HH_F32, p.gate_kind == HH_GATE_GROUP ? group * p.cols : 0, p.cols, p.vec, t);
-    if (p.gate_tanh)
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) g.v[i][j] = tanhf(g.v[i][j]);
-}
-
-template <int NV, int WPR, bool POST, bool PRE>
-__global__ __launch_bounds__(256) void resnorm_fwd_kernel(RnParams p) {
-    __shared__ float red[8];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int t = WPR == 1 ? lane : (int)threadIdx.x;
-    const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
-    if (row >= p.rows) return;                       // (a whole wave, and with WPR = 4 no block at all: its barriers are met by every wave)
-    const int64_t off = row * p.cols;
-    Row<NV> x, y, k;
-    rn_load<NV, WPR>(x, p.x, p.x_dt, off, p.cols, p.vec, t);
-    rn_load<NV, WPR>(y, p.y, p.y_dt, off, p.cols, p.vec, t);
-    if constexpr (POST) {
-        float mean, rstd;
-        rn_stats<NV, WPR>(y, p.cols, p.rms, p.eps1, t, red, mean, rstd);
-        rn_load<NV, WPR>(k, p.g1, HH_F32, 0, p.cols, p.vec, t);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y.v[i][j] = (y.v[i][j] - mean) * rstd * k.v[i][j];
-        if (p.b1) {
-            rn_load<NV, WPR>(k, p.b1, HH_F32, 0, p.cols, p.vec, t);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y.v[i][j] += k.v[i][j];
-        }
-    }
-    rn_gate<NV, WPR>(k, p, row / p.each, t);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x.v[i][j] = x.v[i][j] * p.res_scale + k.v[i][j] * y.v[i][j];
-    rn_store<NV, WPR>(x, p.x_new, p.x_dt, off, p.cols, p.vec, t);
-    if constexpr (PRE) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (!rn_in<NV, WPR>(i, j, t, p.cols)) x.v[i][j] = 0.f;          // (channels behind the row's end: 0 * inf above would be NaN)
-        float mean, rstd;
-        rn_stats<NV, WPR>(x, p.cols, p.rms, p.eps2, t, red, mean, rstd);
-        rn_load<NV, WPR>(k, p.g2, HH_F32, 0, p.cols, p.vec, t);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x.v[i][j] = (x.v[i][j] - mean) * rstd * k.v[i][j];
-        if (p.b2) {
-            rn_load<NV, WPR>(k, p.b2, HH_F32, 0, p.cols, p.vec, t);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x.v[i][j] += k.v[i][j];
-        }
-        rn_store<NV, WPR>(x, p.h, p.h_dt, off, p.cols, p.vec, t);
-    }
-}
-
-// column sums of the four waves (WPR = 1: each saw rows of its own) or of the row's four waves (WPR = 4: each owns its channels) -> one fp32 row
-template <int NV, int WPR>
-__device__ __forceinline__ void rn_put_cols(const Row<NV>& a, float* out, int cols, int t, float* buf) {
-    const int wave = threadIdx.x >> 6;
-    if constexpr (WPR == 1) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) buf[wave * NV * 256 + (i * 64 + t) * 4 + j] = a.v[i][j];
-        __syncthreads();
-        for (int c = threadIdx.x; c < cols; c += 256) out[c] = (buf[c] + buf[NV * 256 + c]) + (buf[2 * NV * 256 + c] + buf[3 * NV * 256 + c]);
-        __syncthreads();
     } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int j = 0; j < 4; ++j)
+            if (c + j < cols) {
+                if (dt == HH_F32) r[j] = ((const unsigned*)base)[off + c + j];
+                else r[j >> 1] |= (unsigned)((const unsigned short*)base)[off + c + j] << (16 * (j & 1));
+            }
+    }
+    return r;
+}
+__device__ __forceinline__ Q4 rn_cvt(const u32x4& r, int dt) {
+    Q4 q;
+    if (dt == HH_F32) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (rn_in<NV, WPR>(i, j, t, cols)) out[(i * 64 * WPR + t) * 4 + j] = a.v[i][j];
+        for (int j = 0; j < 4; ++j) q.v[j] = __uint_as_float(r[j]);
+    } else {
+        q.v[0] = bf16_lo_to_f32(r[0]); q.v[1] = bf16_hi_to_f32(r[0]);
+        q.v[2] = bf16_lo_to_f32(r[1]); q.v[3] = bf16_hi_to_f32(r[1]);
+    }
+    return q;
+}
+template <bool VEC>
+__device__ __forceinline__ Q4 rn_param(const float* base, int64_t off, int c, int cols) { return rn_cvt(rn_raw<VEC>(base, HH_F32, off, c, cols), HH_F32); }
+
+template <bool VEC, bool NT>
+__device__ __forceinline__ void rn_store(const Q4& q, void* base, int dt, int64_t off, int c, int cols) {
+    if (VEC) {
+        if (c < cols) {
+            if (dt == HH_F32) {
+                const f32x4 t = {q.v[0], q.v[1], q.v[2], q.v[3]};
+                f32x4* o = (f32x4*)((float*)base + off + c);
+                if (NT) __builtin_nontemporal_store(t, o); else *o = t;
+            } else {
+                const u32x2 t = {pack_bf16(q.v[0], q.v[1]), pack_bf16(q.v[2], q.v[3])};
+                u32x2* o = (u32x2*)((bf16_t*)base + off + c);
+                if (NT) __builtin_nontemporal_store(t, o); else *o = t;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < cols) {
+                if (dt == HH_F32) ((float*)base)[off + c + j] = q.v[j];
+                else ((bf16_t*)base)[off + c + j] = (bf16_t)q.v[j];
+            }
     }
 }
 
-template <int NV, int WPR, bool POST, bool PRE>
-__global__ __launch_bounds__(256) void resnorm_bwd_kernel(RnParams p) {
-    __shared__ float red[8];
-    __shared__ float buf[WPR == 1 ? 4 * NV * 256 : 8];
+__device__ __forceinline__ float add_swapped32(float a, float b) {     // lanes 0..31: a over both halves, lanes 32..63: b
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_swapped16(float a, float b) {     // even rows of 16 lanes: a over a pair of rows, odd rows: b
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float add_row16(float v) {                  // sum over the 16 lanes of a row, in every lane of it (row rotations)
+    return add_dpp<0x121>(add_dpp<0x122>(add_dpp<0x124>(add_dpp<0x128>(v))));
+}
+
+// N values (1, 2, 4 or 8) summed over the workgroup, in every lane.  A wave halves the number of values that a lane holds with the number of lanes that hold a
+// value (8 values: 20 instructions instead of 48 exchanges), the waves meet in LDS.  `turn` alternates between two buffers: a wave writes a buffer again
+// only behind the barrier of the sums in between, which every wave passes after it has read.
+struct RnRed { float buf[2][16 * 8]; };
+template <int N>
+__device__ __forceinline__ void block_sums(float (&s)[N], RnRed& red, int& turn, int waves) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int t = WPR == 1 ? lane : (int)threadIdx.x;
+    float* buf = red.buf[turn];
+    turn ^= 1;
+    if constexpr (N >= 4) {
+        float t[N / 2], u[N / 4];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) t[i] = add_swapped32(s[i], s[i + N / 2]);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) u[i] = add_row16(add_swapped16(t[i], t[i + N / 4]));
+        if ((lane & 15) == 0)
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) buf[wave * N + (lane >> 4) * (N / 4) + i] = u[i];
+    } else if constexpr (N == 2) {
+        float t = add_swapped32(s[0], s[1]);
+        t = add_row16(add_swapped16(t, t));
+        if ((lane & 31) == 0) buf[wave * 2 + (lane >> 5)] = t;
+    } else {
+        float t = add_swapped32(s[0], s[0]);
+        t = add_row16(add_swapped16(t, t));
+        if (lane == 0) buf[wave] = t;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = 0.f;
+    for (int w = 0; w < waves; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += buf[w * N + i];
+}
+
+// mean and reciprocal standard deviation (or root mean square, with mean 0) of N rows; two passes
+template <int N>
+__device__ __forceinline__ void rn_stats(const Q4 (&v)[N], const bool (&in)[4], float inv, int rms, const float (&eps)[N], RnRed& red, int& turn, int waves, float (&mean)[N], float (&rstd)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) mean[i] = 0.f;
+    if (!rms) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) mean[i] = ((in[0] ? v[i].v[0] : 0.f) + (in[1] ? v[i].v[1] : 0.f)) + ((in[2] ? v[i].v[2] : 0.f) + (in[3] ? v[i].v[3] : 0.f));
+        block_sums<N>(mean, red, turn, waves);
+#pragma unroll
+        for (int i = 0; i < N; ++i) mean[i] *= inv;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        rstd[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float d = in[j] ? v[i].v[j] - mean[i] : 0.f;
+            rstd[i] += d * d;
+        }
+    }
+    block_sums<N>(rstd, red, turn, waves);
+#pragma unroll
+    for (int i = 0; i < N; ++i) rstd[i] = 1.f / sqrtf(rstd[i] * inv + eps[i]);
+}
+
+template <bool VEC>
+__device__ __forceinline__ Q4 rn_gate(const RnParams& p, int64_t group, int c) {
+    Q4 g = {{1.f, 1.f, 1.f, 1.f}};
+    if (p.gate_kind == HH_GATE_NONE) return g;
+    if (p.gate_kind == HH_GATE_SCALAR) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g.v[j] = p.gate[0];
+    } else {
+        g = rn_param<VEC>(p.gate, p.gate_kind == HH_GATE_GROUP ? group * p.cols : 0, c, p.cols);
+    }
+    if (p.gate_tanh)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g.v[j] = tanhf(g.v[j]);
+    return g;
+}
+
+template <int R, bool VEC, bool NT>
+__global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
+    __shared__ RnRed red;
+    const int waves = blockDim.x >> 6, c = threadIdx.x * 4;
     const float inv = 1.f / (float)p.cols;
-    Row<NV> ag1, ab1, ag2, ab2, agt;
+    bool in[4];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int j = 0; j < 4; ++j) in[j] = c + j < p.cols;
+    const int64_t r0 = (int64_t)blockIdx.x * R;
+    u32x4 rx[R], ry[R];
+    int64_t off[R];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ag1.v[i][j] = ab1.v[i][j] = ag2.v[i][j] = ab2.v[i][j] = agt.v[i][j] = 0.f;
+    for (int i = 0; i < R; ++i) {
+        off[i] = (r0 + i < p.rows ? r0 + i : p.rows - 1) * p.cols;       // (behind the last row: that row once more, not stored)
+        rx[i] = rn_raw<VEC>(p.x, p.x_dt, off[i], c, p.cols);
+        ry[i] = rn_raw<VEC>(p.y, p.y_dt, off[i], c, p.cols);
+    }
+    int turn = 0;
+    Q4 g1, b1, g2, b2, gate[R];
+    if (p.g1) { g1 = rn_param<VEC>(p.g1, 0, c, p.cols); b1 = p.b1 ? rn_param<VEC>(p.b1, 0, c, p.cols) : Q4{{0.f, 0.f, 0.f, 0.f}}; }
+    if (p.g2) { g2 = rn_param<VEC>(p.g2, 0, c, p.cols); b2 = p.b2 ? rn_param<VEC>(p.b2, 0, c, p.cols) : Q4{{0.f, 0.f, 0.f, 0.f}}; }
+    if (p.gate_kind == HH_GATE_GROUP) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) gate[i] = rn_gate<VEC>(p, (r0 + i < p.rows ? r0 + i : p.rows - 1) / p.each, c);
+    } else {
+        gate[0] = rn_gate<VEC>(p, 0, c);
+#pragma unroll
+        for (int i = 1; i < R; ++i) gate[i] = gate[0];
+    }
+    Q4 x[R], y[R];
+    float mean[R], rstd[R], eps[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) { x[i] = rn_cvt(rx[i], p.x_dt); y[i] = rn_cvt(ry[i], p.y_dt); }
+    if (p.g1) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) eps[i] = p.eps1;
+        rn_stats<R>(y, in, inv, p.rms, eps, red, turn, waves, mean, rstd);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[i].v[j] = (y[i].v[j] - mean[i]) * rstd[i] * g1.v[j] + b1.v[j];
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i].v[j] = x[i].v[j] * p.res_scale + gate[i].v[j] * y[i].v[j];
+        if (r0 + i < p.rows) rn_store<VEC, NT>(x[i], p.x_new, p.x_dt, off[i], c, p.cols);
+    }
+    if (p.g2) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) eps[i] = p.eps2;
+        rn_stats<R>(x, in, inv, p.rms, eps, red, turn, waves, mean, rstd);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i].v[j] = (x[i].v[j] - mean[i]) * rstd[i] * g2.v[j] + b2.v[j];
+            if (r0 + i < p.rows) rn_store<VEC, NT>(x[i], p.h, p.h_dt, off[i], c, p.cols);
+        }
+    }
+}
+
+template <int R, bool POST, bool PRE, bool VEC, bool NT>
+__global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
+    __shared__ RnRed red;
+    const int waves = blockDim.x >> 6, c = threadIdx.x * 4;
+    const float inv = 1.f / (float)p.cols;
+    const Q4 zero = {{0.f, 0.f, 0.f, 0.f}};
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in[j] = c + j < p.cols;
+    int turn = 0;
+    Q4 g2 = zero, ag1 = zero, ab1 = zero, ag2 = zero, ab2 = zero;
+    if (PRE) g2 = rn_param<VEC>(p.g2, 0, c, p.cols);
     const int64_t u0 = blockIdx.x * p.per_block, u1 = u0 + p.per_block < p.units ? u0 + p.per_block : p.units;
     for (int64_t u = u0; u < u1; ++u) {
         const int64_t group = u / p.chunks, first = (u % p.chunks) * p.chunk;
         const int64_t last = first + p.chunk < p.each ? first + p.chunk : p.each;
-        for (int64_t r = first + (WPR == 1 ? wave : 0); r < last; r += WPR == 1 ? 4 : 1) {
-            const int64_t off = (group * p.each + r) * p.cols;
-            Row<NV> d, y, k, w;
-            rn_load<NV, WPR>(y, p.y, p.y_dt, off, p.cols, p.vec, t);
-            if (p.dx_new) rn_load<NV, WPR>(d, p.dx_new, p.x_dt, off, p.cols, p.vec, t);
-            else {
+        const Q4 gate = rn_gate<VEC>(p, group, c);
+        Q4 w = gate, s0 = zero, s1 = zero;                               // w: g o gamma of post
+        if (POST) {
+            w = rn_param<VEC>(p.g1, 0, c, p.cols);
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+            for (int j = 0; j < 4; ++j) w.v[j] *= gate.v[j];
+        }
+        for (int64_t r = first; r < last; r += R) {
+            u32x4 rx[R], rh[R], rd[R], ry[R];
+            int64_t off[R];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) d.v[i][j] = 0.f;
+            for (int i = 0; i < R; ++i) {
+                // behind the unit's last row: that row once more, with gradients of zero, and not stored
+                off[i] = (group * p.each + (r + i < last ? r + i : last - 1)) * p.cols;
+                if (PRE) rx[i] = rn_raw<VEC>(p.x_new, p.x_dt, off[i], c, p.cols);
+                ry[i] = rn_raw<VEC>(p.y, p.y_dt, off[i], c, p.cols);
+                rd[i] = rh[i] = (u32x4){0u, 0u, 0u, 0u};
+                if (r + i < last) {
+                    if (PRE) rh[i] = rn_raw<VEC>(p.dh, p.h_dt, off[i], c, p.cols);
+                    if (p.dx_new) rd[i] = rn_raw<VEC>(p.dx_new, p.x_dt, off[i], c, p.cols);
+                }
             }
-            float mean[2] = {0.f, 0.f}, rstd[2] = {1.f, 1.f};
+            float mean[2 * R], rstd[2 * R], s[2 * R];
+            Q4 y[R], d[R];
             if constexpr (PRE) {
-                Row<NV> x, dh;
-                rn_load<NV, WPR>(x, p.x_new, p.x_dt, off, p.cols, p.vec, t);
-                rn_load<NV, WPR>(dh, p.dh, p.h_dt, off, p.cols, p.vec, t);
-                rn_load<NV, WPR>(k, p.g2, HH_F32, 0, p.cols, p.vec, t);
-                if constexpr (POST) rn_stats2<NV, WPR>(x, y, p.cols, p.rms, p.eps2, p.eps1, t, red, mean, rstd);
-                else rn_stats<NV, WPR>(x, p.cols, p.rms, p.eps2, t, red, mean[0], rstd[0]);
-                float s[2] = {0.f, 0.f};
+                Q4 x[R];
+                if constexpr (POST) {                                    // both norms' statistics in the same two exchanges
+                    Q4 xy[2 * R];
+                    float eps[2 * R];
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+                    for (int i = 0; i < R; ++i) {
+                        xy[i] = rn_cvt(rx[i], p.x_dt); xy[R + i] = rn_cvt(ry[i], p.y_dt);
+                        eps[i] = p.eps2; eps[R + i] = p.eps1;
+                    }
+                    rn_stats<2 * R>(xy, in, inv, p.rms, eps, red, turn, waves, mean, rstd);
+#pragma unroll
+                    for (int i = 0; i < R; ++i) { x[i] = xy[i]; y[i] = xy[R + i]; }
+                } else {
+                    float eps[R], m[R], q[R];
+#pragma unroll
+                    for (int i = 0; i < R; ++i) { x[i] = rn_cvt(rx[i], p.x_dt); y[i] = rn_cvt(ry[i], p.y_dt); eps[i] = p.eps2; }
+                    rn_stats<R>(x, in, inv, p.rms, eps, red, turn, waves, m, q);
+#pragma unroll
+                    for (int i = 0; i < R; ++i) { mean[i] = m[i]; rstd[i] = q[i]; }
+                }
+                Q4 k[R];
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    k[i] = rn_cvt(rh[i], p.h_dt);
+                    d[i] = rn_cvt(rd[i], p.x_dt);
+                    s[i] = s[R + i] = 0.f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        x.v[i][j] = (x.v[i][j] - mean[0]) * rstd[0];
-                        ag2.v[i][j] += dh.v[i][j] * x.v[i][j];
-                        ab2.v[i][j] += dh.v[i][j];
-                        dh.v[i][j] *= k.v[i][j];
-                        s[0] += dh.v[i][j];
-                        s[1] += dh.v[i][j] * x.v[i][j];
+                        const float xh = (x[i].v[j] - mean[i]) * rstd[i];
+                        ag2.v[j] += k[i].v[j] * xh;
+                        ab2.v[j] += k[i].v[j];
+                        k[i].v[j] *= g2.v[j];
+                        s[i] += in[j] ? k[i].v[j] : 0.f;
+                        s[R + i] += in[j] ? k[i].v[j] * xh : 0.f;
+                        x[i].v[j] = xh;
                     }
-                row_sums<2, WPR>(s, red);
-                s[0] = p.rms ? 0.f : s[0] * inv;
-                s[1] *= inv;
+                }
+                block_sums<2 * R>(s, red, turn, waves);
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+                for (int i = 0; i < R; ++i) {
+                    const float a = p.rms ? 0.f : s[i] * inv, b = s[R + i] * inv;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) d.v[i][j] += rstd[0] * (dh.v[i][j] - s[0] - x.v[i][j] * s[1]);
-            } else if constexpr (POST) {
-                rn_stats<NV, WPR>(y, p.cols, p.rms, p.eps1, t, red, mean[1], rstd[1]);
-            }
-            rn_gate<NV, WPR>(w, p, group, t);
-            if constexpr (POST) {
-                Row<NV> b;
-                rn_load<NV, WPR>(k, p.g1, HH_F32, 0, p.cols, p.vec, t);
-                if (p.b1) rn_load<NV, WPR>(b, p.b1, HH_F32, 0, p.cols, p.vec, t);
-                float s[2] = {0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const bool in = rn_in<NV, WPR>(i, j, t, p.cols);
-                        const float xh = (y.v[i][j] - mean[1]) * rstd[1];
-                        const float dp = in ? d.v[i][j] * w.v[i][j] : 0.f;
-                        const float pv = xh * k.v[i][j] + (p.b1 ? b.v[i][j] : 0.f);
-                        if (in) agt.v[i][j] += d.v[i][j] * pv;
-                        ag1.v[i][j] += dp * xh;
-                        ab1.v[i][j] += dp;
-                        const float kk = dp * k.v[i][j];
-                        s[0] += kk;
-                        s[1] += kk * xh;
-                        y.v[i][j] = xh;
-                        k.v[i][j] = kk;
-                    }
-                row_sums<2, WPR>(s, red);
-                s[0] = p.rms ? 0.f : s[0] * inv;
-                s[1] *= inv;
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) y.v[i][j] = rstd[1] * (k.v[i][j] - s[0] - y.v[i][j] * s[1]);
+                    for (int j = 0; j < 4; ++j) d[i].v[j] += rstd[i] * (k[i].v[j] - a - x[i].v[j] * b);
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+                for (int i = 0; i < R; ++i) { y[i] = rn_cvt(ry[i], p.y_dt); d[i] = rn_cvt(rd[i], p.x_dt); }
+                if constexpr (POST) {
+                    float eps[R], m[R], q[R];
+#pragma unroll
+                    for (int i = 0; i < R; ++i) eps[i] = p.eps1;
+                    rn_stats<R>(y, in, inv, p.rms, eps, red, turn, waves, m, q);
+#pragma unroll
+                    for (int i = 0; i < R; ++i) { mean[R + i] = m[i]; rstd[R + i] = q[i]; }
+                }
+            }
+            if constexpr (POST) {
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    s[i] = s[R + i] = 0.f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if (rn_in<NV, WPR>(i, j, t, p.cols)) agt.v[i][j] += d.v[i][j] * y.v[i][j];
-                        y.v[i][j] = d.v[i][j] * w.v[i][j];
+                        const float xh = (y[i].v[j] - mean[R + i]) * rstd[R + i];
+                        const float dj = r + i < last ? d[i].v[j] : 0.f;
+                        s0.v[j] += dj;
+                        s1.v[j] += dj * xh;
+                        const float k = d[i].v[j] * w.v[j];
+                        s[i] += in[j] ? k : 0.f;
+                        s[R + i] += in[j] ? k * xh : 0.f;
+                        y[i].v[j] = xh;
+                    }
+                }
+                block_sums<2 * R>(s, red, turn, waves);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const float a = p.rms ? 0.f : s[i] * inv, b = s[R + i] * inv;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[i].v[j] = rstd[R + i] * (d[i].v[j] * w.v[j] - a - y[i].v[j] * b);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s1.v[j] += r + i < last ? d[i].v[j] * y[i].v[j] : 0.f;
+                        y[i].v[j] = d[i].v[j] * w.v[j];
                     }
             }
-            rn_store<NV, WPR>(y, p.dy, p.y_dt, off, p.cols, p.vec, t);
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < R; ++i)
+                if (r + i < last) {
+                    rn_store<VEC, NT>(y[i], p.dy, p.y_dt, off[i], c, p.cols);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d.v[i][j] *= p.res_scale;
-            rn_store<NV, WPR>(d, p.dx, p.x_dt, off, p.cols, p.vec, t);
+                    for (int j = 0; j < 4; ++j) d[i].v[j] *= p.res_scale;
+                    rn_store<VEC, NT>(d[i], p.dx, p.x_dt, off[i], c, p.cols);
+                }
         }
-        if (p.gate_kind != HH_GATE_NONE) {            // a unit's row of gate sums: units never cross groups
-            rn_put_cols<NV, WPR>(agt, p.gate_part + u * p.cols, p.cols, t, buf);
+        Q4 t = s1;                                                       // the unit's share of the gate's gradient: sum d o p
+        if constexpr (POST) {
+            const Q4 g1 = rn_param<VEC>(p.g1, 0, c, p.cols);
+            const Q4 b1 = p.b1 ? rn_param<VEC>(p.b1, 0, c, p.cols) : zero;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) agt.v[i][j] = 0.f;
+            for (int j = 0; j < 4; ++j) {
+                ag1.v[j] += gate.v[j] * s1.v[j];
+                ab1.v[j] += gate.v[j] * s0.v[j];
+                t.v[j] = g1.v[j] * s1.v[j] + b1.v[j] * s0.v[j];
+            }
+        }
+        if (p.gate_kind == HH_GATE_SCALAR) {
+            float sum[1] = {((in[0] ? t.v[0] : 0.f) + (in[1] ? t.v[1] : 0.f)) + ((in[2] ? t.v[2] : 0.f) + (in[3] ? t.v[3] : 0.f))};
+            block_sums<1>(sum, red, turn, waves);
+            if (threadIdx.x == 0) p.gate_part[u] = sum[0];
+        } else if (p.gate_kind != HH_GATE_NONE) {
+            rn_store<VEC, false>(t, p.gate_part, HH_F32, u * p.cols, c, p.cols);
         }
     }
-    const int64_t plane = (int64_t)gridDim.x * p.cols;
-    float* out = p.part + blockIdx.x * (int64_t)p.cols;
+    const int64_t plane = (int64_t)gridDim.x * p.cols, at = blockIdx.x * (int64_t)p.cols;
     if constexpr (POST) {
-        rn_put_cols<NV, WPR>(ag1, out, p.cols, t, buf);
-        rn_put_cols<NV, WPR>(ab1, out + plane, p.cols, t, buf);
+        rn_store<VEC, false>(ag1, p.part, HH_F32, at, c, p.cols);
+        rn_store<VEC, false>(ab1, p.part, HH_F32, plane + at, c, p.cols);
     }
     if constexpr (PRE) {
-        rn_put_cols<NV, WPR>(ag2, out + 2 * plane, p.cols, t, buf);
-        rn_put_cols<NV, WPR>(ab2, out + 3 * plane, p.cols, t, buf);
+        rn_store<VEC, false>(ag2, p.part, HH_F32, 2 * plane + at, c, p.cols);
+        rn_store<VEC, false>(ab2, p.part, HH_F32, 3 * plane + at, c, p.cols);
     }
 }
 
-// out[c] = sum over n rows of part[row][c], rows in order within each of 16 waves and the waves in order: 64 channels to a workgroup.
-// blockIdx.y < 4: the norms' planes (out[y] NULL: not wanted); behind them the gate's groups, whose sums take the derivative of tanh
+// The second launch: column sums of the partial rows.  Three kinds of workgroups, told apart by blockIdx.x:
+//   [0, planes * cols16): a plane of the norms' gradients (or, for up to RN_WIDE_GROUPS gate groups, such a group's rows), 16 channels; 64 lanes share a channel's
+//                         rows, eight loads in flight each
+//   then the gate groups, where there are more of them and so few rows in each that a thread takes a channel of a group by itself
+//   then one workgroup for a scalar gate's sum.
+#define RN_WIDE_GROUPS 32
 struct RnReduce {
-    const float* part; const float* gate_part; const float* gate;
-    float* out[4]; float* dgate;
-    int64_t blocks, chunks;
-    int cols, gate_kind, gate_tanh;
+    const float* part[4]; float* out[4];   // the planes that are wanted
+    const float* gate_part; const float* gate; float* dgate;
+    int64_t blocks, chunks, units, groups;
+    int planes, cols, cols16, gate_kind, gate_tanh, wide_groups;
+    int64_t first_narrow, first_scalar;
 };
-__global__ __launch_bounds__(1024) void resnorm_reduce_kernel(RnReduce p) {
-    __shared__ float buf[16][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int c = blockIdx.x * 64 + lane;
-    const bool is_gate = blockIdx.y >= 4;
-    const int64_t group = (int64_t)blockIdx.y - 4;
-    float* out = is_gate ? p.dgate : p.out[blockIdx.y];
-    if (out == nullptr) return;
-    const int64_t n = is_gate ? p.chunks : p.blocks;
-    const float* src = is_gate ? p.gate_part + group * p.chunks * p.cols : p.part + blockIdx.y * p.blocks * p.cols;
-    const int64_t share = (n + 15) / 16, r0 = wave * share, r1 = r0 + share < n ? r0 + share : n;
-    float s = 0.f;
-    if (c < p.cols)
-        for (int64_t r = r0; r < r1; ++r) s += src[r * p.cols + c];
-    buf[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && c < p.cols) {
-        s = 0.f;
-#pragma unroll
-        for (int w = 0; w < 16; ++w) s += buf[w][lane];
-        if (is_gate) {
-            const int64_t at = group * p.cols + c;
-            if (p.gate_tanh) { const float th = tanhf(p.gate[at]); s *= 1.f - th * th; }
-            out[at] = s;
-        } else {
-            out[c] = s;
-        }
-    }
+__device__ __forceinline__ float rn_untanh(const RnReduce& p, int64_t at, float s) {
+    if (p.gate_tanh) { const float th = tanhf(p.gate[at]); s *= 1.f - th * th; }
+    return s;
 }
-// scalar gate: all units' rows summed by one workgroup
-__global__ __launch_bounds__(1024) void resnorm_scalar_gate_kernel(const float* __restrict__ part, int64_t n, const float* __restrict__ gate, int gate_tanh, float* __restrict__ dgate) {
-    __shared__ float buf[16];
-    float s = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += part[i];
-    s = wave_sum(s);
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s = 0.f;
-        for (int w = 0; w < 16; ++w) s += buf[w];
-        if (gate_tanh) { const float th = tanhf(gate[0]); s *= 1.f - th * th; }
-        dgate[0] = s;
+__global__ __launch_bounds__(1024) void resnorm_reduce_kernel(RnReduce p) {
+    __shared__ float buf[16][16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (blockIdx.x < p.first_narrow) {
+        const int which = blockIdx.x / p.cols16, c = (blockIdx.x % p.cols16) * 16 + (lane & 15);
+        const bool is_gate = which >= p.planes;
+        const int64_t group = which - p.planes, n = is_gate ? p.chunks : p.blocks;
+        const float* src = (is_gate ? p.gate_part + group * p.chunks * p.cols : p.part[which]) + c;
+        float s = 0.f;
+        if (c < p.cols)
+            for (int64_t r = wave * 4 + (lane >> 4); r < n; r += 64 * 8) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = r + 64 * i < n ? src[(r + 64 * i) * p.cols] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += v[i];
+            }
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (lane < 16) buf[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0 && lane < 16 && c < p.cols) {
+            s = 0.f;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) s += buf[w][lane];
+            if (is_gate) p.dgate[group * p.cols + c] = rn_untanh(p, group * p.cols + c, s);
+            else p.out[which][c] = s;
+        }
+    } else if (blockIdx.x < p.first_scalar) {
+        const int64_t i = ((int64_t)blockIdx.x - p.first_narrow) * 1024 + threadIdx.x;
+        if (i >= p.groups * p.cols) return;
+        const int64_t group = i / p.cols;
+        const float* src = p.gate_part + group * p.chunks * p.cols + i % p.cols;
+        float s = 0.f;
+        for (int64_t r = 0; r < p.chunks; r += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = r + k < p.chunks ? src[(r + k) * p.cols] : 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
+        p.dgate[i] = rn_untanh(p, i, s);
+    } else {
+        float s = 0.f;
+        for (int64_t i = threadIdx.x; i < p.units; i += 1024) s += p.gate_part[i];
+        s = wave_sum(s);
+        if (lane == 0) buf[wave][0] = s;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            s = 0.f;
+            for (int w = 0; w < 16; ++w) s += buf[w][0];
+            p.dgate[0] = rn_untanh(p, 0, s);
+        }
     }
 }
 
 // ---- entry points ------------------------------------------------------------------------------------------------------------------------
-#define RN_BLOCKS 1024                                // workgroups of the backward pass, about
-struct RnPlan { int64_t each, groups, chunk, chunks, units, per_block, blocks; };
-static RnPlan rn_plan(int64_t rows, int64_t groups) {
+#ifndef RN_BWD_ROWS
+#define RN_BWD_ROWS 2
+#endif
+#ifndef RN_FWD_MANY
+#define RN_FWD_MANY 4096
+#endif
+static int rn_waves(int cols) { return (cols + 255) / 256; }
+
+struct RnPlan { int64_t each, chunk, chunks, units, per_block, blocks; };
+// about 4096 waves (four to a SIMD) in workgroups that take whole units of one gate group's rows; a unit leaves four partial rows, so it has 16 rows if there are
+static RnPlan rn_plan(int64_t rows, int cols, int64_t groups) {
     RnPlan q;
-    q.groups = groups;
+    const int64_t blocks = 4096 / rn_waves(cols);
     q.each = rows / groups;
-    int64_t want = (RN_BLOCKS + groups - 1) / groups;                   // units of a group, none below 8 rows unless the group is
-    const int64_t most = (q.each + 7) / 8;
+    int64_t want = (blocks + groups - 1) / groups;
+    const int64_t most = (q.each + 15) / 16;
     if (want > most) want = most;
     if (want < 1) want = 1;
     q.chunk = (q.each + want - 1) / want;
     q.chunks = (q.each + q.chunk - 1) / q.chunk;
     q.units = q.chunks * groups;
-    q.per_block = (q.units + RN_BLOCKS - 1) / RN_BLOCKS;
+    q.per_block = (q.units + blocks - 1) / blocks;
     q.blocks = (q.units + q.per_block - 1) / q.per_block;
     return q;
 }
@@ -473,7 +531,7 @@ static int rn_check(const hh_residual_norm* d, bool bwd, const char* who) {
     return HH_OK;
 }
 
-static RnParams rn_params(const hh_residual_norm* d) {
+static RnParams rn_params(const hh_residual_norm* d, bool* vec) {
     RnParams p;
     p.x = d->x; p.y = d->y; p.x_new = d->x_new; p.h = d->h; p.dx_new = d->dx_new; p.dh = d->dh; p.dx = d->dx; p.dy = d->dy;
     p.gate = d->gate; p.g1 = d->post_gamma; p.b1 = d->post_beta; p.g2 = d->pre_gamma; p.b2 = d->pre_beta;
@@ -482,43 +540,33 @@ static RnParams rn_params(const hh_residual_norm* d) {
     p.cols = d->cols; p.gate_kind = d->gate_kind; p.gate_tanh = d->gate_tanh; p.rms = d->rms;
     p.x_dt = d->x_dtype; p.y_dt = d->y_dtype; p.h_dt = d->h_dtype;
     p.eps1 = d->post_eps; p.eps2 = d->pre_eps; p.res_scale = d->res_scale;
-    p.vec = d->cols % 4 == 0 && HH_ALIGNED16(p.x) && HH_ALIGNED16(p.y) && HH_ALIGNED16(p.x_new) && HH_ALIGNED16(p.h) && HH_ALIGNED16(p.dx_new) && HH_ALIGNED16(p.dh) && HH_ALIGNED16(p.dx) &&
-            HH_ALIGNED16(p.dy) && HH_ALIGNED16(p.gate) && HH_ALIGNED16(p.g1) && HH_ALIGNED16(p.b1) && HH_ALIGNED16(p.g2) && HH_ALIGNED16(p.b2);
+    *vec = d->cols % 4 == 0 && HH_ALIGNED16(p.x) && HH_ALIGNED16(p.y) && HH_ALIGNED16(p.x_new) && HH_ALIGNED16(p.h) && HH_ALIGNED16(p.dx_new) && HH_ALIGNED16(p.dh) && HH_ALIGNED16(p.dx) &&
+           HH_ALIGNED16(p.dy) && (d->gate_kind == HH_GATE_SCALAR || HH_ALIGNED16(p.gate)) && HH_ALIGNED16(p.g1) && HH_ALIGNED16(p.b1) && HH_ALIGNED16(p.g2) && HH_ALIGNED16(p.b2);
     return p;
 }
-
-#define RN_DISPATCH(KERNEL, NV, WPR, GRID)                                                                              \
-    do {                                                                                                                \
-        if (p.g1 && p.g2) hipLaunchKernelGGL((KERNEL<NV, WPR, true, true>), GRID, dim3(256), 0, s, p);                  \
-        else if (p.g1) hipLaunchKernelGGL((KERNEL<NV, WPR, true, false>), GRID, dim3(256), 0, s, p);                    \
-        else if (p.g2) hipLaunchKernelGGL((KERNEL<NV, WPR, false, true>), GRID, dim3(256), 0, s, p);                    \
-        else hipLaunchKernelGGL((KERNEL<NV, WPR, false, false>), GRID, dim3(256), 0, s, p);                             \
-    } while (0)
-#define RN_BY_COLS(KERNEL, GRID1, GRID4)                                                                                \
-    do {                                                                                                                \
-        if (p.cols <= 256) RN_DISPATCH(KERNEL, 1, 1, GRID1);                                                            \
-        else if (p.cols <= 512) RN_DISPATCH(KERNEL, 2, 1, GRID1);                                                       \
-        else if (p.cols <= 768) RN_DISPATCH(KERNEL, 3, 1, GRID1);                                                       \
-        else if (p.cols <= 1024) RN_DISPATCH(KERNEL, 4, 1, GRID1);                                                      \
-        else if (p.cols <= 2048) RN_DISPATCH(KERNEL, 2, 4, GRID4);                                                      \
-        else RN_DISPATCH(KERNEL, 4, 4, GRID4);                                                                          \
-    } while (0)
+static int64_t rn_size(int dtype) { return dtype == HH_F32 ? 4 : 2; }
 
 extern "C" int hh_residual_norm_fwd(const hh_residual_norm* d, hh_stream_t stream) {
     const int rc = rn_check(d, false, "hh_residual_norm_fwd");
     if (rc != HH_OK || d->rows == 0) return rc;
     HH_REQUIRE(d->rows <= 0x7fffffff, HH_ERR_SHAPE, "hh_residual_norm_fwd: too many rows");
     hipStream_t s = (hipStream_t)stream;
-    const RnParams p = rn_params(d);
-    const dim3 by4((unsigned)((d->rows + 3) / 4)), by1((unsigned)d->rows);
-    RN_BY_COLS(resnorm_fwd_kernel, by4, by1);
+    bool vec;
+    const RnParams p = rn_params(d, &vec);
+    const bool nt = d->rows * d->cols * (rn_size(p.x_dt) + (p.h ? rn_size(p.h_dt) : 0)) > HH_STREAM_BYTES;
+    const int threads = rn_waves(p.cols) * 64;
+#define RF(R, V, N) hipLaunchKernelGGL((resnorm_fwd_kernel<R, V, N>), dim3((unsigned)((d->rows + R - 1) / R)), dim3(threads), 0, s, p)
+    // four rows to a workgroup where that still leaves work for every CU, one where a short call is all latency
+    if (d->rows >= RN_FWD_MANY) { if (!vec) RF(4, false, false); else if (nt) RF(4, true, true); else RF(4, true, false); }
+    else { if (vec) RF(1, true, false); else RF(1, false, false); }
+#undef RF
     return hh_check_launch("hh_residual_norm_fwd");
 }
 
 extern "C" int64_t hh_workspace_bytes_residual_norm_bwd(int64_t rows, int cols, int64_t groups) {
     if (rows < 0 || cols <= 0 || cols > 4096 || groups < 1 || groups > 65000 || rows % groups) return -1;
     if (rows == 0) return 0;
-    const RnPlan q = rn_plan(rows, groups);
+    const RnPlan q = rn_plan(rows, cols, groups);
     return (4 * q.blocks + q.units) * cols * 4;
 }
 
@@ -526,30 +574,45 @@ extern "C" int hh_residual_norm_bwd(const hh_residual_norm* d, hh_stream_t strea
     const int rc = rn_check(d, true, "hh_residual_norm_bwd");
     if (rc != HH_OK) return rc;
     hipStream_t s = (hipStream_t)stream;
-    RnParams p = rn_params(d);
-    RnReduce r;
-    r.out[0] = d->dpost_gamma; r.out[1] = d->dpost_beta; r.out[2] = d->dpre_gamma; r.out[3] = d->dpre_beta; r.dgate = d->dgate;
-    r.part = r.gate_part = nullptr; r.gate = p.gate; r.blocks = r.chunks = 0;
-    r.cols = p.cols; r.gate_kind = p.gate_kind; r.gate_tanh = p.gate_tanh;
+    bool vec;
+    RnParams p = rn_params(d, &vec);
     HH_REQUIRE((p.gate_kind == HH_GATE_NONE) == (d->dgate == nullptr) && (p.g1 != nullptr) == (d->dpost_gamma != nullptr) && (p.g2 != nullptr) == (d->dpre_gamma != nullptr) &&
                    (p.b1 != nullptr || d->dpost_beta == nullptr) && (p.b2 != nullptr || d->dpre_beta == nullptr),
                HH_ERR_ALIGN, "hh_residual_norm_bwd: a gradient's pointer comes with its parameter's");
+    RnPlan q = {0, 0, 0, 0, 0, 0};                                     // (no rows: every sum is over nothing, and the second launch writes zeros)
     if (d->rows > 0) {
-        const RnPlan q = rn_plan(d->rows, d->groups);
+        q = rn_plan(d->rows, p.cols, d->groups);
         HH_REQUIRE(d->workspace != nullptr && HH_ALIGNED16(d->workspace), HH_ERR_ALIGN, "hh_residual_norm_bwd: a 16-byte aligned workspace is needed");
         p.part = (float*)d->workspace;
         p.gate_part = p.part + 4 * q.blocks * p.cols;
         p.chunk = q.chunk; p.chunks = q.chunks; p.units = q.units; p.per_block = q.per_block;
-        r.part = p.part; r.gate_part = p.gate_part; r.blocks = q.blocks; r.chunks = q.chunks;
-        const dim3 grid((unsigned)q.blocks);
-        RN_BY_COLS(resnorm_bwd_kernel, grid, grid);
+        const bool nt = d->rows * p.cols * (rn_size(p.x_dt) + rn_size(p.y_dt)) > HH_STREAM_BYTES;
+        const int threads = rn_waves(p.cols) * 64;
+#define RB(PO, PR, V, N) hipLaunchKernelGGL((resnorm_bwd_kernel<RN_BWD_ROWS, PO, PR, V, N>), dim3((unsigned)q.blocks), dim3(threads), 0, s, p)
+#define RBN(PO, PR) do { if (!vec) RB(PO, PR, false, false); else if (nt) RB(PO, PR, true, true); else RB(PO, PR, true, false); } while (0)
+        if (p.g1 && p.g2) RBN(true, true);
+        else if (p.g1) RBN(true, false);
+        else if (p.g2) RBN(false, true);
+        else RBN(false, false);
+#undef RBN
+#undef RB
     }
-    // (no rows: every sum is over nothing, and the launches below write zeros)
-    if (p.gate_kind == HH_GATE_SCALAR) {
-        hipLaunchKernelGGL(resnorm_scalar_gate_kernel, dim3(1), dim3(1024), 0, s, r.gate_part, d->rows ? r.chunks * p.cols : (int64_t)0, p.gate, p.gate_tanh, d->dgate);
-        r.dgate = nullptr;
-    }
-    if (p.g1 || p.g2 || r.dgate)
-        hipLaunchKernelGGL(resnorm_reduce_kernel, dim3((unsigned)((p.cols + 63) / 64), (unsigned)(4 + (r.dgate ? d->groups : 0))), dim3(1024), 0, s, r);
+    RnReduce r;
+    r.planes = 0;
+    float* outs[4] = {d->dpost_gamma, d->dpost_beta, d->dpre_gamma, d->dpre_beta};
+    for (int i = 0; i < 4; ++i)
+        if (outs[i]) {
+            r.part[r.planes] = p.part + (int64_t)i * q.blocks * p.cols;
+            r.out[r.planes++] = outs[i];
+        }
+    r.gate_part = p.gate_part; r.gate = p.gate; r.dgate = d->dgate;
+    r.blocks = q.blocks; r.chunks = q.chunks; r.units = q.units; r.groups = d->groups;
+    r.cols = p.cols; r.cols16 = (p.cols + 15) / 16; r.gate_kind = p.gate_kind; r.gate_tanh = p.gate_tanh;
+    const bool rowed = p.gate_kind == HH_GATE_CHANNEL || p.gate_kind == HH_GATE_GROUP;
+    r.wide_groups = rowed && d->groups <= RN_WIDE_GROUPS ? (int)d->groups : 0;
+    r.first_narrow = (int64_t)(r.planes + r.wide_groups) * r.cols16;
+    r.first_scalar = r.first_narrow + (rowed && !r.wide_groups ? (d->groups * p.cols + 1023) / 1024 : 0);
+    const int64_t grid = r.first_scalar + (p.gate_kind == HH_GATE_SCALAR);
+    if (grid) hipLaunchKernelGGL(resnorm_reduce_kernel, dim3((unsigned)grid), dim3(1024), 0, s, r);
     return hh_check_launch("hh_residual_norm_bwd");
 }
