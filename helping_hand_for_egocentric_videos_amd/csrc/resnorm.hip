@@ -26,36 +26,42 @@ struct RnParams {
     float* part;                       // [4][blocks][cols]: dgamma / dbeta of post, of pre
     float* gate_part;                  // [units][cols], or [units] for a scalar gate
     int64_t rows, each;                // rows of one gate group (all of them without groups)
-    int64_t chunk, chunks;             // rows of a unit, units of a group
+    int64_t chunks;                    // units of a group: unit j takes the rows j R .. j R + R - 1 and every chunks R-th behind them
     int64_t units, per_block;          // units in all, and of one workgroup
     int cols, gate_kind, gate_tanh, rms;
     int x_dt, y_dt, h_dt;
     float eps1, eps2, res_scale;
 };
 
+// Types: HH_F32, HH_BF16, or RN_ANY, read at run time -- the form for rows that take no wide accesses.
+#define RN_ANY 2
+template <int DT> __device__ __forceinline__ bool rn_f32(int dt) { return DT == RN_ANY ? dt == HH_F32 : DT == HH_F32; }
+// a row's address (the same in all lanes, so that a load is a scalar base and the lane's offset)
+template <int DT, typename T>
+__device__ __forceinline__ T* rn_row(T* base, int dt, int64_t off) { return base + off * (rn_f32<DT>(dt) ? 4 : 2); }
+
 // four channels as they lie in memory: 4 dwords of fp32, 2 of bf16; turned into fp32 only when all loads of a step have been issued (a conversion behind
-// each load would wait for it)
-template <bool VEC>
-__device__ __forceinline__ u32x4 rn_raw(const void* base, int dt, int64_t off, int c, int cols) {
+// each load would wait for it).  Channels behind the row's end are zero (VEC: the caller asks with c < cols).
+template <bool VEC, int DT>
+__device__ __forceinline__ u32x4 rn_raw(const char* row, int dt, int c, int cols) {
     u32x4 r = {0u, 0u, 0u, 0u};
     if (VEC) {
-        if (c < cols) {
-            if (dt == HH_F32) r = *(const u32x4*)((const float*)base + off + c);
-            else { const u32x2 t = *(const u32x2*)((const bf16_t*)base + off + c); r[0] = t[0]; r[1] = t[1]; }
-        }
+        if (rn_f32<DT>(dt)) r = *(const u32x4*)(row + (unsigned)(c * 4));
+        else { const u32x2 t = *(const u32x2*)(row + (unsigned)(c * 2)); r[0] = t[0]; r[1] = t[1]; }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (c + j < cols) {
-                if (dt == HH_F32) r[j] = ((const unsigned*)base)[off + c + j];
-                else r[j >> 1] |= (unsigned)((const unsigned short*)base)[off + c + j] << (16 * (j & 1));
+                if (rn_f32<DT>(dt)) r[j] = ((const unsigned*)row)[c + j];
+                else r[j >> 1] |= (unsigned)((const unsigned short*)row)[c + j] << (16 * (j & 1));
             }
     }
     return r;
 }
+template <int DT>
 __device__ __forceinline__ Q4 rn_cvt(const u32x4& r, int dt) {
     Q4 q;
-    if (dt == HH_F32) {
+    if (rn_f32<DT>(dt)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) q.v[j] = __uint_as_float(r[j]);
     } else {
@@ -65,30 +71,35 @@ __device__ __forceinline__ Q4 rn_cvt(const u32x4& r, int dt) {
     return q;
 }
 template <bool VEC>
-__device__ __forceinline__ Q4 rn_param(const float* base, int64_t off, int c, int cols) { return rn_cvt(rn_raw<VEC>(base, HH_F32, off, c, cols), HH_F32); }
+__device__ __forceinline__ Q4 rn_param(const float* base, int64_t off, int c, int cols) {
+    if (VEC && c >= cols) return Q4{{0.f, 0.f, 0.f, 0.f}};
+    return rn_cvt<HH_F32>(rn_raw<VEC, HH_F32>((const char*)(base + off), HH_F32, c, cols), HH_F32);
+}
 
-template <bool VEC, bool NT>
-__device__ __forceinline__ void rn_store(const Q4& q, void* base, int dt, int64_t off, int c, int cols) {
+template <bool VEC, bool NT, int DT>
+__device__ __forceinline__ void rn_store(const Q4& q, char* row, int dt, int c, int cols) {
     if (VEC) {
-        if (c < cols) {
-            if (dt == HH_F32) {
-                const f32x4 t = {q.v[0], q.v[1], q.v[2], q.v[3]};
-                f32x4* o = (f32x4*)((float*)base + off + c);
-                if (NT) __builtin_nontemporal_store(t, o); else *o = t;
-            } else {
-                const u32x2 t = {pack_bf16(q.v[0], q.v[1]), pack_bf16(q.v[2], q.v[3])};
-                u32x2* o = (u32x2*)((bf16_t*)base + off + c);
-                if (NT) __builtin_nontemporal_store(t, o); else *o = t;
-            }
+        if (rn_f32<DT>(dt)) {
+            const f32x4 t = {q.v[0], q.v[1], q.v[2], q.v[3]};
+            f32x4* o = (f32x4*)(row + (unsigned)(c * 4));
+            if (NT) __builtin_nontemporal_store(t, o); else *o = t;
+        } else {
+            const u32x2 t = {pack_bf16(q.v[0], q.v[1]), pack_bf16(q.v[2], q.v[3])};
+            u32x2* o = (u32x2*)(row + (unsigned)(c * 2));
+            if (NT) __builtin_nontemporal_store(t, o); else *o = t;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (c + j < cols) {
-                if (dt == HH_F32) ((float*)base)[off + c + j] = q.v[j];
-                else ((bf16_t*)base)[off + c + j] = (bf16_t)q.v[j];
+                if (rn_f32<DT>(dt)) ((float*)row)[c + j] = q.v[j];
+                else ((bf16_t*)row)[c + j] = (bf16_t)q.v[j];
             }
     }
+}
+template <bool VEC>
+__device__ __forceinline__ void rn_put(const Q4& q, float* row, int c, int cols) {
+    if (!VEC || c < cols) rn_store<VEC, false, HH_F32>(q, (char*)row, HH_F32, c, cols);
 }
 
 __device__ __forceinline__ float add_swapped32(float a, float b) {     // lanes 0..31: a over both halves, lanes 32..63: b
@@ -101,7 +112,7 @@ __device__ __forceinline__ float add_swapped16(float a, float b) {     // even r
 }
 template <int CTRL>
 __device__ __forceinline__ float add_dpp(float v) {
-    return v + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, false));
+    return v + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
 }
 __device__ __forceinline__ float add_row16(float v) {                  // sum over the 16 lanes of a row, in every lane of it (row rotations)
     return add_dpp<0x121>(add_dpp<0x122>(add_dpp<0x124>(add_dpp<0x128>(v))));
@@ -109,8 +120,13 @@ __device__ __forceinline__ float add_row16(float v) {                  // sum ov
 
 // N values (1, 2, 4 or 8) summed over the workgroup, in every lane.  A wave halves the number of values that a lane holds with the number of lanes that hold a
 // value (8 values: 20 instructions instead of 48 exchanges), the waves meet in LDS.  `turn` alternates between two buffers: a wave writes a buffer again
-// only behind the barrier of the sums in between, which every wave passes after it has read.
-struct RnRed { float buf[2][16 * 8]; };
+// only behind the barrier of the sums in between, which every wave passes after it has read.  Places of waves that there are not hold zeros (four are read
+// at once).
+struct RnRed { __attribute__((aligned(16))) float buf[2][16 * 8]; };
+__device__ __forceinline__ void rn_clear(RnRed& red) {
+    for (int i = threadIdx.x; i < 2 * 16 * 8; i += blockDim.x) red.buf[0][i] = 0.f;
+    __syncthreads();
+}
 template <int N>
 __device__ __forceinline__ void block_sums(float (&s)[N], RnRed& red, int& turn, int waves) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -124,48 +140,60 @@ __device__ __forceinline__ void block_sums(float (&s)[N], RnRed& red, int& turn,
         for (int i = 0; i < N / 4; ++i) u[i] = add_row16(add_swapped16(t[i], t[i + N / 4]));
         if ((lane & 15) == 0)
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i) buf[wave * N + (lane >> 4) * (N / 4) + i] = u[i];
+            for (int i = 0; i < N / 4; ++i) buf[wave * 8 + (lane >> 4) * (N / 4) + i] = u[i];
     } else if constexpr (N == 2) {
         float t = add_swapped32(s[0], s[1]);
         t = add_row16(add_swapped16(t, t));
-        if ((lane & 31) == 0) buf[wave * 2 + (lane >> 5)] = t;
+        if ((lane & 31) == 0) buf[wave * 8 + (lane >> 5)] = t;
     } else {
         float t = add_swapped32(s[0], s[0]);
         t = add_row16(add_swapped16(t, t));
-        if (lane == 0) buf[wave] = t;
+        if (lane == 0) buf[wave * 8] = t;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = 0.f;
-    for (int w = 0; w < waves; ++w)
+    for (int w = 0; w < waves; w += 4) {
+        f32x4 a[4], b[4];
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] += buf[w * N + i];
+        for (int k = 0; k < 4; ++k) {
+            a[k] = *(const f32x4*)(buf + (w + k) * 8);
+            if constexpr (N == 8) b[k] = *(const f32x4*)(buf + (w + k) * 8 + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += i < 4 ? (a[0][i & 3] + a[1][i & 3]) + (a[2][i & 3] + a[3][i & 3]) : (b[0][i & 3] + b[1][i & 3]) + (b[2][i & 3] + b[3][i & 3]);
+    }
+}
+
+// sum of a lane's four channels.  KNOWN: channels behind the row's end hold zeros already
+template <bool KNOWN>
+__device__ __forceinline__ float rn_sum4(const Q4& q, int c, int cols) {
+    if (KNOWN) return (q.v[0] + q.v[1]) + (q.v[2] + q.v[3]);
+    return ((c < cols ? q.v[0] : 0.f) + (c + 1 < cols ? q.v[1] : 0.f)) + ((c + 2 < cols ? q.v[2] : 0.f) + (c + 3 < cols ? q.v[3] : 0.f));
 }
 
 // mean and reciprocal standard deviation (or root mean square, with mean 0) of N rows; two passes
-template <int N>
-__device__ __forceinline__ void rn_stats(const Q4 (&v)[N], const bool (&in)[4], float inv, int rms, const float (&eps)[N], RnRed& red, int& turn, int waves, float (&mean)[N], float (&rstd)[N]) {
+template <bool VEC, bool KNOWN, int N>
+__device__ __forceinline__ void rn_stats(const Q4 (&v)[N], int c, int cols, float inv, int rms, const float (&eps)[N], RnRed& red, int& turn, int waves, float (&mean)[N], float (&rstd)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) mean[i] = 0.f;
     if (!rms) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) mean[i] = ((in[0] ? v[i].v[0] : 0.f) + (in[1] ? v[i].v[1] : 0.f)) + ((in[2] ? v[i].v[2] : 0.f) + (in[3] ? v[i].v[3] : 0.f));
+        for (int i = 0; i < N; ++i) mean[i] = rn_sum4<KNOWN>(v[i], c, cols);
         block_sums<N>(mean, red, turn, waves);
 #pragma unroll
         for (int i = 0; i < N; ++i) mean[i] *= inv;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        rstd[i] = 0.f;
+        Q4 q;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float d = in[j] ? v[i].v[j] - mean[i] : 0.f;
-            rstd[i] += d * d;
-        }
+        for (int j = 0; j < 4; ++j) { const float d = v[i].v[j] - mean[i]; q.v[j] = d * d; }
+        rstd[i] = VEC ? (c < cols ? rn_sum4<true>(q, c, cols) : 0.f) : rn_sum4<false>(q, c, cols);
     }
     block_sums<N>(rstd, red, turn, waves);
 #pragma unroll
-    for (int i = 0; i < N; ++i) rstd[i] = 1.f / sqrtf(rstd[i] * inv + eps[i]);
+    for (int i = 0; i < N; ++i) rstd[i] = rsqrtf(rstd[i] * inv + eps[i]);
 }
 
 template <bool VEC>
@@ -184,30 +212,36 @@ __device__ __forceinline__ Q4 rn_gate(const RnParams& p, int64_t group, int c) {
     return g;
 }
 
-template <int R, bool VEC, bool NT>
+template <int R, bool VEC, bool NT, int XT, int YT, int HT>
 __global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
     __shared__ RnRed red;
     const int waves = blockDim.x >> 6, c = threadIdx.x * 4;
+    const bool on = !VEC || c < p.cols;
     const float inv = 1.f / (float)p.cols;
-    bool in[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) in[j] = c + j < p.cols;
+    const Q4 zero = {{0.f, 0.f, 0.f, 0.f}};
     const int64_t r0 = (int64_t)blockIdx.x * R;
     u32x4 rx[R], ry[R];
-    int64_t off[R];
+    int64_t row[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        off[i] = (r0 + i < p.rows ? r0 + i : p.rows - 1) * p.cols;       // (behind the last row: that row once more, not stored)
-        rx[i] = rn_raw<VEC>(p.x, p.x_dt, off[i], c, p.cols);
-        ry[i] = rn_raw<VEC>(p.y, p.y_dt, off[i], c, p.cols);
+        row[i] = r0 + i < p.rows ? r0 + i : p.rows - 1;                  // (behind the last row: that row once more, not stored)
+        rx[i] = ry[i] = (u32x4){0u, 0u, 0u, 0u};
     }
+    if (on) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            rx[i] = rn_raw<VEC, XT>(rn_row<XT>((const char*)p.x, p.x_dt, row[i] * p.cols), p.x_dt, c, p.cols);
+            ry[i] = rn_raw<VEC, YT>(rn_row<YT>((const char*)p.y, p.y_dt, row[i] * p.cols), p.y_dt, c, p.cols);
+        }
+    }
+    rn_clear(red);
     int turn = 0;
-    Q4 g1, b1, g2, b2, gate[R];
-    if (p.g1) { g1 = rn_param<VEC>(p.g1, 0, c, p.cols); b1 = p.b1 ? rn_param<VEC>(p.b1, 0, c, p.cols) : Q4{{0.f, 0.f, 0.f, 0.f}}; }
-    if (p.g2) { g2 = rn_param<VEC>(p.g2, 0, c, p.cols); b2 = p.b2 ? rn_param<VEC>(p.b2, 0, c, p.cols) : Q4{{0.f, 0.f, 0.f, 0.f}}; }
+    Q4 g1 = zero, b1 = zero, g2 = zero, b2 = zero, gate[R];
+    if (p.g1) { g1 = rn_param<VEC>(p.g1, 0, c, p.cols); if (p.b1) b1 = rn_param<VEC>(p.b1, 0, c, p.cols); }
+    if (p.g2) { g2 = rn_param<VEC>(p.g2, 0, c, p.cols); if (p.b2) b2 = rn_param<VEC>(p.b2, 0, c, p.cols); }
     if (p.gate_kind == HH_GATE_GROUP) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) gate[i] = rn_gate<VEC>(p, (r0 + i < p.rows ? r0 + i : p.rows - 1) / p.each, c);
+        for (int i = 0; i < R; ++i) gate[i] = rn_gate<VEC>(p, row[i] / p.each, c);
     } else {
         gate[0] = rn_gate<VEC>(p, 0, c);
 #pragma unroll
@@ -216,11 +250,11 @@ __global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
     Q4 x[R], y[R];
     float mean[R], rstd[R], eps[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) { x[i] = rn_cvt(rx[i], p.x_dt); y[i] = rn_cvt(ry[i], p.y_dt); }
+    for (int i = 0; i < R; ++i) { x[i] = rn_cvt<XT>(rx[i], p.x_dt); y[i] = rn_cvt<YT>(ry[i], p.y_dt); }
     if (p.g1) {
 #pragma unroll
         for (int i = 0; i < R; ++i) eps[i] = p.eps1;
-        rn_stats<R>(y, in, inv, p.rms, eps, red, turn, waves, mean, rstd);
+        rn_stats<VEC, true, R>(y, c, p.cols, inv, p.rms, eps, red, turn, waves, mean, rstd);
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -230,37 +264,36 @@ __global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
     for (int i = 0; i < R; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[i].v[j] = x[i].v[j] * p.res_scale + gate[i].v[j] * y[i].v[j];
-        if (r0 + i < p.rows) rn_store<VEC, NT>(x[i], p.x_new, p.x_dt, off[i], c, p.cols);
+        if (r0 + i < p.rows && on) rn_store<VEC, NT, XT>(x[i], rn_row<XT>((char*)p.x_new, p.x_dt, row[i] * p.cols), p.x_dt, c, p.cols);
     }
     if (p.g2) {
 #pragma unroll
         for (int i = 0; i < R; ++i) eps[i] = p.eps2;
-        rn_stats<R>(x, in, inv, p.rms, eps, red, turn, waves, mean, rstd);
+        rn_stats<VEC, false, R>(x, c, p.cols, inv, p.rms, eps, red, turn, waves, mean, rstd);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[i].v[j] = (x[i].v[j] - mean[i]) * rstd[i] * g2.v[j] + b2.v[j];
-            if (r0 + i < p.rows) rn_store<VEC, NT>(x[i], p.h, p.h_dt, off[i], c, p.cols);
+            if (r0 + i < p.rows && on) rn_store<VEC, NT, HT>(x[i], rn_row<HT>((char*)p.h, p.h_dt, row[i] * p.cols), p.h_dt, c, p.cols);
         }
     }
 }
 
-template <int R, bool POST, bool PRE, bool VEC, bool NT>
+template <int R, bool POST, bool PRE, bool VEC, bool NT, int XT, int YT, int HT>
 __global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
     __shared__ RnRed red;
     const int waves = blockDim.x >> 6, c = threadIdx.x * 4;
+    const bool on = !VEC || c < p.cols;
     const float inv = 1.f / (float)p.cols;
     const Q4 zero = {{0.f, 0.f, 0.f, 0.f}};
-    bool in[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) in[j] = c + j < p.cols;
+    const u32x4 none = {0u, 0u, 0u, 0u};
+    rn_clear(red);
     int turn = 0;
     Q4 g2 = zero, ag1 = zero, ab1 = zero, ag2 = zero, ab2 = zero;
     if (PRE) g2 = rn_param<VEC>(p.g2, 0, c, p.cols);
     const int64_t u0 = blockIdx.x * p.per_block, u1 = u0 + p.per_block < p.units ? u0 + p.per_block : p.units;
     for (int64_t u = u0; u < u1; ++u) {
-        const int64_t group = u / p.chunks, first = (u % p.chunks) * p.chunk;
-        const int64_t last = first + p.chunk < p.each ? first + p.chunk : p.each;
+        const int64_t group = u / p.chunks, first = group * p.each + (u % p.chunks) * R, last = (group + 1) * p.each;
         const Q4 gate = rn_gate<VEC>(p, group, c);
         Q4 w = gate, s0 = zero, s1 = zero;                               // w: g o gamma of post
         if (POST) {
@@ -268,19 +301,21 @@ __global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) w.v[j] *= gate.v[j];
         }
-        for (int64_t r = first; r < last; r += R) {
+        for (int64_t r = first; r < last; r += p.chunks * R) {
             u32x4 rx[R], rh[R], rd[R], ry[R];
-            int64_t off[R];
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                // behind the unit's last row: that row once more, with gradients of zero, and not stored
-                off[i] = (group * p.each + (r + i < last ? r + i : last - 1)) * p.cols;
-                if (PRE) rx[i] = rn_raw<VEC>(p.x_new, p.x_dt, off[i], c, p.cols);
-                ry[i] = rn_raw<VEC>(p.y, p.y_dt, off[i], c, p.cols);
-                rd[i] = rh[i] = (u32x4){0u, 0u, 0u, 0u};
-                if (r + i < last) {
-                    if (PRE) rh[i] = rn_raw<VEC>(p.dh, p.h_dt, off[i], c, p.cols);
-                    if (p.dx_new) rd[i] = rn_raw<VEC>(p.dx_new, p.x_dt, off[i], c, p.cols);
+            for (int i = 0; i < R; ++i) rx[i] = rh[i] = rd[i] = ry[i] = none;
+            if (on) {
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    // behind the group's last row: that row once more, with gradients of zero, and not stored
+                    const int64_t off = (r + i < last ? r + i : last - 1) * p.cols;
+                    if (PRE) rx[i] = rn_raw<VEC, XT>(rn_row<XT>((const char*)p.x_new, p.x_dt, off), p.x_dt, c, p.cols);
+                    ry[i] = rn_raw<VEC, YT>(rn_row<YT>((const char*)p.y, p.y_dt, off), p.y_dt, c, p.cols);
+                    if (i == 0 || r + i < last) {
+                        if (PRE) rh[i] = rn_raw<VEC, HT>(rn_row<HT>((const char*)p.dh, p.h_dt, off), p.h_dt, c, p.cols);
+                        if (p.dx_new) rd[i] = rn_raw<VEC, XT>(rn_row<XT>((const char*)p.dx_new, p.x_dt, off), p.x_dt, c, p.cols);
+                    }
                 }
             }
             float mean[2 * R], rstd[2 * R], s[2 * R];
@@ -292,34 +327,34 @@ __global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
                     float eps[2 * R];
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
-                        xy[i] = rn_cvt(rx[i], p.x_dt); xy[R + i] = rn_cvt(ry[i], p.y_dt);
+                        xy[i] = rn_cvt<XT>(rx[i], p.x_dt); xy[R + i] = rn_cvt<YT>(ry[i], p.y_dt);
                         eps[i] = p.eps2; eps[R + i] = p.eps1;
                     }
-                    rn_stats<2 * R>(xy, in, inv, p.rms, eps, red, turn, waves, mean, rstd);
+                    rn_stats<VEC, true, 2 * R>(xy, c, p.cols, inv, p.rms, eps, red, turn, waves, mean, rstd);
 #pragma unroll
                     for (int i = 0; i < R; ++i) { x[i] = xy[i]; y[i] = xy[R + i]; }
                 } else {
                     float eps[R], m[R], q[R];
 #pragma unroll
-                    for (int i = 0; i < R; ++i) { x[i] = rn_cvt(rx[i], p.x_dt); y[i] = rn_cvt(ry[i], p.y_dt); eps[i] = p.eps2; }
-                    rn_stats<R>(x, in, inv, p.rms, eps, red, turn, waves, m, q);
+                    for (int i = 0; i < R; ++i) { x[i] = rn_cvt<XT>(rx[i], p.x_dt); y[i] = rn_cvt<YT>(ry[i], p.y_dt); eps[i] = p.eps2; }
+                    rn_stats<VEC, true, R>(x, c, p.cols, inv, p.rms, eps, red, turn, waves, m, q);
 #pragma unroll
                     for (int i = 0; i < R; ++i) { mean[i] = m[i]; rstd[i] = q[i]; }
                 }
                 Q4 k[R];
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
-                    k[i] = rn_cvt(rh[i], p.h_dt);
-                    d[i] = rn_cvt(rd[i], p.x_dt);
+                    k[i] = rn_cvt<HT>(rh[i], p.h_dt);
+                    d[i] = rn_cvt<XT>(rd[i], p.x_dt);
                     s[i] = s[R + i] = 0.f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float xh = (x[i].v[j] - mean[i]) * rstd[i];
                         ag2.v[j] += k[i].v[j] * xh;
                         ab2.v[j] += k[i].v[j];
-                        k[i].v[j] *= g2.v[j];
-                        s[i] += in[j] ? k[i].v[j] : 0.f;
-                        s[R + i] += in[j] ? k[i].v[j] * xh : 0.f;
+                        k[i].v[j] *= g2.v[j];                            // (channels behind the row's end: dh and gamma are zero there)
+                        s[i] += k[i].v[j];
+                        s[R + i] += k[i].v[j] * xh;
                         x[i].v[j] = xh;
                     }
                 }
@@ -332,16 +367,17 @@ __global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < R; ++i) { y[i] = rn_cvt(ry[i], p.y_dt); d[i] = rn_cvt(rd[i], p.x_dt); }
+                for (int i = 0; i < R; ++i) { y[i] = rn_cvt<YT>(ry[i], p.y_dt); d[i] = rn_cvt<XT>(rd[i], p.x_dt); }
                 if constexpr (POST) {
                     float eps[R], m[R], q[R];
 #pragma unroll
                     for (int i = 0; i < R; ++i) eps[i] = p.eps1;
-                    rn_stats<R>(y, in, inv, p.rms, eps, red, turn, waves, m, q);
+                    rn_stats<VEC, true, R>(y, c, p.cols, inv, p.rms, eps, red, turn, waves, m, q);
 #pragma unroll
                     for (int i = 0; i < R; ++i) { mean[R + i] = m[i]; rstd[R + i] = q[i]; }
                 }
             }
+            // (a row behind the group's last has d = 0 - rstd * (0 - 0 - xh * 0) = 0: its gradients are zero, so it adds nothing below either)
             if constexpr (POST) {
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
@@ -349,12 +385,11 @@ __global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float xh = (y[i].v[j] - mean[R + i]) * rstd[R + i];
-                        const float dj = r + i < last ? d[i].v[j] : 0.f;
-                        s0.v[j] += dj;
-                        s1.v[j] += dj * xh;
-                        const float k = d[i].v[j] * w.v[j];
-                        s[i] += in[j] ? k : 0.f;
-                        s[R + i] += in[j] ? k * xh : 0.f;
+                        s0.v[j] += d[i].v[j];
+                        s1.v[j] += d[i].v[j] * xh;
+                        const float k = d[i].v[j] * w.v[j];              // (channels behind the row's end: w is zero there)
+                        s[i] += k;
+                        s[R + i] += k * xh;
                         y[i].v[j] = xh;
                     }
                 }
@@ -370,18 +405,21 @@ __global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
                 for (int i = 0; i < R; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        s1.v[j] += r + i < last ? d[i].v[j] * y[i].v[j] : 0.f;
+                        s1.v[j] += d[i].v[j] * y[i].v[j];
                         y[i].v[j] = d[i].v[j] * w.v[j];
                     }
             }
+            if (on) {
 #pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (r + i < last) {
-                    rn_store<VEC, NT>(y[i], p.dy, p.y_dt, off[i], c, p.cols);
+                for (int i = 0; i < R; ++i)
+                    if (i == 0 || r + i < last) {
+                        const int64_t off = (r + i) * p.cols;
+                        rn_store<VEC, NT, YT>(y[i], rn_row<YT>((char*)p.dy, p.y_dt, off), p.y_dt, c, p.cols);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) d[i].v[j] *= p.res_scale;
-                    rn_store<VEC, NT>(d[i], p.dx, p.x_dt, off[i], c, p.cols);
-                }
+                        for (int j = 0; j < 4; ++j) d[i].v[j] *= p.res_scale;
+                        rn_store<VEC, NT, XT>(d[i], rn_row<XT>((char*)p.dx, p.x_dt, off), p.x_dt, c, p.cols);
+                    }
+            }
         }
         Q4 t = s1;                                                       // the unit's share of the gate's gradient: sum d o p
         if constexpr (POST) {
@@ -395,21 +433,22 @@ __global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
             }
         }
         if (p.gate_kind == HH_GATE_SCALAR) {
-            float sum[1] = {((in[0] ? t.v[0] : 0.f) + (in[1] ? t.v[1] : 0.f)) + ((in[2] ? t.v[2] : 0.f) + (in[3] ? t.v[3] : 0.f))};
+            float sum[1] = {rn_sum4<false>(t, c, p.cols)};
             block_sums<1>(sum, red, turn, waves);
             if (threadIdx.x == 0) p.gate_part[u] = sum[0];
         } else if (p.gate_kind != HH_GATE_NONE) {
-            rn_store<VEC, false>(t, p.gate_part, HH_F32, u * p.cols, c, p.cols);
+            rn_put<VEC>(t, p.gate_part + u * p.cols, c, p.cols);
         }
     }
-    const int64_t plane = (int64_t)gridDim.x * p.cols, at = blockIdx.x * (int64_t)p.cols;
+    const int64_t plane = (int64_t)gridDim.x * p.cols;
+    float* out = p.part + blockIdx.x * (int64_t)p.cols;
     if constexpr (POST) {
-        rn_store<VEC, false>(ag1, p.part, HH_F32, at, c, p.cols);
-        rn_store<VEC, false>(ab1, p.part, HH_F32, plane + at, c, p.cols);
+        rn_put<VEC>(ag1, out, c, p.cols);
+        rn_put<VEC>(ab1, out + plane, c, p.cols);
     }
     if constexpr (PRE) {
-        rn_store<VEC, false>(ag2, p.part, HH_F32, 2 * plane + at, c, p.cols);
-        rn_store<VEC, false>(ab2, p.part, HH_F32, 3 * plane + at, c, p.cols);
+        rn_put<VEC>(ag2, out + 2 * plane, c, p.cols);
+        rn_put<VEC>(ab2, out + 3 * plane, c, p.cols);
     }
 }
 
@@ -495,18 +534,14 @@ __global__ __launch_bounds__(1024) void resnorm_reduce_kernel(RnReduce p) {
 #endif
 static int rn_waves(int cols) { return (cols + 255) / 256; }
 
-struct RnPlan { int64_t each, chunk, chunks, units, per_block, blocks; };
+struct RnPlan { int64_t chunks, units, per_block, blocks; };
 // about 4096 waves (four to a SIMD) in workgroups that take whole units of one gate group's rows; a unit leaves four partial rows, so it has 16 rows if there are
 static RnPlan rn_plan(int64_t rows, int cols, int64_t groups) {
     RnPlan q;
     const int64_t blocks = 4096 / rn_waves(cols);
-    q.each = rows / groups;
-    int64_t want = (blocks + groups - 1) / groups;
-    const int64_t most = (q.each + 15) / 16;
-    if (want > most) want = most;
-    if (want < 1) want = 1;
-    q.chunk = (q.each + want - 1) / want;
-    q.chunks = (q.each + q.chunk - 1) / q.chunk;
+    const int64_t most = (rows / groups + 15) / 16;
+    q.chunks = (blocks + groups - 1) / groups;
+    if (q.chunks > most) q.chunks = most;
     q.units = q.chunks * groups;
     q.per_block = (q.units + blocks - 1) / blocks;
     q.blocks = (q.units + q.per_block - 1) / q.per_block;
@@ -536,7 +571,7 @@ static RnParams rn_params(const hh_residual_norm* d, bool* vec) {
     p.x = d->x; p.y = d->y; p.x_new = d->x_new; p.h = d->h; p.dx_new = d->dx_new; p.dh = d->dh; p.dx = d->dx; p.dy = d->dy;
     p.gate = d->gate; p.g1 = d->post_gamma; p.b1 = d->post_beta; p.g2 = d->pre_gamma; p.b2 = d->pre_beta;
     p.part = p.gate_part = nullptr;
-    p.rows = d->rows; p.each = d->rows / d->groups; p.chunk = p.chunks = p.units = p.per_block = 0;
+    p.rows = d->rows; p.each = d->rows / d->groups; p.chunks = p.units = p.per_block = 0;
     p.cols = d->cols; p.gate_kind = d->gate_kind; p.gate_tanh = d->gate_tanh; p.rms = d->rms;
     p.x_dt = d->x_dtype; p.y_dt = d->y_dtype; p.h_dt = d->h_dtype;
     p.eps1 = d->post_eps; p.eps2 = d->pre_eps; p.res_scale = d->res_scale;
@@ -555,10 +590,15 @@ extern "C" int hh_residual_norm_fwd(const hh_residual_norm* d, hh_stream_t strea
     const RnParams p = rn_params(d, &vec);
     const bool nt = d->rows * d->cols * (rn_size(p.x_dt) + (p.h ? rn_size(p.h_dt) : 0)) > HH_STREAM_BYTES;
     const int threads = rn_waves(p.cols) * 64;
-#define RF(R, V, N) hipLaunchKernelGGL((resnorm_fwd_kernel<R, V, N>), dim3((unsigned)((d->rows + R - 1) / R)), dim3(threads), 0, s, p)
+#define RF(R, V, N, X, Y, H) hipLaunchKernelGGL((resnorm_fwd_kernel<R, V, N, X, Y, H>), dim3((unsigned)((d->rows + R - 1) / R)), dim3(threads), 0, s, p)
+#define RFN(X, Y, H) do { if (d->rows < RN_FWD_MANY) RF(1, true, false, X, Y, H); else if (nt) RF(4, true, true, X, Y, H); else RF(4, true, false, X, Y, H); } while (0)
+#define RFH(X, Y) do { if (p.h_dt == HH_F32) RFN(X, Y, HH_F32); else RFN(X, Y, HH_BF16); } while (0)
     // four rows to a workgroup where that still leaves work for every CU, one where a short call is all latency
-    if (d->rows >= RN_FWD_MANY) { if (!vec) RF(4, false, false); else if (nt) RF(4, true, true); else RF(4, true, false); }
-    else { if (vec) RF(1, true, false); else RF(1, false, false); }
+    if (!vec) { if (d->rows >= RN_FWD_MANY) RF(4, false, false, RN_ANY, RN_ANY, RN_ANY); else RF(1, false, false, RN_ANY, RN_ANY, RN_ANY); }
+    else if (p.x_dt == HH_F32) { if (p.y_dt == HH_F32) RFH(HH_F32, HH_F32); else RFH(HH_F32, HH_BF16); }
+    else { if (p.y_dt == HH_F32) RFH(HH_BF16, HH_F32); else RFH(HH_BF16, HH_BF16); }
+#undef RFH
+#undef RFN
 #undef RF
     return hh_check_launch("hh_residual_norm_fwd");
 }
@@ -579,21 +619,25 @@ extern "C" int hh_residual_norm_bwd(const hh_residual_norm* d, hh_stream_t strea
     HH_REQUIRE((p.gate_kind == HH_GATE_NONE) == (d->dgate == nullptr) && (p.g1 != nullptr) == (d->dpost_gamma != nullptr) && (p.g2 != nullptr) == (d->dpre_gamma != nullptr) &&
                    (p.b1 != nullptr || d->dpost_beta == nullptr) && (p.b2 != nullptr || d->dpre_beta == nullptr),
                HH_ERR_ALIGN, "hh_residual_norm_bwd: a gradient's pointer comes with its parameter's");
-    RnPlan q = {0, 0, 0, 0, 0, 0};                                     // (no rows: every sum is over nothing, and the second launch writes zeros)
+    RnPlan q = {0, 0, 0, 0};                                     // (no rows: every sum is over nothing, and the second launch writes zeros)
     if (d->rows > 0) {
         q = rn_plan(d->rows, p.cols, d->groups);
         HH_REQUIRE(d->workspace != nullptr && HH_ALIGNED16(d->workspace), HH_ERR_ALIGN, "hh_residual_norm_bwd: a 16-byte aligned workspace is needed");
         p.part = (float*)d->workspace;
         p.gate_part = p.part + 4 * q.blocks * p.cols;
-        p.chunk = q.chunk; p.chunks = q.chunks; p.units = q.units; p.per_block = q.per_block;
+        p.chunks = q.chunks; p.units = q.units; p.per_block = q.per_block;
         const bool nt = d->rows * p.cols * (rn_size(p.x_dt) + rn_size(p.y_dt)) > HH_STREAM_BYTES;
         const int threads = rn_waves(p.cols) * 64;
-#define RB(PO, PR, V, N) hipLaunchKernelGGL((resnorm_bwd_kernel<RN_BWD_ROWS, PO, PR, V, N>), dim3((unsigned)q.blocks), dim3(threads), 0, s, p)
-#define RBN(PO, PR) do { if (!vec) RB(PO, PR, false, false); else if (nt) RB(PO, PR, true, true); else RB(PO, PR, true, false); } while (0)
-        if (p.g1 && p.g2) RBN(true, true);
-        else if (p.g1) RBN(true, false);
-        else if (p.g2) RBN(false, true);
-        else RBN(false, false);
+#define RB(PO, PR, V, N, X, Y, H) hipLaunchKernelGGL((resnorm_bwd_kernel<RN_BWD_ROWS, PO, PR, V, N, X, Y, H>), dim3((unsigned)q.blocks), dim3(threads), 0, s, p)
+#define RBN(PO, PR, X, Y, H) do { if (nt) RB(PO, PR, true, true, X, Y, H); else RB(PO, PR, true, false, X, Y, H); } while (0)
+#define RBY(PO, PR, X, H) do { if (p.y_dt == HH_F32) RBN(PO, PR, X, HH_F32, H); else RBN(PO, PR, X, HH_BF16, H); } while (0)
+#define RBX(PO, PR, H) do { if (!vec) RB(PO, PR, false, false, RN_ANY, RN_ANY, RN_ANY); else if (p.x_dt == HH_F32) RBY(PO, PR, HH_F32, H); else RBY(PO, PR, HH_BF16, H); } while (0)
+        if (p.g1 && p.g2) { if (p.h_dt == HH_F32) RBX(true, true, HH_F32); else RBX(true, true, HH_BF16); }
+        else if (p.g2) { if (p.h_dt == HH_F32) RBX(false, true, HH_F32); else RBX(false, true, HH_BF16); }
+        else if (p.g1) RBX(true, false, HH_F32);
+        else RBX(false, false, HH_F32);
+#undef RBX
+#undef RBY
 #undef RBN
 #undef RB
     }
