@@ -42,12 +42,18 @@ __device__ __forceinline__ T* rn_row(T* base, int dt, int64_t off) { return base
 
 // four channels as they lie in memory: 4 dwords of fp32, 2 of bf16; turned into fp32 only when all loads of a step have been issued (a conversion behind
 // each load would wait for it).  Channels behind the row's end are zero (VEC: the caller asks with c < cols).
-template <bool VEC, int DT>
+template <bool VEC, int DT, bool NT = false>
 __device__ __forceinline__ u32x4 rn_raw(const char* row, int dt, int c, int cols) {
     u32x4 r = {0u, 0u, 0u, 0u};
     if (VEC) {
-        if (rn_f32<DT>(dt)) r = *(const u32x4*)(row + (unsigned)(c * 4));
-        else { const u32x2 t = *(const u32x2*)(row + (unsigned)(c * 2)); r[0] = t[0]; r[1] = t[1]; }
+        if (rn_f32<DT>(dt)) {
+            const u32x4* at = (const u32x4*)(row + (unsigned)(c * 4));
+            r = NT ? __builtin_nontemporal_load(at) : *at;
+        } else {
+            const u32x2* at = (const u32x2*)(row + (unsigned)(c * 2));
+            const u32x2 t = NT ? __builtin_nontemporal_load(at) : *at;
+            r[0] = t[0]; r[1] = t[1];
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -230,8 +236,8 @@ __global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
     if (on) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            rx[i] = rn_raw<VEC, XT>(rn_row<XT>((const char*)p.x, p.x_dt, row[i] * p.cols), p.x_dt, c, p.cols);
-            ry[i] = rn_raw<VEC, YT>(rn_row<YT>((const char*)p.y, p.y_dt, row[i] * p.cols), p.y_dt, c, p.cols);
+            rx[i] = rn_raw<VEC, XT, NT>(rn_row<XT>((const char*)p.x, p.x_dt, row[i] * p.cols), p.x_dt, c, p.cols);
+            ry[i] = rn_raw<VEC, YT, NT>(rn_row<YT>((const char*)p.y, p.y_dt, row[i] * p.cols), p.y_dt, c, p.cols);
         }
     }
     rn_clear(red);
@@ -310,11 +316,11 @@ __global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
                 for (int i = 0; i < R; ++i) {
                     // behind the group's last row: that row once more, with gradients of zero, and not stored
                     const int64_t off = (r + i < last ? r + i : last - 1) * p.cols;
-                    if (PRE) rx[i] = rn_raw<VEC, XT>(rn_row<XT>((const char*)p.x_new, p.x_dt, off), p.x_dt, c, p.cols);
-                    ry[i] = rn_raw<VEC, YT>(rn_row<YT>((const char*)p.y, p.y_dt, off), p.y_dt, c, p.cols);
+                    if (PRE) rx[i] = rn_raw<VEC, XT, NT>(rn_row<XT>((const char*)p.x_new, p.x_dt, off), p.x_dt, c, p.cols);
+                    ry[i] = rn_raw<VEC, YT, NT>(rn_row<YT>((const char*)p.y, p.y_dt, off), p.y_dt, c, p.cols);
                     if (i == 0 || r + i < last) {
-                        if (PRE) rh[i] = rn_raw<VEC, HT>(rn_row<HT>((const char*)p.dh, p.h_dt, off), p.h_dt, c, p.cols);
-                        if (p.dx_new) rd[i] = rn_raw<VEC, XT>(rn_row<XT>((const char*)p.dx_new, p.x_dt, off), p.x_dt, c, p.cols);
+                        if (PRE) rh[i] = rn_raw<VEC, HT, NT>(rn_row<HT>((const char*)p.dh, p.h_dt, off), p.h_dt, c, p.cols);
+                        if (p.dx_new) rd[i] = rn_raw<VEC, XT, NT>(rn_row<XT>((const char*)p.dx_new, p.x_dt, off), p.x_dt, c, p.cols);
                     }
                 }
             }

@@ -373,8 +373,8 @@ def test_act8(rows, cols, dt, act):
     assert none is None and torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, s)
     # exp within 4 steps and its argument (1.702 rounded, the product) within 2 U of itself, which exp turns into |1.702 v| times as much
     slack = lambda v: (16 + 4 * (1.702 * v).abs().clamp_max(100)) * U  # noqa: E731
-    # 1 + exp(x) ends at 2^128 in fp32: a sigmoid below 2^-128 (v below -52.1) is zero, which takes at most 2^-128 of what multiplies it
-    tiny = 2.0 ** -127
+    # a reciprocal below fp32's smallest normal number, 2^-126, is zero: a sigmoid there (v below -51.3) loses at most 2^-126 of what multiplies it
+    tiny = 2.0 ** -125
     ud = u.double()
     ra, _ = act_ref(ud, act)
     within(a, ra, (slack(ud) * ra.abs() if act == ops.ACT_QUICKGELU else 0) + stored(ra, dt) * (act == ops.ACT_QUICKGELU) + tiny * (1 + ud.abs()), "act8 a")
