@@ -7,6 +7,7 @@
 // tokens that a lane of the matrix instruction wants.  16-byte chunk c of row r lies at c ^ tn8_key(r), which spreads the four rows x 32 B that
 // a 16-lane group reads, and the rows 8 apart of the two groups of a half wave, over the banks.
 #include "common.h"
+#include <type_traits>
 
 typedef short s16x4_t8 __attribute__((ext_vector_type(4)));
 
@@ -16,152 +17,232 @@ __device__ __forceinline__ bf16x4 tn8_tr4(const char* addr) {
     return __builtin_bit_cast(bf16x4, r);
 }
 
+// d += a b.  PIN: in asm, with d in one accumulation register tuple for good -- with 256 accumulators hipcc otherwise permutes them between the products (700 copies in
+// the loop, half of its time).  Nothing but these products touches d inside the loop, and two products of one d are WT^2 - 1 others apart.
+template <bool PIN>
+__device__ __forceinline__ void tn8_mfma(f32x4& d, const bf16x8& a, const bf16x8& b) {
+    if constexpr (PIN) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(d) : "v"(a), "v"(b));
+    else d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, d, 0, 0, 0);
+}
+
 struct Tn8Params {
     const bf16_t* A; int64_t lda;
     const unsigned char* q; int64_t ldq;
     const float* scale;                    // [K][groups]
     float* C;                              // [splits][M][N]
-    float* colsum;                         // [splits][M] or NULL
-    int M, N, groups, tiles_n, vec_a, vec_q;
-    int64_t K, k_per_split;                // k_per_split: a multiple of 64
+    float* colsum;                         // [splits * tiles_n][M] or NULL
+    int M, N, groups, tiles_m, tiles_n, splits;
+    int64_t K, k_per_split;                // k_per_split: a multiple of the tile's tokens
 };
 
-__global__ __launch_bounds__(256, 2) void gemm_tn8_kernel(Tn8Params p) {
-    __shared__ __attribute__((aligned(16))) char smem[2 * 2 * 16384];        // [buffer][A | B][64 rows x 256 B]
+// One tile of the output for one slice of the tokens: 2 x 2 waves of (16 WT) x (16 WT), 32 tokens at a time.
+//
+// A step is 32 tokens: WT^2 matrix instructions on fragments that the previous step has read, while this one reads the next.  Each of the two
+// LDS buffers holds a tile; a step also puts the tile after next into LDS and requests the one two further on, which gives a request two tiles'
+// time.  WT = 8 (256 x 256, one wave to a SIMD, 256 accumulators): 16 KB of fragments feed 64 instructions of 16 cycles, 512 of whose 1024 cycles the four
+// waves' reads take of LDS; WT = 4 (128 x 128) reads as many bytes for a quarter of the products and is bound by LDS, and is for small outputs.
+template <int WT, bool VEC>
+__global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Params p) {
+    constexpr int BLOCK = 32 * WT, BK = 32, ROW = BLOCK * 2, HALF = BK * ROW;     // bytes of a row and of one operand's tile in LDS
+    constexpr int CA = BLOCK / 8, CQ = BLOCK / 16;                                       // 16-byte pieces of a row of dY / of q
+    constexpr int NA = BK * CA / 256, NQ = BK * CQ / 256, RA = 256 / CA, RQ = 256 / CQ;  // pieces for a thread, rows between them
+    constexpr int BUFS = 4;                                                               // tiles in LDS
+    extern __shared__ __attribute__((aligned(16))) char smem[];                           // [BUFS][dY | q][BK][BLOCK] bf16
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1;
-    const int m0 = (blockIdx.x / p.tiles_n) * 128, n0 = (blockIdx.x % p.tiles_n) * 128;
-    const int64_t k0 = (int64_t)blockIdx.y * p.k_per_split;
+    // work in the order slice, column tile, row tile; an XCD (blockIdx.x mod 8) takes a contiguous part of it, so that its L2 holds few columns of one slice
+    const int total = p.tiles_m * p.tiles_n * p.splits, tiles = p.tiles_m * p.tiles_n;
+    const int xcd = blockIdx.x & 7, per = total >> 3, extra = total & 7;
+    const int work = xcd * per + (xcd < extra ? xcd : extra) + (blockIdx.x >> 3);
+    const int split = work / tiles, tile_n = work % tiles / p.tiles_m, tile_m = work % tiles % p.tiles_m;
+    const int m0 = tile_m * BLOCK, n0 = tile_n * BLOCK;
+    const int64_t k0 = (int64_t)split * p.k_per_split;
     const int64_t k1 = k0 + p.k_per_split < p.K ? k0 + p.k_per_split : p.K;
-    const int nk = (int)((k1 - k0 + 63) / 64);                                // (0 for a slice behind the last token: zeros are written)
+    const int nk = k1 > k0 ? (int)((k1 - k0 + BK - 1) / BK) : 0;                        // (0 for a slice behind the last token: zeros are written)
 
-    u32x4 ra[4], rq[2];
-    float rs[2];
-    auto fetch = [&](int kt) {
+    // Columns behind the last are read from the first (their products are not stored); rows behind the slice's last are zero in dY, and q's last row again.
+    const int ra0 = tid / CA, rq0 = tid / CQ, ca = tid % CA, cq = tid % CQ;
+    const int am = m0 + ca * 8 < p.M ? m0 + ca * 8 : 0, qn = n0 + cq * 16 < p.N ? n0 + cq * 16 : 0;
+    const char* a_base = (const char*)(p.A + k0 * p.lda);                                 // the same in all lanes; a lane adds 32 bits
+    const char* q_base = (const char*)(p.q + k0 * p.ldq);
+    const char* s_base = (const char*)(p.scale + k0 * p.groups);
+    const int len = (int)(k1 - k0);                                                       // (K is at most 2^30)
+    const unsigned lda = (unsigned)p.lda * 2, ldq = (unsigned)p.ldq, lds = (unsigned)p.groups * 4;      // bytes; rows of a tile lie within 2^31 (checked by the caller)
+    struct Regs { u32x4 a[NA], q[NQ]; float s[NQ]; };
+    // piece i of tile t's rows of dY / of q
+    auto fetch_a = [&](int t, int i, Regs& r) {
+        const int kt = t * BK, row = ra0 + RA * i;
+        const bool cut = kt + BK > len;                                                   // (the same in all lanes)
+        const char* base = a_base + (int64_t)(cut ? 0 : kt) * lda;
+        const int64_t tail = kt + row < len ? kt + row : len - 1;
+        const char* src = cut ? base + tail * lda + (unsigned)am * 2 : base + ((unsigned)row * lda + (unsigned)am * 2);
+        if (VEC) r.a[i] = *(const u32x4*)src;
+        else {
+            r.a[i] = (u32x4){0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = tid + 256 * i;
-            const int64_t k = k0 + (int64_t)kt * 64 + (at >> 4);
-            const int m = m0 + (at & 15) * 8;
-            ra[i] = (u32x4){0u, 0u, 0u, 0u};
-            if (k < k1 && m < p.M) {
-                const bf16_t* src = p.A + k * p.lda + m;
-                if (p.vec_a) ra[i] = *(const u32x4*)src;
-                else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (m + j < p.M) ra[i][j >> 1] |= (unsigned)((const unsigned short*)src)[j] << (16 * (j & 1));
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int at = tid + 256 * i;
-            const int64_t k = k0 + (int64_t)kt * 64 + (at >> 3);
-            const int n = n0 + (at & 7) * 16;
-            rq[i] = (u32x4){0u, 0u, 0u, 0u};
-            rs[i] = 1.f;
-            if (k < k1 && n < p.N) {
-                const unsigned char* src = p.q + k * p.ldq + n;
-                if (p.vec_q) rq[i] = *(const u32x4*)src;
-                else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (n + j < p.N) rq[i][j >> 2] |= (unsigned)src[j] << (8 * (j & 3));
-                }
-                rs[i] = p.scale[k * p.groups + n / 128];
-            }
+            for (int j = 0; j < 8; ++j)
+                if (am + j < p.M) r.a[i][j >> 1] |= (unsigned)((const unsigned short*)src)[j] << (16 * (j & 1));
         }
     };
-    auto put = [&](int buf) {
-        char* dA = smem + buf * 32768;
-        char* dB = dA + 16384;
+    auto fetch_q = [&](int t, int i, Regs& r) {
+        const int kt = t * BK, row = rq0 + RQ * i;
+        const bool cut = kt + BK > len;
+        const char* base = q_base + (int64_t)(cut ? 0 : kt) * ldq;
+        const char* sbase = s_base + (int64_t)(cut ? 0 : kt) * lds;
+        const int64_t tail = kt + row < len ? kt + row : len - 1;
+        const char* src = cut ? base + tail * ldq + (unsigned)qn : base + ((unsigned)row * ldq + (unsigned)qn);
+        const char* ssrc = cut ? sbase + tail * lds + (unsigned)(qn / 128) * 4 : sbase + ((unsigned)row * lds + (unsigned)(qn / 128) * 4);
+        if (VEC) r.q[i] = *(const u32x4*)src;
+        else {
+            r.q[i] = (u32x4){0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = tid + 256 * i, r = at >> 4, c = at & 15;
-            *(u32x4*)(dA + r * 256 + ((c ^ tn8_key(r)) << 4)) = ra[i];
+            for (int j = 0; j < 16; ++j)
+                if (qn + j < p.N) r.q[i][j >> 2] |= (unsigned)((const unsigned char*)src)[j] << (8 * (j & 3));
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int at = tid + 256 * i, r = at >> 3, c = (at & 7) * 2;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32x4 w;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    w[2 * j] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rq[i][2 * h + j], rs[i], false));
-                    w[2 * j + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(rq[i][2 * h + j], rs[i], true));
-                }
-                *(u32x4*)(dB + r * 256 + (((c + h) ^ tn8_key(r)) << 4)) = w;
-            }
-        }
+        r.s[i] = *(const float*)ssrc;
     };
-    // 16-lane group g reads tokens 8 g .. 8 g + 7 (+ 32 for the second half of the 64); lane 4 qd + pc of the group gives the address of row qd, columns 4 pc ..
+    float db[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) db[j] = 0.f;
+    int db_tile = p.colsum != nullptr ? tile_n : -1;     // db: the column tiles share the tokens, each adds up every tiles_n-th tile's rows on their way into LDS
+    auto put_a = [&](int t, int i, Regs& r) {
+        const int row = ra0 + RA * i;
+        if ((t + 1) * BK > len && t * BK + row >= len) r.a[i] = (u32x4){0u, 0u, 0u, 0u};
+        if (t == db_tile) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { db[2 * j] += bf16_lo_to_f32(r.a[i][j]); db[2 * j + 1] += bf16_hi_to_f32(r.a[i][j]); }
+            if (i == NA - 1) db_tile += p.tiles_n;
+        }
+        *(u32x4*)(smem + (t & (BUFS - 1)) * 2 * HALF + row * ROW + ((ca ^ tn8_key(row)) << 4)) = r.a[i];
+    };
+    auto put_q = [&](int t, int i, int h, const Regs& r) {                                // half h of piece i: 8 values, 16 bytes of bf16
+        const int row = rq0 + RQ * i;
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            w[2 * j] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.q[i][2 * h + j], r.s[i], false));
+            w[2 * j + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.q[i][2 * h + j], r.s[i], true));
+        }
+        *(u32x4*)(smem + (t & (BUFS - 1)) * 2 * HALF + HALF + row * ROW + (((2 * cq + h) ^ tn8_key(row)) << 4)) = w;
+    };
+    auto fetch = [&](int t, Regs& r) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) fetch_a(t, i, r);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) fetch_q(t, i, r);
+    };
+    auto put = [&](int t, Regs& r) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) put_a(t, i, r);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) { put_q(t, i, 0, r); put_q(t, i, 1, r); }
+    };
+    static_assert(NA + 2 * NQ == WT, "the step below places these pieces");
+    // 16-lane group g reads tokens 8 g .. 8 g + 7 of a step; lane 4 qd + pc of the group gives the address of row qd, columns 4 pc .. 4 pc + 3 of 16
     const int g = lane >> 4, qd = (lane & 15) >> 2, pc = lane & 3;
-    auto frag = [&](const char* tile, int col0, int ks) -> bf16x8 {
-        const int r0 = 32 * ks + 8 * g + qd, r1 = r0 + 4;
-        const int ch = (col0 >> 3) + (pc >> 1);
-        const bf16x4 a = tn8_tr4(tile + r0 * 256 + ((ch ^ tn8_key(r0)) << 4) + (pc & 1) * 8);
-        const bf16x4 b = tn8_tr4(tile + r1 * 256 + ((ch ^ tn8_key(r1)) << 4) + (pc & 1) * 8);
+    // rows 4 apart have the same key; piece 2 i + (pc >> 1) of a row lies at 32 (i ^ (key >> 1)) bytes and the low bit: one address for each i
+    const int row = 8 * g + qd, key = tn8_key(row) >> 1;
+    const int low = row * ROW + ((pc >> 1) << 4) + (pc & 1) * 8;
+    int at_a[WT], at_b[WT];
+#pragma unroll
+    for (int i = 0; i < WT; ++i) {
+        const int ia = wm * WT + i, ib = wn * WT + i;
+        at_a[i] = low + (((ia & ~7) | ((ia & 7) ^ key)) << 5);
+        at_b[i] = low + HALF + (((ib & ~7) | ((ib & 7) ^ key)) << 5);
+    }
+    auto frag = [&](int at, int buf) -> bf16x8 {
+        const char* base = smem + at + (buf & (BUFS - 1)) * 2 * HALF;
+        const bf16x4 a = tn8_tr4(base), b = tn8_tr4(base + 4 * ROW);
         return (bf16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     };
-
-    const bool want_cs = p.colsum != nullptr && n0 == 0 && wn == 0;            // db: one more product, against ones
-    const bf16x8 ones = {(bf16_t)1.f, (bf16_t)1.f, (bf16_t)1.f, (bf16_t)1.f, (bf16_t)1.f, (bf16_t)1.f, (bf16_t)1.f, (bf16_t)1.f};
-    f32x4 cs[4], acc[4][4];                                                    // acc[tn][tm]: rows n, columns m
+    auto frag_a = [&](int buf, int i) { return frag(at_a[i], buf); };
+    auto frag_b = [&](int buf, int i) { return frag(at_b[i], buf); };
+    f32x4 acc[WT][WT];                                                                    // acc[tn][tm]: rows n, columns m
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-        cs[a] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < WT; ++i)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) acc[a][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
+        for (int j = 0; j < WT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if (nk > 0) {
-        fetch(0);
-        put(0);
-    }
-    __syncthreads();
-    for (int t = 0; t < nk; ++t) {
-        const int cur = t & 1;
-        if (t + 1 < nk) fetch(t + 1);
-        const char* tA = smem + cur * 32768;
-        const char* tB = tA + 16384;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            bf16x8 af[4], bf[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                af[i] = frag(tA, wm * 64 + i * 16, ks);
-                bf[i] = frag(tB, wn * 64 + i * 16, ks);
-            }
-#pragma unroll
-            for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-                for (int tm = 0; tm < 4; ++tm) acc[tn][tm] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[tn], af[tm], acc[tn][tm], 0, 0, 0);
-            if (want_cs) {
-#pragma unroll
-                for (int tm = 0; tm < 4; ++tm) cs[tm] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, af[tm], cs[tm], 0, 0, 0);
-            }
-        }
-        if (t + 1 < nk) put(cur ^ 1);
+        Regs r0, r1;
+        fetch(0, r0);
+        fetch(1, r1);
+        put(0, r0);
+        fetch(2, r0);
+        put(1, r1);
+        fetch(3, r1);
         __syncthreads();
+        bf16x8 fa[4], fb[2][WT];                                                         // the next fragments of dY in a ring, this and the next step's of q
+#pragma unroll
+        for (int i = 0; i < WT; ++i) fb[0][i] = frag_b(0, i);
+        fa[0] = frag_a(0, 0);
+        fa[1] = frag_a(0, 1);
+        // One step: the 32 tokens of tile t, P = t mod 4.  The WT^2 matrix instructions go row by row of dY's fragments.  A wave issues in order and a SIMD has
+        // one wave (WT = 8), so that everything else is placed between them, an instruction or two behind a product (a product takes 16 cycles): the fragment
+        // of dY that is needed two rows later, one of the next tile's of q, and the pieces of tile t + 2 that go into LDS with the requests for tile
+        // t + 4 that take their registers.  The barrier behind the step shows tile t + 2 to step t + 1, which reads its first fragments; the tile that
+        // it replaces, t - 2, was last read before the barrier of step t - 2.
+        // The number of steps is rounded up to 4: tiles behind the last are zeros in dY (and what is read ahead of the last step is not used).
+        auto step = [&](int t, auto P_) {
+            constexpr int P = decltype(P_)::value, cur = P & 1;
+            Regs& r = cur ? r1 : r0;
+#pragma unroll
+            for (int tm = 0; tm < WT; ++tm) {
+#pragma unroll
+                for (int tn = 0; tn < WT; ++tn) {
+                    tn8_mfma<WT == 8>(acc[tn][tm], fb[cur][tn], fa[tm & 3]);
+                    if (tn == 0) fa[(tm + 2) & 3] = tm + 2 < WT ? frag_a(P, tm + 2) : frag_a(P + 1, tm + 2 - WT);
+                    if (tn == WT / 4) fb[cur ^ 1][tm] = frag_b(P + 1, tm);
+                    if (tn == WT / 2) {
+                        if (tm < NA) put_a(t + 2, tm, r);
+                        else put_q(t + 2, (tm - NA) / 2, (tm - NA) & 1, r);
+                    }
+                    if (tn == WT / 2 + WT / 4) {
+                        if (tm >= 1 && tm <= NA) fetch_a(t + 4, tm - 1, r);
+                        else if (tm > NA && ((tm - NA) & 1)) fetch_q(t + 4, (tm - NA) / 2, r);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            __syncthreads();
+        };
+        for (int t = 0; t < nk; t += 4) {
+            step(t, std::integral_constant<int, 0>());
+            step(t + 1, std::integral_constant<int, 1>());
+            step(t + 2, std::integral_constant<int, 2>());
+            step(t + 3, std::integral_constant<int, 3>());
+        }
+    }
+    if constexpr (WT == 8) {
+        // the compiler does not see that these are results of matrix instructions: 16 wait states where 11 are needed before anything else reads one
+#pragma unroll
+        for (int i = 0; i < WT; ++i)
+#pragma unroll
+            for (int j = 0; j < WT; ++j) asm volatile("s_nop 15" : "+a"(acc[i][j]));
+    }
+    if (p.colsum != nullptr) {                                                            // the RA threads of a column, in row order
+        float* buf = (float*)smem;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) buf[(ra0 * CA + ca) * 8 + j] = db[j];
+        __syncthreads();
+        const int m = m0 + tid;
+        if (tid < BLOCK && m < p.M) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < RA; ++i) sum += buf[i * BLOCK + tid];
+            p.colsum[((int64_t)split * p.tiles_n + tile_n) * p.M + m] = sum;
+        }
     }
     const int mr = lane & 15;
-    float* Cp = p.C + (int64_t)blockIdx.y * p.M * p.N;
-    if (want_cs && g == 0) {
+    float* Cp = p.C + (int64_t)split * p.M * p.N;
 #pragma unroll
-        for (int tm = 0; tm < 4; ++tm) {
-            const int m = m0 + wm * 64 + tm * 16 + mr;
-            if (m < p.M) p.colsum[(int64_t)blockIdx.y * p.M + m] = cs[tm][0];
-        }
-    }
-#pragma unroll
-    for (int tm = 0; tm < 4; ++tm) {
-        const int m = m0 + wm * 64 + tm * 16 + mr;
+    for (int tm = 0; tm < WT; ++tm) {
+        const int m = m0 + wm * 16 * WT + tm * 16 + mr;
         if (m >= p.M) continue;
 #pragma unroll
-        for (int tn = 0; tn < 4; ++tn) {
-            const int n = n0 + wn * 64 + tn * 16 + 4 * g;
+        for (int tn = 0; tn < WT; ++tn) {
+            const int n = n0 + wn * 16 * WT + tn * 16 + 4 * g;
             if (n + 4 <= p.N && p.N % 4 == 0) *(f32x4*)(Cp + (int64_t)m * p.N + n) = acc[tn][tm];
             else {
 #pragma unroll
@@ -172,58 +253,105 @@ __global__ __launch_bounds__(256, 2) void gemm_tn8_kernel(Tn8Params p) {
     }
 }
 
-// dW and db from the slices' planes, added in slice order
-__global__ __launch_bounds__(256) void tn8_join_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, const float* __restrict__ cs_part, float* __restrict__ cs, int m,
-                                                       int splits) {
-    const int64_t total = n + (cs ? m : 0), stride = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
-        const float* src = i < n ? part + i : cs_part + (i - n);
-        const int64_t step = i < n ? n : m;
-        float a = 0.f;
-        for (int s = 0; s < splits; ++s) a += src[s * step];
-        if (i < n) out[i] = a;
-        else cs[i - n] = a;
+// dW and db from their planes, added in order
+__global__ __launch_bounds__(256) void tn8_join_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, int splits, const float* __restrict__ cs_part, float* __restrict__ cs,
+                                                       int m, int cs_planes, int wide) {
+    const int64_t stride = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (splits > 1) {
+        if (wide) {
+            for (int64_t i = first; i < n / 4; i += stride) {
+                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                for (int s = 0; s < splits; ++s) a += *((const f32x4*)(part + s * n) + i);
+                *((f32x4*)out + i) = a;
+            }
+        } else {
+            for (int64_t i = first; i < n; i += stride) {
+                float a = 0.f;
+#pragma unroll 4
+                for (int s = 0; s < splits; ++s) a += part[s * n + i];
+                out[i] = a;
+            }
+        }
     }
+    if (cs)
+        for (int64_t i = first; i < m; i += stride) {
+            float a = 0.f;
+#pragma unroll 8
+            for (int s = 0; s < cs_planes; ++s) a += cs_part[(int64_t)s * m + i];
+            cs[i] = a;
+        }
 }
 
-static int tn8_splits(int M, int N, int64_t K) {
-    const int64_t tiles = ((int64_t)(M + 127) / 128) * ((N + 127) / 128);
-    int64_t s = 512 / tiles;                                                   // two workgroups to a CU
-    const int64_t most = (K + 511) / 512;                                      // and no slice below 512 tokens
+struct Tn8Plan { int wt, tiles_m, tiles_n, splits; };
+static Tn8Plan tn8_plan(int M, int N, int64_t K) {
+    Tn8Plan q;
+    const int64_t large = ((int64_t)(M + 255) / 256) * ((N + 255) / 256);
+    // 256 x 256 tiles (one workgroup to a CU) where slices of 1024 tokens or more of them fill the chip
+    q.wt = large * ((K + 1023) / 1024) >= 256 && M > 128 && N > 128 ? 8 : 4;
+    const int block = 32 * q.wt;
+    q.tiles_m = (M + block - 1) / block;
+    q.tiles_n = (N + block - 1) / block;
+    const int64_t tiles = (int64_t)q.tiles_m * q.tiles_n;
+    int64_t s = (q.wt == 8 ? 256 : 512) / tiles;
+    const int64_t most = (K + 255) / 256;                                      // no slice below 256 tokens
     if (s > most) s = most;
-    return (int)(s < 1 ? 1 : s);
+    q.splits = (int)(s < 1 ? 1 : s);
+    return q;
 }
 static bool tn8_shape_ok(int M, int N, int64_t K) {
-    return M > 0 && N > 0 && K >= 0 && M <= (1 << 24) && N <= (1 << 24) && ((int64_t)(M + 127) / 128) * ((N + 127) / 128) <= 0x7fffffff;
+    return M > 0 && N > 0 && K >= 0 && K <= (1 << 30) && M <= (1 << 24) && N <= (1 << 24) && ((int64_t)(M + 127) / 128) * ((N + 127) / 128) <= (1 << 24);
 }
 
 extern "C" int64_t hh_workspace_bytes_gemm_tn_act8(int M, int N, int64_t K) {
     if (!tn8_shape_ok(M, N, K)) return -1;
-    const int64_t s = tn8_splits(M, N, K);
-    return s == 1 ? 0 : s * ((int64_t)M * N + M) * 4;
+    const Tn8Plan q = tn8_plan(M, N, K);
+    const int64_t db = (int64_t)q.splits * q.tiles_n * M;
+    return (q.splits == 1 ? db : ((int64_t)q.splits * M * N + 3) / 4 * 4 + db) * 4;
 }
 
 extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int64_t ldq, const float* scale, float* dw, float* db, int M, int N, int64_t K, void* workspace,
                                hh_stream_t stream) {
     HH_REQUIRE(tn8_shape_ok(M, N, K) && ld_dy >= M && ldq >= N, HH_ERR_SHAPE, "hh_gemm_tn_act8: bad shape (M=%d N=%d K=%lld ld_dy=%lld ldq=%lld)", M, N, (long long)K, (long long)ld_dy, (long long)ldq);
+    HH_REQUIRE(ld_dy <= (1 << 24) && ldq <= (1 << 24), HH_ERR_SHAPE, "hh_gemm_tn_act8: leading dimensions up to 2^24");
     HH_REQUIRE(dw != nullptr && (K == 0 || (dy != nullptr && q != nullptr && scale != nullptr)), HH_ERR_ALIGN, "hh_gemm_tn_act8: NULL pointer");
     HH_REQUIRE((((uintptr_t)dw) & 15) == 0, HH_ERR_ALIGN, "hh_gemm_tn_act8: dw must be 16-byte aligned");
-    const int splits = tn8_splits(M, N, K);
-    HH_REQUIRE(splits == 1 || (workspace != nullptr && HH_ALIGNED16(workspace)), HH_ERR_ALIGN, "hh_gemm_tn_act8: a 16-byte aligned workspace is needed");
+    HH_REQUIRE(workspace != nullptr && HH_ALIGNED16(workspace), HH_ERR_ALIGN, "hh_gemm_tn_act8: a 16-byte aligned workspace is needed");
     hipStream_t s = (hipStream_t)stream;
+    const Tn8Plan pl = tn8_plan(M, N, K);
+    const int64_t n = (int64_t)M * N;
     Tn8Params p;
     p.A = (const bf16_t*)dy; p.lda = ld_dy; p.q = (const unsigned char*)q; p.ldq = ldq; p.scale = scale;
-    p.M = M; p.N = N; p.K = K; p.groups = (N + 127) / 128; p.tiles_n = (N + 127) / 128;
-    p.vec_a = M % 8 == 0 && ld_dy % 8 == 0 && HH_ALIGNED16(dy);
-    p.vec_q = N % 16 == 0 && ldq % 16 == 0 && HH_ALIGNED16(q);
-    p.k_per_split = ((K + 63) / 64 + splits - 1) / splits * 64;
-    p.C = splits == 1 ? dw : (float*)workspace;
-    p.colsum = db == nullptr ? nullptr : splits == 1 ? db : (float*)workspace + (int64_t)splits * M * N;
-    const dim3 grid((unsigned)(((M + 127) / 128) * p.tiles_n), (unsigned)splits);
-    hipLaunchKernelGGL(gemm_tn8_kernel, grid, dim3(256), 0, s, p);
-    if (splits > 1) {
-        const int64_t n = (int64_t)M * N, blocks = (n + M + 255) / 256;
-        hipLaunchKernelGGL(tn8_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, p.C, dw, n, p.colsum, db, M, splits);
+    p.M = M; p.N = N; p.K = K; p.groups = (N + 127) / 128; p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.splits = pl.splits;
+    const int tokens = 32;
+    p.k_per_split = ((K + tokens - 1) / tokens + pl.splits - 1) / pl.splits * tokens;
+    p.C = pl.splits == 1 ? dw : (float*)workspace;
+    float* cs = (float*)workspace + (pl.splits == 1 ? 0 : (n * pl.splits + 3) / 4 * 4);
+    p.colsum = db == nullptr ? nullptr : cs;
+    const bool vec = M % 8 == 0 && ld_dy % 8 == 0 && HH_ALIGNED16(dy) && N % 16 == 0 && ldq % 16 == 0 && HH_ALIGNED16(q);
+    const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n * pl.splits));
+    const int lds = 4 * 2 * 32 * 64 * pl.wt;
+    if (pl.wt == 8) {
+        static std::atomic<uint64_t> attr{0};
+        if (hh_attr_needed(attr)) {
+            hipError_t e = hipFuncSetAttribute((const void*)gemm_tn8_kernel<8, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            if (e == hipSuccess) e = hipFuncSetAttribute((const void*)gemm_tn8_kernel<8, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            HH_REQUIRE(e == hipSuccess, HH_ERR_LAUNCH, "hh_gemm_tn_act8: %s", hipGetErrorString(e));
+            hh_attr_done(attr);
+        }
+    }
+    if (pl.wt == 8) {
+        if (vec) hipLaunchKernelGGL((gemm_tn8_kernel<8, true>), grid, dim3(256), lds, s, p);
+        else hipLaunchKernelGGL((gemm_tn8_kernel<8, false>), grid, dim3(256), lds, s, p);
+    } else {
+        if (vec) hipLaunchKernelGGL((gemm_tn8_kernel<4, true>), grid, dim3(256), lds, s, p);
+        else hipLaunchKernelGGL((gemm_tn8_kernel<4, false>), grid, dim3(256), lds, s, p);
+    }
+    if (pl.splits > 1 || db) {
+        const int wide = n % 4 == 0;
+        int64_t blocks = ((pl.splits > 1 ? (wide ? n / 4 : n) : 0) + 255) / 256;
+        if (blocks < (M + 255) / 256) blocks = (M + 255) / 256;
+        hipLaunchKernelGGL(tn8_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, p.C, dw, n, pl.splits, p.colsum, db, M, pl.splits * pl.tiles_n, wide);
     }
     return hh_check_launch("hh_gemm_tn_act8");
 }
