@@ -253,34 +253,39 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
     }
 }
 
-// dW and db from their planes, added in order
+// dW and db from their planes, added in order: blockIdx.x < blocks: dW, a piece of 4 (wide) or 1 to a thread;  behind them 64 channels of db to a workgroup, whose
+// waves take a quarter of the planes each
 __global__ __launch_bounds__(256) void tn8_join_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, int splits, const float* __restrict__ cs_part, float* __restrict__ cs,
-                                                       int m, int cs_planes, int wide) {
-    const int64_t stride = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (splits > 1) {
+                                                       int m, int cs_planes, int wide, int blocks) {
+    if ((int)blockIdx.x < blocks) {
+        const int64_t stride = (int64_t)blocks * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
         if (wide) {
             for (int64_t i = first; i < n / 4; i += stride) {
                 f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
                 for (int s = 0; s < splits; ++s) a += *((const f32x4*)(part + s * n) + i);
                 *((f32x4*)out + i) = a;
             }
         } else {
             for (int64_t i = first; i < n; i += stride) {
                 float a = 0.f;
-#pragma unroll 4
+#pragma unroll 8
                 for (int s = 0; s < splits; ++s) a += part[s * n + i];
                 out[i] = a;
             }
         }
+        return;
     }
-    if (cs)
-        for (int64_t i = first; i < m; i += stride) {
-            float a = 0.f;
+    __shared__ float buf[4][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = ((int)blockIdx.x - blocks) * 64 + lane;
+    const int share = (cs_planes + 3) / 4, p0 = wave * share, p1 = p0 + share < cs_planes ? p0 + share : cs_planes;
+    float a = 0.f;
+    if (c < m)
 #pragma unroll 8
-            for (int s = 0; s < cs_planes; ++s) a += cs_part[(int64_t)s * m + i];
-            cs[i] = a;
-        }
+        for (int s = p0; s < p1; ++s) a += cs_part[(int64_t)s * m + c];
+    buf[wave][lane] = a;
+    __syncthreads();
+    if (wave == 0 && c < m) cs[c] = (buf[0][lane] + buf[1][lane]) + (buf[2][lane] + buf[3][lane]);
 }
 
 struct Tn8Plan { int wt, tiles_m, tiles_n, splits; };
@@ -294,7 +299,8 @@ static Tn8Plan tn8_plan(int M, int N, int64_t K) {
     q.tiles_n = (N + block - 1) / block;
     const int64_t tiles = (int64_t)q.tiles_m * q.tiles_n;
     int64_t s = (q.wt == 8 ? 256 : 512) / tiles;
-    const int64_t most = (K + 255) / 256;                                      // no slice below 256 tokens
+    // no slice below 512 tokens: every slice leaves a plane of dW to write and to add (2464 x 768 x 768: 10 slices 25.4 us, 5 slices 21.3)
+    const int64_t most = (K + 511) / 512;
     if (s > most) s = most;
     q.splits = (int)(s < 1 ? 1 : s);
     return q;
@@ -350,8 +356,8 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
     if (pl.splits > 1 || db) {
         const int wide = n % 4 == 0;
         int64_t blocks = ((pl.splits > 1 ? (wide ? n / 4 : n) : 0) + 255) / 256;
-        if (blocks < (M + 255) / 256) blocks = (M + 255) / 256;
-        hipLaunchKernelGGL(tn8_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, p.C, dw, n, pl.splits, p.colsum, db, M, pl.splits * pl.tiles_n, wide);
+        if (blocks > 4096) blocks = 4096;
+        hipLaunchKernelGGL(tn8_join_kernel, dim3((unsigned)(blocks + (db ? (M + 63) / 64 : 0))), dim3(256), 0, s, p.C, dw, n, pl.splits, p.colsum, db, M, pl.splits * pl.tiles_n, wide, (int)blocks);
     }
     return hh_check_launch("hh_gemm_tn_act8");
 }

@@ -1011,13 +1011,24 @@ def tv_accuracy(sim, text_cos, sim_v, sim_n):
 
 
 # ---- training a token stream: embedding, the end of a residual block, activation checkpoints in 8 bits --------------------------------
-def _chk_here(*tensors):
-    """_chk, and every tensor on the current device: the launch goes to that device's current stream."""
-    _chk(*tensors)
-    dev = torch.cuda.current_device()
+def _here(*tensors):
+    """_chk, and every tensor on the current device -> that device's current stream, as an integer.  (torch.cuda.current_stream() builds an object, 2.6 us of a call
+    whose kernel takes 3.)"""
+    dev = -1
     for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise RuntimeError("libhh ops run on the current device (cuda:%d), got a tensor on %s: enter torch.cuda.device(tensor.device)" % (dev, t.device))
+        if t is None:
+            continue
+        d = t.get_device()
+        if d < 0:
+            raise RuntimeError("libhh ops need GPU tensors (got device %s); there is no CPU fallback" % t.device)
+        if d != dev:
+            cur = torch.cuda.current_device()
+            if d != cur:
+                raise RuntimeError("libhh ops run on the current device (cuda:%d), got a tensor on %s: enter torch.cuda.device(tensor.device)" % (cur, t.device))
+            dev = d
+        if not t.is_contiguous():
+            raise RuntimeError("libhh ops need contiguous tensors")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _bytes(nbytes, what, device):
@@ -1042,19 +1053,19 @@ def embed_tokens(ids, weight, scale=1.0, pos=None, out_dtype=None):
     ids int64 / int32 [..., L]; weight fp32 / bf16 [V, D]; pos fp32 [P >= L, D] or None: row t is added at index t of the last dimension (a decoding step
     at position t passes pos[t:t + 1]).  -> out_dtype (weight's by default) [..., L, D].  An id outside [0, V) gives a row of NaN (nothing
     can be raised without waiting for the device)."""
-    _chk_here(ids, weight, pos)
+    stream = _here(ids, weight, pos)
     length, seqs = _ids_of(ids, "embed_tokens")
     if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError("embed_tokens: weight must be [V, D], got %s" % (tuple(weight.shape),))
     V, D = weight.shape
     if pos is not None and (pos.dtype != torch.float32 or pos.dim() != 2 or pos.shape[1] != D or pos.shape[0] < length):
         raise ValueError("embed_tokens: pos must be fp32 [>= %d, %d], got %s %s" % (length, D, pos.dtype, tuple(pos.shape)))
-    out = torch.empty((*ids.shape, D), dtype=weight.dtype if out_dtype is None else out_dtype, device=weight.device)
+    out = weight.new_empty((*ids.shape, D), dtype=out_dtype)
     wd, od = _dt(weight), _dt(out)
-    if out.numel() == 0:
+    if seqs == 0 or length == 0:
         return out
-    _lib.check(_lib.lib().hh_embed_tokens_fwd(_p(ids), ids.element_size(), _p(weight), wd, _p(pos), _p(out), od, seqs, length, V, D, float(scale), _stream()),
-               "hh_embed_tokens_fwd")
+    _lib.check(_lib.lib().hh_embed_tokens_fwd(ids.data_ptr(), ids.element_size(), weight.data_ptr(), wd, None if pos is None else pos.data_ptr(), out.data_ptr(), od, seqs,
+                                              length, V, D, scale, stream), "hh_embed_tokens_fwd")
     return out
 
 
@@ -1065,7 +1076,7 @@ def embed_tokens_bwd(ids, dy, num_rows, scale=1.0, skip_id=None, pos_grad=False,
     ids int64 / int32 [..., L], dy fp32 / bf16 [..., L, D].  skip_id: an id without a gradient (nn.Embedding's padding_idx); ids outside [0, num_rows) have
     none either.  out: a fp32 [num_rows, D] buffer that the gradient is ACCUMULATED into (a parameter's slice of the gradient arena), a fresh one by
     default.  Equal inputs give equal bits (the ids are sorted, no floating-point atomics)."""
-    _chk_here(ids, dy, out)
+    stream = _here(ids, dy, out)
     length, seqs = _ids_of(ids, "embed_tokens_bwd")
     if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] == 0:
         raise ValueError("embed_tokens_bwd: dy must be ids' shape and a last dimension D, got %s for ids %s" % (tuple(dy.shape), tuple(ids.shape)))
@@ -1078,7 +1089,7 @@ def embed_tokens_bwd(ids, dy, num_rows, scale=1.0, skip_id=None, pos_grad=False,
     dw = torch.empty((V, D), dtype=torch.float32, device=dy.device) if out is None else out
     dpos = torch.empty((length, D), dtype=torch.float32, device=dy.device) if pos_grad else None
     _lib.check(L.hh_embed_tokens_bwd(_p(ids), ids.element_size(), _p(dy), dd, _p(dw), int(out is not None), _p(dpos) if length else None, seqs, max(length, 1), V, D,
-                                     float(scale), -1 if skip_id is None else int(skip_id), _p(ws), _stream()), "hh_embed_tokens_bwd")
+                                     scale, -1 if skip_id is None else int(skip_id), _p(ws), stream), "hh_embed_tokens_bwd")
     return (dw, dpos) if pos_grad else dw
 
 
@@ -1087,43 +1098,40 @@ ResidualNormGrads = namedtuple("ResidualNormGrads", "dx dy dgate dpost_gamma dpo
 
 
 def _residual_norm_desc(what, x, y, gate, gate_tanh, res_scale, post, pre, rms):
-    cols = x.shape[-1] if x.dim() else 0
-    if cols == 0 or y.shape != x.shape:
-        raise ValueError("%s: stream and branch must have one shape [..., cols], got %s and %s" % (what, tuple(x.shape), tuple(y.shape)))
-    d = ResidualNorm()
-    d.rows, d.groups, d.cols = x.numel() // cols, 1, cols
-    d.x_dtype, d.y_dtype, d.h_dtype = _dt(x), _dt(y), F32
-    d.rms, d.res_scale, d.gate_tanh = int(bool(rms)), float(res_scale), int(bool(gate_tanh))
-    d.y = y.data_ptr()
+    shape = x.shape
+    cols = shape[-1] if shape else 0
+    if cols == 0 or y.shape != shape:
+        raise ValueError("%s: stream and branch must have one shape [..., cols], got %s and %s" % (what, tuple(shape), tuple(y.shape)))
+    rows, groups, kind, gate_at = x.numel() // cols, 1, GATE_NONE, None
     if gate is not None:
         if gate.dtype != torch.float32:
             raise TypeError("%s: the gate must be fp32" % what)
         if gate.dim() == 2 and gate.shape[1] == cols:
-            d.gate_kind, d.groups = (GATE_GROUP, gate.shape[0]) if gate.shape[0] != 1 else (GATE_CHANNEL, 1)
-            if d.groups == 0 or d.rows % d.groups:
-                raise ValueError("%s: %d rows do not split into %d gate groups" % (what, d.rows, d.groups))
+            kind, groups = (GATE_GROUP, gate.shape[0]) if gate.shape[0] != 1 else (GATE_CHANNEL, 1)
+            if groups == 0 or rows % groups:
+                raise ValueError("%s: %d rows do not split into %d gate groups" % (what, rows, groups))
         elif gate.numel() == 1:
-            d.gate_kind = GATE_SCALAR
+            kind = GATE_SCALAR
         elif gate.dim() == 1 and gate.numel() == cols:
-            d.gate_kind = GATE_CHANNEL
+            kind = GATE_CHANNEL
         else:
             raise ValueError("%s: the gate must hold one value, [cols] or [groups, cols], got %s" % (what, tuple(gate.shape)))
-        d.gate = gate.data_ptr()
-    for name, norm in (("post", post), ("pre", pre)):
+        gate_at = gate.data_ptr()
+    at, eps = [None] * 4, [0.0, 0.0]
+    for i, norm in enumerate((post, pre)):
         if norm is None:
             continue
-        gamma, beta, eps = norm
-        for v in (gamma, beta):
-            if v is not None and (v.dtype != torch.float32 or v.numel() != cols):
-                raise ValueError("%s: %s norm's gamma / beta must be fp32 [%d]" % (what, name, cols))
-        setattr(d, name + "_gamma", gamma.data_ptr())
-        setattr(d, name + "_beta", beta.data_ptr() if beta is not None else None)
-        setattr(d, name + "_eps", float(eps))
-    return d
+        gamma, beta, eps[i] = norm
+        for k, v in ((2 * i, gamma), (2 * i + 1, beta)):
+            if v is not None:
+                if v.dtype != torch.float32 or v.numel() != cols:
+                    raise ValueError("%s: %s norm's gamma / beta must be fp32 [%d]" % (what, ("post", "pre")[i], cols))
+                at[k] = v.data_ptr()
+    return ResidualNorm(rows, groups, cols, _dt(x), _dt(y), F32, kind, 1 if gate_tanh else 0, 1 if rms else 0, res_scale, eps[0], eps[1], gate_at, *at, None, y.data_ptr())
 
 
 def _norm_tensors(post, pre):
-    return [t for n in (post, pre) if n is not None for t in n[:2]]
+    return (() if post is None else post[:2]) + (() if pre is None else pre[:2])
 
 
 def residual_norm(x, y, *, gate=None, gate_tanh=False, res_scale=1.0, post=None, pre=None, rms=False, out_dtype=torch.bfloat16, out=None):
@@ -1133,24 +1141,24 @@ def residual_norm(x, y, *, gate=None, gate_tanh=False, res_scale=1.0, post=None,
     x, y fp32 / bf16 [..., cols], x_new like x, h of out_dtype.  post / pre: (gamma, beta or None, eps) of a norm (fp32 [cols]) or None; rms: root-mean-square norms
     instead of LayerNorms.  gate fp32, through tanh with gate_tanh: one value, [cols], or [groups, cols] for `groups` groups of consecutive rows (a
     clip's, a caption's).  out: x_new's buffer, may be x itself (the stream updated in place)."""
-    _chk_here(x, y, gate, out, *_norm_tensors(post, pre))
+    stream = _here(x, y, gate, out, *_norm_tensors(post, pre))
     d = _residual_norm_desc("residual_norm", x, y, gate, gate_tanh, res_scale, post, pre, rms)
     if out is not None and (out.dtype != x.dtype or out.shape != x.shape):
         raise ValueError("residual_norm: out must have x's shape and type")
     x_new = torch.empty_like(x) if out is None else out
     h = None
     if pre is not None:
-        h = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        h = x.new_empty(x.shape, dtype=out_dtype)
         d.h_dtype, d.h = _dt(h), h.data_ptr()
     d.x, d.x_new = x.data_ptr(), x_new.data_ptr()
-    _lib.check(_lib.lib().hh_residual_norm_fwd(ctypes.byref(d), _stream()), "hh_residual_norm_fwd")
+    _lib.check(_lib.lib().hh_residual_norm_fwd(ctypes.byref(d), stream), "hh_residual_norm_fwd")
     return x_new, h
 
 
 def residual_norm_bwd(x_new, y, dx_new=None, dh=None, *, gate=None, gate_tanh=False, res_scale=1.0, post=None, pre=None, rms=False):
     """Gradients of residual_norm from its x_new and y and the gradients of x_new (None: zeros) and of h (with `pre`) -> ResidualNormGrads: dx like x_new, dy like
     y, and fp32 dgate (the gate's shape), dpost_gamma, dpost_beta, dpre_gamma, dpre_beta, None where the parameter is (include/hh.h: hh_residual_norm_bwd)."""
-    _chk_here(x_new, y, dx_new, dh, gate, *_norm_tensors(post, pre))
+    stream = _here(x_new, y, dx_new, dh, gate, *_norm_tensors(post, pre))
     d = _residual_norm_desc("residual_norm_bwd", x_new, y, gate, gate_tanh, res_scale, post, pre, rms)
     if (dh is None) != (pre is None):
         raise ValueError("residual_norm_bwd: dh comes with pre")
@@ -1168,7 +1176,7 @@ def residual_norm_bwd(x_new, y, dx_new=None, dh=None, *, gate=None, gate_tanh=Fa
     L = _lib.lib()
     ws = _bytes(L.hh_workspace_bytes_residual_norm_bwd(d.rows, d.cols, d.groups), "residual_norm_bwd", dev)
     d.workspace = ws.data_ptr() if ws is not None else None
-    _lib.check(L.hh_residual_norm_bwd(ctypes.byref(d), _stream()), "hh_residual_norm_bwd")
+    _lib.check(L.hh_residual_norm_bwd(ctypes.byref(d), stream), "hh_residual_norm_bwd")
     return ResidualNormGrads(dx, dy, *grads)
 
 
@@ -1176,9 +1184,10 @@ ACT8_GROUP = 128                                                       # channel
 
 
 def _chk_act8(q, scale, what):
-    if q.dtype != torch.float8_e4m3fn or q.dim() != 2 or q.shape[1] == 0:
+    shape = q.shape
+    if q.dtype != torch.float8_e4m3fn or len(shape) != 2 or shape[1] == 0:
         raise TypeError("%s: q must be float8_e4m3fn [rows, cols] (act8's), got %s %s" % (what, q.dtype, tuple(q.shape)))
-    if scale.dtype != torch.float32 or tuple(scale.shape) != (q.shape[0], -(-q.shape[1] // ACT8_GROUP)):
+    if scale.dtype != torch.float32 or scale.shape != (shape[0], -(-shape[1] // ACT8_GROUP)):
         raise TypeError("%s: scale must be fp32 [rows, ceil(cols / 128)] (act8's), got %s %s" % (what, scale.dtype, tuple(scale.shape)))
 
 
@@ -1186,29 +1195,29 @@ def act8(u, act=ACT_NONE, want_out=True):
     """An activation and its 8-bit checkpoint in one pass (include/hh.h: hh_act8_fwd): -> (a = act(u) like u or None, q float8_e4m3fn, scale fp32).
     u fp32 / bf16 [rows, cols]; u ~ q * scale with one power of two for every 128 channels (q.float() * scale.repeat_interleave(128, 1)[:, :cols] has the
     values): 1.03 bytes for an element that a backward pass would keep in 2 or 4.  want_out=False: the checkpoint alone (the input of a linear layer)."""
-    _chk_here(u)
+    stream = _here(u)
     if u.dim() != 2 or u.shape[1] == 0:
         raise ValueError("act8: u must be [rows, cols], got %s" % (tuple(u.shape),))
     dt = _dt(u)
     rows, cols = u.shape
     a = torch.empty_like(u) if want_out else None
-    q = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=u.device)
-    scale = torch.empty((rows, -(-cols // ACT8_GROUP)), dtype=torch.float32, device=u.device)
-    _lib.check(_lib.lib().hh_act8_fwd(_p(u), dt, _p(a), _p(q), _p(scale), rows, cols, int(act), _stream()), "hh_act8_fwd")
+    q = u.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
+    scale = u.new_empty((rows, -(-cols // ACT8_GROUP)), dtype=torch.float32)
+    _lib.check(_lib.lib().hh_act8_fwd(u.data_ptr(), dt, None if a is None else a.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, cols, act, stream), "hh_act8_fwd")
     return a, q, scale
 
 
 def act8_bwd(q, scale, da, act, want_out=False):
     """du = da * act'(v) with v = q * scale, the values of act8's checkpoint (include/hh.h: hh_act8_bwd) -> du like da; with want_out (du, act(v)): the
     activation again, the operand of the next layer's weight gradient."""
-    _chk_here(q, scale, da)
+    stream = _here(q, scale, da)
     _chk_act8(q, scale, "act8_bwd")
     if da.shape != q.shape:
         raise ValueError("act8_bwd: da must have q's shape")
     dt = _dt(da)
     du = torch.empty_like(da)
     a = torch.empty_like(da) if want_out else None
-    _lib.check(_lib.lib().hh_act8_bwd(_p(q), _p(scale), _p(da), _p(du), _p(a), dt, q.shape[0], q.shape[1], int(act), _stream()), "hh_act8_bwd")
+    _lib.check(_lib.lib().hh_act8_bwd(q.data_ptr(), scale.data_ptr(), da.data_ptr(), du.data_ptr(), None if a is None else a.data_ptr(), dt, *q.shape, act, stream), "hh_act8_bwd")
     return (du, a) if want_out else du
 
 
@@ -1219,7 +1228,10 @@ def gemm_tn_act8(dy, q, scale, colsum=False, out=None):
     for t in (dy, q):
         if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
             raise ValueError("gemm_tn_act8: dy and q must be 2-D with unit inner stride and rows that do not overlap")
-    _chk_here(scale, out, dy[:0], q[:0])
+    for t in (dy, q):                                # (row-strided views: not contiguous, and looked at above)
+        if t.get_device() != scale.get_device():
+            raise RuntimeError("libhh ops need GPU tensors on one device (got %s and %s); there is no CPU fallback" % (t.device, scale.device))
+    stream = _here(scale, out)
     _chk_act8(q, scale, "gemm_tn_act8")
     K, M = dy.shape
     N = q.shape[1]
@@ -1232,5 +1244,5 @@ def gemm_tn_act8(dy, q, scale, colsum=False, out=None):
     db = torch.empty((M,), dtype=torch.float32, device=dy.device) if colsum else None
     L = _lib.lib()
     ws = _bytes(L.hh_workspace_bytes_gemm_tn_act8(M, N, K), "gemm_tn_act8", dy.device)
-    _lib.check(L.hh_gemm_tn_act8(_p(dy), dy.stride(0) if K > 1 else M, _p(q), q.stride(0) if K > 1 else N, _p(scale), _p(out), _p(db), M, N, K, _p(ws), _stream()), "hh_gemm_tn_act8")
+    _lib.check(L.hh_gemm_tn_act8(_p(dy), dy.stride(0) if K > 1 else M, _p(q), q.stride(0) if K > 1 else N, _p(scale), _p(out), _p(db), M, N, K, _p(ws), stream), "hh_gemm_tn_act8")
     return (out, db) if colsum else out

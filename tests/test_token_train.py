@@ -62,9 +62,9 @@ def test_act8_refusals():
     b = lambda q=16, s=16, da=16, du=16, dt=0, r=2, c=8, act=0: L.hh_act8_bwd(q, s, da, du, None, dt, r, c, act, None)  # noqa: E731
     assert b(r=0) == 0 and b(c=-3) == -1 and b(dt=9) == -2 and b(act=-1) == -3 and b(q=None) == -5 and b(s=None) == -5 and b(da=None) == -5 and b(du=None) == -5
     g = lambda dy=16, ld=8, q=16, ldq=16, s=16, dw=16, M=8, N=16, K=64, ws=16: L.hh_gemm_tn_act8(dy, ld, q, ldq, s, dw, None, M, N, K, ws, None)  # noqa: E731
-    assert g(M=0) == -1 and g(N=0) == -1 and g(K=-1) == -1 and g(ld=7) == -1 and g(ldq=15) == -1
+    assert g(M=0) == -1 and g(N=0) == -1 and g(K=-1) == -1 and g(ld=7) == -1 and g(ldq=15) == -1 and g(ld=(1 << 24) + 8) == -1 and g(K=(1 << 30) + 1) == -1
     assert g(dy=None) == -5 and g(q=None) == -5 and g(s=None) == -5 and g(dw=None) == -5 and g(dw=8) == -5 and g(K=4096, ws=None) == -5
-    assert L.hh_workspace_bytes_gemm_tn_act8(0, 16, 64) == -1 and L.hh_workspace_bytes_gemm_tn_act8(8, 16, 64) == 0
+    assert L.hh_workspace_bytes_gemm_tn_act8(0, 16, 64) == -1 and L.hh_workspace_bytes_gemm_tn_act8(8, 16, 64) == 4 * 8      # (a row of db)
     assert L.hh_workspace_bytes_gemm_tn_act8(128, 128, 1 << 16) >= 2 * 128 * 128 * 4
 
 
