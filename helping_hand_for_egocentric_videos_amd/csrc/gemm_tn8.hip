@@ -61,46 +61,56 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
     const int64_t k1 = k0 + p.k_per_split < p.K ? k0 + p.k_per_split : p.K;
     const int nk = k1 > k0 ? (int)((k1 - k0 + BK - 1) / BK) : 0;                        // (0 for a slice behind the last token: zeros are written)
 
-    // Columns behind the last are read from the first (their products are not stored); rows behind the slice's last are zero in dY, and q's last row again.
+    // Buffer loads: a resource ends with the slice, and what lies behind reads as zero -- the rows that fill up the last tile, and the tiles behind it.  Columns behind
+    // the last belong to the next row or are zero; their products are not stored.  The resource moves with the tile that is requested, so that offsets stay
+    // below 2^31 whatever the slice's length.
     const int ra0 = tid / CA, rq0 = tid / CQ, ca = tid % CA, cq = tid % CQ;
-    const int am = m0 + ca * 8 < p.M ? m0 + ca * 8 : 0, qn = n0 + cq * 16 < p.N ? n0 + cq * 16 : 0;
-    const char* a_base = (const char*)(p.A + k0 * p.lda);                                 // the same in all lanes; a lane adds 32 bits
-    const char* q_base = (const char*)(p.q + k0 * p.ldq);
-    const char* s_base = (const char*)(p.scale + k0 * p.groups);
-    const int len = (int)(k1 - k0);                                                       // (K is at most 2^30)
-    const unsigned lda = (unsigned)p.lda * 2, ldq = (unsigned)p.ldq, lds = (unsigned)p.groups * 4;      // bytes; rows of a tile lie within 2^31 (checked by the caller)
-    struct Regs { u32x4 a[NA], q[NQ]; float s[NQ]; };
-    // piece i of tile t's rows of dY / of q
-    auto fetch_a = [&](int t, int i, Regs& r) {
-        const int kt = t * BK, row = ra0 + RA * i;
-        const bool cut = kt + BK > len;                                                   // (the same in all lanes)
-        const char* base = a_base + (int64_t)(cut ? 0 : kt) * lda;
-        const int64_t tail = kt + row < len ? kt + row : len - 1;
-        const char* src = cut ? base + tail * lda + (unsigned)am * 2 : base + ((unsigned)row * lda + (unsigned)am * 2);
-        if (VEC) r.a[i] = *(const u32x4*)src;
-        else {
-            r.a[i] = (u32x4){0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (am + j < p.M) r.a[i][j >> 1] |= (unsigned)((const unsigned short*)src)[j] << (16 * (j & 1));
+    const unsigned lda = (unsigned)p.lda * 2, ldq = (unsigned)p.ldq, lds = (unsigned)p.groups * 4;      // bytes
+    const unsigned a_off = (unsigned)ra0 * lda + (unsigned)(m0 + ca * 8) * 2, q_off = (unsigned)rq0 * ldq + (unsigned)(n0 + cq * 16);
+    const unsigned s_off = (unsigned)rq0 * lds + (unsigned)((n0 + cq * 16) / 128) * 4;
+    struct Stream {
+        const char* at; int64_t left;
+        __device__ __amdgpu_buffer_rsrc_t next(unsigned bytes) {                          // the resource of this tile; moves on to the next
+            const int64_t n = left < 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, (int)n, 0x27000);
+            at += bytes; left -= bytes;
+            return r;
         }
     };
-    auto fetch_q = [&](int t, int i, Regs& r) {
-        const int kt = t * BK, row = rq0 + RQ * i;
-        const bool cut = kt + BK > len;
-        const char* base = q_base + (int64_t)(cut ? 0 : kt) * ldq;
-        const char* sbase = s_base + (int64_t)(cut ? 0 : kt) * lds;
-        const int64_t tail = kt + row < len ? kt + row : len - 1;
-        const char* src = cut ? base + tail * ldq + (unsigned)qn : base + ((unsigned)row * ldq + (unsigned)qn);
-        const char* ssrc = cut ? sbase + tail * lds + (unsigned)(qn / 128) * 4 : sbase + ((unsigned)row * lds + (unsigned)(qn / 128) * 4);
-        if (VEC) r.q[i] = *(const u32x4*)src;
+    const int64_t len = k1 - k0;
+    Stream a_str = {(const char*)(p.A + k0 * p.lda), len * (int64_t)lda}, q_str = {(const char*)(p.q + k0 * p.ldq), len * (int64_t)ldq},
+           s_str = {(const char*)(p.scale + k0 * p.groups), len * (int64_t)lds};
+    // (the last row of a strided operand ends where its columns do, not where a next row would begin)
+    a_str.left -= (int64_t)(p.lda - p.M) * 2;
+    q_str.left -= p.ldq - p.N;
+    struct Regs { u32x4 a[NA], q[NQ]; float s[NQ]; };
+    __amdgpu_buffer_rsrc_t a_res, q_res, s_res;
+    // piece i of the next tile's rows of dY / of q: pieces in order, tiles in order
+    auto fetch_a = [&](int i, Regs& r) {
+        if (i == 0) a_res = a_str.next(BK * lda);
+        const unsigned off = a_off + (unsigned)(RA * i) * lda;
+        if (VEC) r.a[i] = __builtin_amdgcn_raw_buffer_load_b128(a_res, off, 0, 0);
         else {
-            r.q[i] = (u32x4){0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (qn + j < p.N) r.q[i][j >> 2] |= (unsigned)((const unsigned char*)src)[j] << (8 * (j & 3));
+            for (int j = 0; j < 4; ++j)
+                r.a[i][j] = (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(a_res, off + 4 * j, 0, 0) |
+                            (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(a_res, off + 4 * j + 2, 0, 0) << 16;
         }
-        r.s[i] = *(const float*)ssrc;
+    };
+    auto fetch_q = [&](int i, Regs& r) {
+        if (i == 0) { q_res = q_str.next(BK * ldq); s_res = s_str.next(BK * lds); }
+        const unsigned off = q_off + (unsigned)(RQ * i) * ldq;
+        if (VEC) r.q[i] = __builtin_amdgcn_raw_buffer_load_b128(q_res, off, 0, 0);
+        else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                unsigned w = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w |= (unsigned)(unsigned char)__builtin_amdgcn_raw_buffer_load_b8(q_res, off + 4 * j + k, 0, 0) << (8 * k);
+                r.q[i][j] = w;
+            }
+        }
+        r.s[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(s_res, s_off + (unsigned)(RQ * i) * lds, 0, 0));
     };
     float db[8];
 #pragma unroll
@@ -108,7 +118,6 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
     int db_tile = p.colsum != nullptr ? tile_n : -1;     // db: the column tiles share the tokens, each adds up every tiles_n-th tile's rows on their way into LDS
     auto put_a = [&](int t, int i, Regs& r) {
         const int row = ra0 + RA * i;
-        if ((t + 1) * BK > len && t * BK + row >= len) r.a[i] = (u32x4){0u, 0u, 0u, 0u};
         if (t == db_tile) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) { db[2 * j] += bf16_lo_to_f32(r.a[i][j]); db[2 * j + 1] += bf16_hi_to_f32(r.a[i][j]); }
@@ -126,11 +135,11 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
         }
         *(u32x4*)(smem + (t & (BUFS - 1)) * 2 * HALF + HALF + row * ROW + (((2 * cq + h) ^ tn8_key(row)) << 4)) = w;
     };
-    auto fetch = [&](int t, Regs& r) {
+    auto fetch = [&](Regs& r) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) fetch_a(t, i, r);
+        for (int i = 0; i < NA; ++i) fetch_a(i, r);
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) fetch_q(t, i, r);
+        for (int i = 0; i < NQ; ++i) fetch_q(i, r);
     };
     auto put = [&](int t, Regs& r) {
 #pragma unroll
@@ -165,21 +174,25 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
         for (int j = 0; j < WT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if (nk > 0) {
         Regs r0, r1;
-        fetch(0, r0);
-        fetch(1, r1);
+        fetch(r0);
+        fetch(r1);
         put(0, r0);
-        fetch(2, r0);
+        fetch(r0);
         put(1, r1);
-        fetch(3, r1);
+        fetch(r1);
         __syncthreads();
-        bf16x8 fa[4], fb[2][WT];                                                         // the next fragments of dY in a ring, this and the next step's of q
+        // fragments: this and the next step's of q, and of dY (WT = 4: a row's four products are shorter than a read's latency) or the next few of it in a ring (WT = 8:
+        // there are no registers for two sets, and eight products are longer)
+        constexpr bool RING = WT == 8;
+        bf16x8 fa[RING ? 4 : 2 * WT], fb[2][WT];
 #pragma unroll
-        for (int i = 0; i < WT; ++i) fb[0][i] = frag_b(0, i);
-        fa[0] = frag_a(0, 0);
-        fa[1] = frag_a(0, 1);
+        for (int i = 0; i < WT; ++i) {
+            fb[0][i] = frag_b(0, i);
+            if (!RING || i < 2) fa[i] = frag_a(0, i);
+        }
         // One step: the 32 tokens of tile t, P = t mod 4.  The WT^2 matrix instructions go row by row of dY's fragments.  A wave issues in order and a SIMD has
         // one wave (WT = 8), so that everything else is placed between them, an instruction or two behind a product (a product takes 16 cycles): the fragment
-        // of dY that is needed two rows later, one of the next tile's of q, and the pieces of tile t + 2 that go into LDS with the requests for tile
+        // of dY that is needed two rows (or a step) later, one of the next tile's of q, and the pieces of tile t + 2 that go into LDS with the requests for tile
         // t + 4 that take their registers.  The barrier behind the step shows tile t + 2 to step t + 1, which reads its first fragments; the tile that
         // it replaces, t - 2, was last read before the barrier of step t - 2.
         // The number of steps is rounded up to 4: tiles behind the last are zeros in dY (and what is read ahead of the last step is not used).
@@ -190,16 +203,19 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
             for (int tm = 0; tm < WT; ++tm) {
 #pragma unroll
                 for (int tn = 0; tn < WT; ++tn) {
-                    tn8_mfma<WT == 8>(acc[tn][tm], fb[cur][tn], fa[tm & 3]);
-                    if (tn == 0) fa[(tm + 2) & 3] = tm + 2 < WT ? frag_a(P, tm + 2) : frag_a(P + 1, tm + 2 - WT);
+                    tn8_mfma<WT == 8>(acc[tn][tm], fb[cur][tn], fa[RING ? tm & 3 : cur * WT + tm]);
+                    if (tn == 0) {
+                        if (RING) fa[(tm + 2) & 3] = tm + 2 < WT ? frag_a(P, tm + 2) : frag_a(P + 1, tm + 2 - WT);
+                        else fa[(cur ^ 1) * WT + tm] = frag_a(P + 1, tm);
+                    }
                     if (tn == WT / 4) fb[cur ^ 1][tm] = frag_b(P + 1, tm);
                     if (tn == WT / 2) {
                         if (tm < NA) put_a(t + 2, tm, r);
                         else put_q(t + 2, (tm - NA) / 2, (tm - NA) & 1, r);
                     }
                     if (tn == WT / 2 + WT / 4) {
-                        if (tm >= 1 && tm <= NA) fetch_a(t + 4, tm - 1, r);
-                        else if (tm > NA && ((tm - NA) & 1)) fetch_q(t + 4, (tm - NA) / 2, r);
+                        if (tm >= 1 && tm <= NA) fetch_a(tm - 1, r);
+                        else if (tm > NA && ((tm - NA) & 1)) fetch_q((tm - NA) / 2, r);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
