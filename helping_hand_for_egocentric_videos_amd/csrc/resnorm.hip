@@ -285,8 +285,9 @@ __global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
     }
 }
 
+// (four rows at a time take 192 registers: for up to 1024 channels, whose workgroups have no more than four waves)
 template <int R, bool POST, bool PRE, bool VEC, bool NT, int XT, int YT, int HT>
-__global__ __launch_bounds__(1024) void resnorm_bwd_kernel(RnParams p) {
+__global__ __launch_bounds__(R == 4 ? 256 : 1024) void resnorm_bwd_kernel(RnParams p) {
     __shared__ RnRed red;
     const int waves = blockDim.x >> 6, c = threadIdx.x * 4;
     const bool on = !VEC || c < p.cols;
@@ -532,9 +533,6 @@ __global__ __launch_bounds__(1024) void resnorm_reduce_kernel(RnReduce p) {
 }
 
 // ---- entry points ------------------------------------------------------------------------------------------------------------------------
-#ifndef RN_BWD_ROWS
-#define RN_BWD_ROWS 2
-#endif
 #ifndef RN_FWD_MANY
 #define RN_FWD_MANY 4096
 #endif
@@ -542,6 +540,7 @@ static int rn_waves(int cols) { return (cols + 255) / 256; }
 
 struct RnPlan { int64_t chunks, units, per_block, blocks; };
 // about 4096 waves (four to a SIMD) in workgroups that take whole units of one gate group's rows; a unit leaves four partial rows, so it has 16 rows if there are
+// (12 320 x 768: 8 rows 38.3 us, 16 rows 34.5, 32 rows 38.8)
 static RnPlan rn_plan(int64_t rows, int cols, int64_t groups) {
     RnPlan q;
     const int64_t blocks = 4096 / rn_waves(cols);
@@ -634,10 +633,11 @@ extern "C" int hh_residual_norm_bwd(const hh_residual_norm* d, hh_stream_t strea
         p.chunks = q.chunks; p.units = q.units; p.per_block = q.per_block;
         const bool nt = d->rows * p.cols * (rn_size(p.x_dt) + rn_size(p.y_dt)) > HH_STREAM_BYTES;
         const int threads = rn_waves(p.cols) * 64;
-#define RB(PO, PR, V, N, X, Y, H) hipLaunchKernelGGL((resnorm_bwd_kernel<RN_BWD_ROWS, PO, PR, V, N, X, Y, H>), dim3((unsigned)q.blocks), dim3(threads), 0, s, p)
-#define RBN(PO, PR, X, Y, H) do { if (nt) RB(PO, PR, true, true, X, Y, H); else RB(PO, PR, true, false, X, Y, H); } while (0)
+// four rows at a time for large calls (131 104 x 1024: 500 -> 472 us with two -> four), two for the others (12 320 x 768: 34.5, four 39.4)
+#define RB(R, PO, PR, V, N, X, Y, H) hipLaunchKernelGGL((resnorm_bwd_kernel<R, PO, PR, V, N, X, Y, H>), dim3((unsigned)q.blocks), dim3(threads), 0, s, p)
+#define RBN(PO, PR, X, Y, H) do { if (!nt) RB(2, PO, PR, true, false, X, Y, H); else if (threads <= 256) RB(4, PO, PR, true, true, X, Y, H); else RB(2, PO, PR, true, true, X, Y, H); } while (0)
 #define RBY(PO, PR, X, H) do { if (p.y_dt == HH_F32) RBN(PO, PR, X, HH_F32, H); else RBN(PO, PR, X, HH_BF16, H); } while (0)
-#define RBX(PO, PR, H) do { if (!vec) RB(PO, PR, false, false, RN_ANY, RN_ANY, RN_ANY); else if (p.x_dt == HH_F32) RBY(PO, PR, HH_F32, H); else RBY(PO, PR, HH_BF16, H); } while (0)
+#define RBX(PO, PR, H) do { if (!vec) RB(2, PO, PR, false, false, RN_ANY, RN_ANY, RN_ANY); else if (p.x_dt == HH_F32) RBY(PO, PR, HH_F32, H); else RBY(PO, PR, HH_BF16, H); } while (0)
         if (p.g1 && p.g2) { if (p.h_dt == HH_F32) RBX(true, true, HH_F32); else RBX(true, true, HH_BF16); }
         else if (p.g2) { if (p.h_dt == HH_F32) RBX(false, true, HH_F32); else RBX(false, true, HH_BF16); }
         else if (p.g1) RBX(true, false, HH_F32);
