@@ -272,6 +272,33 @@ __device__ __forceinline__ void put_row(const RunParams& p, const RunList& l, u3
     store_e<E, float>(o, v, whole, p.dim - c);
 }
 
+// 16 bytes of dy as they lie in memory (E = 4 of fp32, 8 of bf16): turned into fp32 when they are added, so that eight rows on their way take 32 registers
+template <typename T, bool NT>
+__device__ __forceinline__ u32x4 raw16(const T* p, bool whole, int n) {
+    if (whole) return NT ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
+    u32x4 r = {0u, 0u, 0u, 0u};
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) r[i] = ((const u32*)p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) r[i >> 1] |= (u32)((const unsigned short*)p)[i] << (16 * (i & 1));
+    }
+    return r;
+}
+template <typename T, int E>
+__device__ __forceinline__ void add_raw16(fvec<E>& acc, const u32x4& r) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc.v[i] += __uint_as_float(r[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { acc.v[2 * i] += bf16_lo_to_f32(r[i]); acc.v[2 * i + 1] += bf16_hi_to_f32(r[i]); }
+    }
+}
+
 // blockIdx.x: a chunk of the list blockIdx.z;  eight rows are requested before the first is added (the gather's latency is what there is to hide)
 template <typename T, int E, bool NT>
 __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
@@ -292,19 +319,18 @@ __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
         l.flags[blockIdx.x] = !cross ? RUN_ENDS : head && key == at_end ? RUN_COVERS : RUN_STARTS;
     }
     for (int j = j0; j < j1 && (int64_t)key < l.rows; j += 8) {
-        fvec<E> v[8];
+        u32x4 v[8];
         u32 next[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int at = j + i < j1 ? j + i : j1 - 1;              // (behind the chunk: its last row once more, not added)
-            v[i] = load_e<E, T, NT>((const T*)p.dy + run_from(p, l, at) * p.dim + c, whole, p.dim - c);
+            v[i] = raw16<T, NT>((const T*)p.dy + run_from(p, l, at) * p.dim + c, whole, p.dim - c);
             next[i] = at + 1 < p.n ? run_key(p, l, at + 1) : ~0u;   // (~0: no key is that large)
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (j + i < j1 && (int64_t)key < l.rows) {
-#pragma unroll
-                for (int k = 0; k < E; ++k) acc.v[k] += v[i].v[k];
+                add_raw16<T, E>(acc, v[i]);
                 if (next[i] != key || j + i + 1 == j1) {
                     if (head) store_e<E, float>(part, acc, whole, p.dim - c);
                     else if (next[i] == key) store_e<E, float>(part + p.dim, acc, whole, p.dim - c);
@@ -389,11 +415,16 @@ __global__ __launch_bounds__(1024) void run_join_kernel(RunParams p) {
 
 __global__ __launch_bounds__(SORT_THREADS) void zero_kernel(ZeroPart z) { zero_part(z, blockIdx.x, gridDim.x); }
 
-static int run_chunk(int64_t n) {
-    int64_t c = (n + 4095) / 4096;                   // up to 4096 workgroups, and at least 16 rows for each
-    return (int)(c < 16 ? 16 : c);
+// Rows of a chunk: as many workgroups as fit the chip at once (run_sum_kernel leaves room for 7 waves on each of 1024 SIMDs; a second round of them waits for the
+// first: 64 x 2048 x 1024 bf16 in chunks of 32 rows 165 us, 48 rows 142, 64 rows 154), whole batches of eight rows, and 16 rows at least, because every
+// border between chunks may leave two partial rows (160 x 77 x 768 fp32: 8 rows 68 us, 16 rows 61, 32 rows 65).
+#define RUN_WAVES 6600
+static int run_waves(int dim, int e) { return (dim + 64 * e - 1) / (64 * e); }
+static int run_chunk(int64_t n, int waves) {
+    const int64_t c = (n * waves + RUN_WAVES - 1) / RUN_WAVES;
+    return (int)(c < 16 ? 16 : (c + 7) / 8 * 8);
 }
-static int64_t run_chunks(int64_t n) { return n ? (n + run_chunk(n) - 1) / run_chunk(n) : 0; }
+static int64_t run_chunks(int64_t n, int waves) { return n ? (n + run_chunk(n, waves) - 1) / run_chunk(n, waves) : 0; }
 
 // ---- entry points ------------------------------------------------------------------------------------------------------------------------
 static bool embed_shape_ok(int64_t seqs, int length, int64_t rows, int dim) {
@@ -434,8 +465,8 @@ static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 
 extern "C" int64_t hh_workspace_bytes_embed_tokens_bwd(int64_t seqs, int length, int64_t rows, int dim) {
     if (!embed_shape_ok(seqs, length, rows, dim)) return -1;
-    const int64_t n = seqs * length;
-    return 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4) + 2 * align256(4 * run_chunks(n)) + 2 * align256(run_chunks(n) * 2 * (int64_t)dim * 4);
+    const int64_t n = seqs * length, chunks = run_chunks(n, run_waves(dim, 8));      // (bf16; fp32 rows take more waves, and fewer chunks)
+    return 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4) + 2 * align256(4 * chunks) + 2 * align256(chunks * 2 * (int64_t)dim * 4);
 }
 
 // part i of `parts` of the zeros of out, and the workgroups that write it
@@ -477,7 +508,8 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     u32* from[2] = {(u32*)(ws + 2 * align256(4 * n)), (u32*)(ws + 3 * align256(4 * n))};
     u32* hist = (u32*)(ws + 4 * align256(4 * n));
     u32* flags = (u32*)((char*)hist + align256(SORT_BLOCKS * 256 * 4));
-    const int64_t flag_bytes = align256(4 * run_chunks(n)), part_bytes = align256(run_chunks(n) * 2 * (int64_t)dim * 4);
+    const int e = dy_dtype == HH_F32 ? 4 : 8;
+    const int64_t chunks = run_chunks(n, run_waves(dim, e)), flag_bytes = align256(4 * chunks), part_bytes = align256(chunks * 2 * (int64_t)dim * 4);
     char* part = (char*)flags + 2 * flag_bytes;
     const SortPlan sp = sort_plan(n, rows);
     for (int i = 0; i < sp.passes; ++i) {
@@ -489,8 +521,7 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
                            sp.per_block, sp.pass[i].shift, sp.pass[i].bits, sp.blocks, z);
     }
     RunParams p;
-    p.dy = dy; p.n = (int)n; p.chunk = run_chunk(n); p.chunks = (int)run_chunks(n); p.dim = dim; p.length = length; p.seqs = (int)seqs;
-    const int e = dy_dtype == HH_F32 ? 4 : 8;
+    p.dy = dy; p.n = (int)n; p.chunk = run_chunk(n, run_waves(dim, e)); p.chunks = (int)chunks; p.dim = dim; p.length = length; p.seqs = (int)seqs;
     p.list[0] = RunList{keys[sp.passes & 1], from[sp.passes & 1], dweight, (float*)part, flags, rows, accumulate != 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dweight), scale};
     p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), (u32*)((char*)flags + flag_bytes), length, 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dpos), 1.f};
     const int need = (dim + e - 1) / e;

@@ -466,7 +466,11 @@ class CLIP(nn.Module):
                                       "utils/train_utils.py:42-43, gives it no optimizer group); a trainable text tower has no libhh backward and there is "
                                       "no stock-op fallback -- call under torch.no_grad() or freeze the parameters")
         with torch.no_grad(), ops.prof_role(ops.PROF_ROLE_TEXT):
-            x = self.token_embedding(text) + self.positional_embedding[:text.shape[1]]
+            pos = self.positional_embedding[:text.shape[1]]
+            if self.token_embedding.weight.dtype == pos.dtype == torch.float32:      # one launch, and the bits of the two stock operations
+                x = ops.embed_tokens(text.contiguous(), self.token_embedding.weight, pos=pos)
+            else:
+                x = self.token_embedding(text) + pos
             x = self.transformer.forward_frozen(x, final_ln=(self.ln_final.weight.detach().float(), self.ln_final.bias.detach().float(),
                                                              self.ln_final.eps), owns_x=True)
         if not want_cls and not apply_project:          # (the training step gathers the EOT rows itself, run/train.py:124: four launches saved)
