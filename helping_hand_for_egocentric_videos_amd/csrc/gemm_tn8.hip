@@ -37,10 +37,13 @@ struct Tn8Params {
 
 // One tile of the output for one slice of the tokens: 2 x 2 waves of (16 WT) x (16 WT), 32 tokens at a time.
 //
-// A step is 32 tokens: WT^2 matrix instructions on fragments that the previous step has read, while this one reads the next.  Each of the two
-// LDS buffers holds a tile; a step also puts the tile after next into LDS and requests the one two further on, which gives a request two tiles'
-// time.  WT = 8 (256 x 256, one wave to a SIMD, 256 accumulators): 16 KB of fragments feed 64 instructions of 16 cycles, 512 of whose 1024 cycles the four
-// waves' reads take of LDS; WT = 4 (128 x 128) reads as many bytes for a quarter of the products and is bound by LDS, and is for small outputs.
+// A step is 32 tokens: WT^2 matrix instructions for each wave.  LDS holds four tiles of 32 tokens and the registers are on their way with two more, so that a
+// request has two steps' time before its data are put into LDS, and a tile stands there a step before its first fragment is read: one barrier a step.
+// WT = 8 (256 x 256, one wave to a SIMD, 256 accumulators): 16 KB of fragments feed 64 instructions of 16 cycles; the four waves' reads take 512 of those
+//   1024 cycles of LDS, the writes 256.  Bound by the matrix core and the power that it may draw: 65 552 tokens x 1024 x 4096 with db 449 us = 1224 TFLOP/s, where a
+//   library product of 8192^3 in bf16 reaches 1263 on the same card, and its product of this shape and layout, from operands that are bf16 already, 818.
+// WT = 4 (128 x 128, two workgroups to a CU) for outputs and lengths that give the other too few workgroups; bound by latencies (7 us of a launch with one step,
+//   0.3 us for each further one): 2464 x 768 x 768 takes 20 us with the launch that joins its five slices.
 template <int WT, bool VEC>
 __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Params p) {
     constexpr int BLOCK = 32 * WT, BK = 32, ROW = BLOCK * 2, HALF = BK * ROW;     // bytes of a row and of one operand's tile in LDS
@@ -228,13 +231,13 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
             step(t + 2, std::integral_constant<int, 2>());
             step(t + 3, std::integral_constant<int, 3>());
         }
-    }
-    if constexpr (WT == 8) {
-        // the compiler does not see that these are results of matrix instructions: 16 wait states where 11 are needed before anything else reads one
+        if constexpr (WT == 8) {
+            // the compiler does not see that these are results of matrix instructions: 16 wait states where 11 are needed before anything else reads one
 #pragma unroll
-        for (int i = 0; i < WT; ++i)
+            for (int i = 0; i < WT; ++i)
 #pragma unroll
-            for (int j = 0; j < WT; ++j) asm volatile("s_nop 15" : "+a"(acc[i][j]));
+                for (int j = 0; j < WT; ++j) asm volatile("s_nop 15" : "+a"(acc[i][j]));
+        }
     }
     if (p.colsum != nullptr) {                                                            // the RA threads of a column, in row order
         float* buf = (float*)smem;
@@ -308,7 +311,8 @@ struct Tn8Plan { int wt, tiles_m, tiles_n, splits; };
 static Tn8Plan tn8_plan(int M, int N, int64_t K) {
     Tn8Plan q;
     const int64_t large = ((int64_t)(M + 255) / 256) * ((N + 255) / 256);
-    // 256 x 256 tiles (one workgroup to a CU) where slices of 1024 tokens or more of them fill the chip
+    // 256 x 256 tiles (one workgroup to a CU) where slices of 1024 tokens or more of them fill the chip: 32 776 x 512 x 2048 86 us (94 in tiles of 128), but
+    // 12 320 x 768 x 768, 117 of them, 44 us (36)
     q.wt = large * ((K + 1023) / 1024) >= 256 && M > 128 && N > 128 ? 8 : 4;
     const int block = 32 * q.wt;
     q.tiles_m = (M + block - 1) / block;

@@ -88,3 +88,45 @@ def test_cpu_tensors_and_wrong_types_are_refused():
         ops.gemm_tn_act8(f.bfloat16().t(), f.to(torch.float8_e4m3fn), f)
     with pytest.raises(ValueError, match="rows that do not overlap"):
         ops.gemm_tn_act8(torch.zeros(1, 8, dtype=torch.bfloat16).expand(4, 8), f.to(torch.float8_e4m3fn), f)
+
+
+def test_pinned_matrix_products_keep_their_distances(tmp_path):
+    """gemm_tn8.hip's matrix instructions in inline asm are opaque to hipcc: in what it makes of them, no vector instruction writes a source of one right before it, nothing
+    but them touches an accumulator inside the loop, and behind the last one every accumulator is read only after 16 wait states of its own (s_nop 15)."""
+    import os
+    import re
+    import subprocess
+    from helping_hand_for_egocentric_videos_amd import build
+    if not os.path.exists(build.HIPCC):
+        pytest.skip("no hipcc")
+    out = str(tmp_path / "gemm_tn8.s")
+    subprocess.run([build.HIPCC] + build.FLAGS + ["--cuda-device-only", "-S", os.path.join(build.CSRC, "gemm_tn8.hip"), "-o", out], check=True, capture_output=True)
+    text = open(out).read()
+
+    def regs(token):
+        m = re.match(r"([va])\[(\d+):(\d+)\]$", token)
+        if m:
+            return {m[1] + str(i) for i in range(int(m[2]), int(m[3]) + 1)}
+        return {token} if re.match(r"[va]\d+$", token) else set()
+    found = 0
+    for body in re.findall(r"^_Z15gemm_tn8_kernelILi8E.*?\.end_amdhsa_kernel", text, re.S | re.M):
+        insts = []
+        for line in body.split("\n"):
+            line = line.split(";")[0].strip()
+            if re.match(r"[a-z]+_", line):
+                op, _, rest = line.partition(" ")
+                insts.append((op, [t.split()[0] for t in re.split(r",\s*", rest) if t]))
+        at = [i for i, (op, _) in enumerate(insts) if op.startswith("v_mfma")]
+        assert len(at) == 4 * 64
+        found += 1
+        for i in at:
+            sources = set().union(*[regs(t) for t in insts[i][1][1:3]])
+            for op, args in insts[max(0, i - 6):i]:
+                assert not (op.startswith("v_") and not op.startswith("v_mfma") and args and regs(args[0]) & sources), (op, args, insts[i])
+        for op, args in insts[at[0]:at[-1] + 1]:
+            assert op.startswith("v_mfma") or not any(t.startswith("a") and regs(t) for t in args), (op, args)
+        nops = [i for i, (op, args) in enumerate(insts) if op == "s_nop" and args == ["15"]]
+        assert len(nops) >= 64 and nops[0] > at[-1]
+        for op, args in insts[at[-1] + 1:nops[0]]:              # (the zeros of a slice without tokens are written here)
+            assert not any(regs(t) and t.startswith("a") for t in args[1:]), (op, args)
+    assert found == 2

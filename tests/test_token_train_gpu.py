@@ -285,6 +285,69 @@ def test_residual_norm_bwd(rows, cols, gate, post, pre, rms, xt, yt, ht):
                 within(v, ref, 2 * N * (mag() * torch.ones_like(rx)).sum(0) + 1e-30, "residual_norm " + name)
 
 
+@pytest.mark.parametrize("rows,cols,groups", [(16504, 1024, 4), (17003, 1000, 1), (8402, 2048, 2), (33500, 512, 1)])
+@pytest.mark.parametrize("post,pre", [(True, True), (False, True), (True, False)])
+def test_residual_norm_of_large_calls(rows, cols, groups, post, pre):
+    """Over 96 MB of outputs: the non-temporal kernels and four rows at a time, against the same rows in calls of a few thousand (whose kernels the tests above hold to their
+    definition).  Rows are independent, so that they agree bit for bit up to the order of a sum over a row's waves, which is the same; column sums to their bound."""
+    gate = "group" if groups > 1 else "channel"
+    s = make_block(rows, cols, gate, post, pre, False, F32, BF16, groups=groups)
+    kw = dict(res_scale=0.75, post=s["post"], pre=s["pre"], gate_tanh=True)
+    dxn, dh = rnd(rows, cols, seed=31), rnd(rows, cols, seed=32, dtype=BF16) if pre else None
+    x_new, h = ops.residual_norm(s["x"], s["y"], gate=s["gate"], **kw)
+    got = ops.residual_norm_bwd(s["x"], s["y"], dxn, dh, gate=s["gate"], **kw)
+    sums = None
+    cut = lambda t, i, j: None if t is None else t[i:j].contiguous()  # noqa: E731
+    each = rows // groups
+    for k in range(groups):
+        for i in range(k * each, (k + 1) * each, 2100):
+            j = min(i + 2100, (k + 1) * each)
+            g = s["gate"][k] if groups > 1 else s["gate"]
+            a, b = ops.residual_norm(cut(s["x"], i, j), cut(s["y"], i, j), gate=g, **kw)
+            assert torch.equal(a, x_new[i:j]) and (h is None or torch.equal(b, h[i:j]))
+            p = ops.residual_norm_bwd(cut(s["x"], i, j), cut(s["y"], i, j), cut(dxn, i, j), cut(dh, i, j), gate=g, **kw)
+            assert torch.equal(p.dx, got.dx[i:j]) and torch.equal(p.dy, got.dy[i:j])
+            add = [None if t is None else t.double() for t in p[2:]]
+            if groups > 1:
+                rest = torch.zeros(groups, cols, dtype=torch.float64, device=DEV)
+                rest[k] = add[0]
+                add[0] = rest
+            sums = add if sums is None else [None if t is None else t + v for t, v in zip(sums, add)]
+    for name, t, v in zip(got._fields[2:], got[2:], sums):
+        assert (t is None) == (v is None)
+        if t is not None:                                           # both sides add about `rows` terms of a size near 1 (xh, dh, d, gammas) in fp32
+            assert float((t.double() - v).abs().max()) <= 2 * (rows + 64) * U * 40 * rows ** 0.5, name
+
+
+def test_large_outputs_of_embed_and_act8():
+    """Over 96 MB: the non-temporal kernels give what calls on a part of the rows give."""
+    w, pos, ids = rnd(1000, 1024, seed=1), rnd(77, 1024, seed=2), rints(0, 1000, (420, 77), seed=3)
+    for ot in (F32, BF16):
+        for wt in (F32, BF16):
+            n = 420 if ot == F32 else 840
+            i = ids.repeat(n // 420, 1)
+            big = ops.embed_tokens(i, w.to(wt), scale=3.0, pos=pos, out_dtype=ot)
+            assert big.numel() * big.element_size() > 96 << 20
+            assert torch.equal(big[-3:], ops.embed_tokens(i[-3:], w.to(wt), scale=3.0, pos=pos, out_dtype=ot))
+            assert torch.equal(big[:100], ops.embed_tokens(i[:100], w.to(wt), scale=3.0, pos=pos, out_dtype=ot))
+    for dt, rows, cols in ((F32, 13000, 2048), (BF16, 26000, 2056)):
+        u, da = rnd(rows, cols, seed=4, dtype=dt), rnd(rows, cols, seed=5, dtype=dt)
+        a, q, sc = ops.act8(u, ops.ACT_QUICKGELU)
+        du, a2 = ops.act8_bwd(q, sc, da, ops.ACT_QUICKGELU, want_out=True)
+        for i in (slice(0, 50), slice(rows - 50, rows)):
+            b, r, t = ops.act8(u[i].contiguous(), ops.ACT_QUICKGELU)
+            assert torch.equal(a[i], b) and torch.equal(q[i].view(torch.uint8), r.view(torch.uint8)) and torch.equal(sc[i], t)
+            dv, b2 = ops.act8_bwd(r, t, da[i].contiguous(), ops.ACT_QUICKGELU, want_out=True)
+            assert torch.equal(du[i], dv) and torch.equal(a2[i], b2)
+    dy = rnd(340, 77, 2048, seed=6, dtype=BF16)                      # a gradient over 96 MB with positions: read past the cache
+    assert dy.numel() * 2 > 96 << 20
+    i = rints(0, 5000, (340, 77), seed=7)
+    dw, dpos = ops.embed_tokens_bwd(i, dy, 5000, pos_grad=True)
+    ref, bound = embed_grad_ref(i, dy, 5000, 1.0, None)
+    within(dw, ref, bound, "embed grad, large")
+    within(dpos, dy.double().sum(0), 342 * U * dy.double().abs().sum(0), "pos grad, large")
+
+
 def test_residual_norm_bwd_against_differences():
     """A directional derivative of the kernels' own forward (fp32 in and out) against the gradients: central differences of step t are off by t^2 / 6 of the third
     derivative (below 50 of the sizes here: unit rows, gammas near 1) and by the forward's rounding / t."""
@@ -457,6 +520,15 @@ def test_gemm_tn_act8(K, M, N):
     u = rnd(K, N, seed=1, dtype=BF16) * torch.exp(2 * rnd(K, 1, seed=2)).to(BF16)
     _, q, s = ops.act8(u, want_out=False)
     check_wgrad(rnd(K, M, seed=3, dtype=BF16), q, s, "act8 wgrad")
+
+
+@pytest.mark.parametrize("K,M,N", [(66000, 264, 272), (132001, 136, 400), (11003, 1030, 1037), (45000, 512, 520), (40961, 768, 1024)])
+def test_gemm_tn_act8_in_large_tiles(K, M, N):
+    """Enough tokens and outputs for the 256 x 256 tiles: slices that end inside a tile, slices without a token, ragged outputs, unaligned rows."""
+    assert -(-M // 256) * -(-N // 256) * -(-K // 1024) >= 256
+    u = rnd(K, N, seed=1, dtype=BF16) * torch.exp(rnd(K, 1, seed=2)).to(BF16)
+    _, q, s = ops.act8(u, want_out=False)
+    check_wgrad(rnd(K, M, seed=3, dtype=BF16), q, s, "act8 wgrad, large tiles")
 
 
 def test_gemm_tn_act8_takes_every_code_and_scale_exactly():
