@@ -340,7 +340,7 @@ struct RunList {
     const u32* keys; const u32* from;                // sorted keys and the positions they came from; keys == NULL: the list of dpos, see run_key
     float* out;                                      // [rows, dim]
     float* part;                                     // [chunks][2][dim]: a chunk's first run where it began earlier, its last where it goes on
-    u32* flags;                                      // [chunks]: what crosses the border behind the chunk
+    unsigned char* flags;                            // [chunks]: what crosses the border behind the chunk
     int64_t rows;
     int accumulate, aligned;
     float scale;
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
     if (c == 0) {
         const u32 at_end = run_key(p, l, j1 - 1);
         const bool cross = j1 < p.n && (int64_t)at_end < l.rows && run_key(p, l, j1) == at_end;
-        l.flags[blockIdx.x] = !cross ? RUN_ENDS : head && key == at_end ? RUN_COVERS : RUN_STARTS;
+        l.flags[blockIdx.x] = (unsigned char)(!cross ? RUN_ENDS : head && key == at_end ? RUN_COVERS : RUN_STARTS);
     }
     for (int j = j0; j < j1 && (int64_t)key < l.rows; j += 8) {
         u32x4 v[8];
@@ -453,11 +453,28 @@ __global__ __launch_bounds__(1024) void run_join_kernel(RunParams p) {
     const int b = blockIdx.x * 16 + wave;
     int heads = 0;                                               // chunks b + 1 .. b + heads belong to the run that starts in chunk b
     if (b < p.chunks && l.flags[b] == RUN_STARTS) {
-        for (int k = b + 1;; k += 64) {
-            const uint64_t g = __ballot(k + lane < p.chunks && l.flags[k + lane] == RUN_COVERS);
-            if (~g != 0) { heads += __builtin_ctzll(~g) + 1; break; }
-            heads += 64;
+        // the chunks behind b that the run covers: the next 64, one to a lane, and for a longer run 1024 at a time, 16 bytes of the list to a lane
+        const uint64_t covers = __ballot(b + 1 + lane < p.chunks && l.flags[b + 1 + lane] == RUN_COVERS);
+        heads = ~covers ? __builtin_ctzll(~covers) : 64;
+        for (int k0 = (b + 65) & ~15, more = covers == ~0ull; more; k0 += 1024) {
+            const int k = k0 + lane * 16;
+            u32x4 f = {0u, 0u, 0u, 0u};
+            if (k < p.chunks) f = *(const u32x4*)(l.flags + k);      // (the list is padded to 16 bytes)
+            int n = 0;                                           // this lane's bytes that count (chunks behind b + 64), while the run goes on
+            bool on = true;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (k + i > b + 64) {
+                    on = on && k + i < p.chunks && ((f[i >> 2] >> (8 * (i & 3))) & 0xffu) == RUN_COVERS;
+                    n += on;
+                }
+            const uint64_t stop = __ballot(!on);
+            const int last = stop ? __builtin_ctzll(stop) : 63;
+            const int first = k0 <= b + 64 ? 16 - (b + 65 - k0) : 16;      // bytes of lane 0 that count
+            heads += last == 0 ? __shfl(n, 0, 64) : first + 16 * (last - 1) + __shfl(n, last, 64);
+            more = stop == 0;
         }
+        ++heads;                                                 // and the chunk in which it ends
     }
     if (lane == 0) heavy[wave] = heads > JOIN_LIGHT ? heads : 0;
     if (heads > 0 && heads <= JOIN_LIGHT && mine) {
@@ -560,7 +577,7 @@ static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 extern "C" int64_t hh_workspace_bytes_embed_tokens_bwd(int64_t seqs, int length, int64_t rows, int dim) {
     if (!embed_shape_ok(seqs, length, rows, dim)) return -1;
     const int64_t n = seqs * length, chunks = run_chunks(n, run_waves(dim, 8));      // (bf16; fp32 rows take more waves, and fewer chunks)
-    return 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4) + 2 * align256(4 * chunks) + 2 * align256(chunks * 2 * (int64_t)dim * 4);
+    return 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4) + 2 * align256(chunks) + 2 * align256(chunks * 2 * (int64_t)dim * 4);
 }
 
 // part i of `parts` of the zeros of out, and the workgroups that write it
@@ -601,9 +618,9 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     u32* keys[2] = {(u32*)ws, (u32*)(ws + align256(4 * n))};
     u32* from[2] = {(u32*)(ws + 2 * align256(4 * n)), (u32*)(ws + 3 * align256(4 * n))};
     u32* hist = (u32*)(ws + 4 * align256(4 * n));
-    u32* flags = (u32*)((char*)hist + align256(SORT_BLOCKS * 256 * 4));
+    unsigned char* flags = (unsigned char*)hist + align256(SORT_BLOCKS * 256 * 4);
     const int e = dy_dtype == HH_F32 ? 4 : 8;
-    const int64_t chunks = run_chunks(n, run_waves(dim, e)), flag_bytes = align256(4 * chunks), part_bytes = align256(chunks * 2 * (int64_t)dim * 4);
+    const int64_t chunks = run_chunks(n, run_waves(dim, e)), flag_bytes = align256(chunks), part_bytes = align256(chunks * 2 * (int64_t)dim * 4);
     char* part = (char*)flags + 2 * flag_bytes;
     const SortPlan sp = sort_plan(n, rows);
     int sorted = sp.passes & 1;                                                   // the buffers that hold the sorted list
@@ -626,7 +643,7 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     RunParams p;
     p.dy = dy; p.n = (int)n; p.chunk = run_chunk(n, run_waves(dim, e)); p.chunks = (int)chunks; p.dim = dim; p.length = length; p.seqs = (int)seqs;
     p.list[0] = RunList{keys[sorted], from[sorted], dweight, (float*)part, flags, rows, accumulate != 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dweight), scale};
-    p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), (u32*)((char*)flags + flag_bytes), length, 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dpos), 1.f};
+    p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), flags + flag_bytes, length, 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dpos), 1.f};
     const int need = (dim + e - 1) / e;
     const int threads = need >= 256 ? 256 : (need + 63) / 64 * 64;
     const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), dpos ? 2u : 1u);
