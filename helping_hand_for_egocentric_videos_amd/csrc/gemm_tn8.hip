@@ -45,13 +45,16 @@ struct Tn8Params {
 // WT = 4 (128 x 128, two workgroups to a CU) for outputs and lengths that give the other too few workgroups; bound by latencies (7 us of a launch with one step,
 //   0.3 us for each further one): 2464 x 768 x 768 takes 20 us with the launch that joins its five slices.
 template <int WT, bool VEC>
-__global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Params p) {
+__global__ __launch_bounds__(WT == 8 ? 256 : 512) void gemm_tn8_kernel(Tn8Params p) {
+    constexpr int G = WT == 8 ? 1 : 2;                                                    // groups of four waves: every G-th tile of the slice to each
     constexpr int BLOCK = 32 * WT, BK = 32, ROW = BLOCK * 2, HALF = BK * ROW;     // bytes of a row and of one operand's tile in LDS
     constexpr int CA = BLOCK / 8, CQ = BLOCK / 16;                                       // 16-byte pieces of a row of dY / of q
     constexpr int NA = BK * CA / 256, NQ = BK * CQ / 256, RA = 256 / CA, RQ = 256 / CQ;  // pieces for a thread, rows between them
     constexpr int BUFS = 4;                                                               // tiles in LDS
-    extern __shared__ __attribute__((aligned(16))) char smem[];                           // [BUFS][dY | q][BK][BLOCK] bf16
-    const int tid = threadIdx.x, lane = tid & 63;
+    extern __shared__ __attribute__((aligned(16))) char smem_all[];                       // [G][BUFS][dY | q][BK][BLOCK] bf16
+    const int group = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    char* smem = smem_all + group * BUFS * 2 * HALF;
+    const int tid = threadIdx.x & 255, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1;
     // work in the order slice, column tile, row tile; an XCD (blockIdx.x mod 8) takes a contiguous part of it, so that its L2 holds few columns of one slice
@@ -62,7 +65,7 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
     const int m0 = tile_m * BLOCK, n0 = tile_n * BLOCK;
     const int64_t k0 = (int64_t)split * p.k_per_split;
     const int64_t k1 = k0 + p.k_per_split < p.K ? k0 + p.k_per_split : p.K;
-    const int nk = k1 > k0 ? (int)((k1 - k0 + BK - 1) / BK) : 0;                        // (0 for a slice behind the last token: zeros are written)
+    const int nk = k1 > k0 ? (int)((k1 - k0 + G * BK - 1) / (G * BK)) : 0;              // tiles of a group (0 for a slice behind the last token: zeros are written)
 
     // Buffer loads: a resource ends with the slice, and what lies behind reads as zero -- the rows that fill up the last tile, and the tiles behind it.  Columns behind
     // the last belong to the next row or are zero; their products are not stored.  The resource moves with the tile that is requested, so that offsets stay
@@ -86,11 +89,12 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
     // (the last row of a strided operand ends where its columns do, not where a next row would begin)
     a_str.left -= (int64_t)(p.lda - p.M) * 2;
     q_str.left -= p.ldq - p.N;
+    if (group) { a_str.next(BK * lda); q_str.next(BK * ldq); s_str.next(BK * lds); }
     struct Regs { u32x4 a[NA], q[NQ]; float s[NQ]; };
     __amdgpu_buffer_rsrc_t a_res, q_res, s_res;
     // piece i of the next tile's rows of dY / of q: pieces in order, tiles in order
     auto fetch_a = [&](int i, Regs& r) {
-        if (i == 0) a_res = a_str.next(BK * lda);
+        if (i == 0) a_res = a_str.next(G * BK * lda);
         const unsigned off = a_off + (unsigned)(RA * i) * lda;
         if (VEC) r.a[i] = __builtin_amdgcn_raw_buffer_load_b128(a_res, off, 0, 0);
         else {
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
         }
     };
     auto fetch_q = [&](int i, Regs& r) {
-        if (i == 0) { q_res = q_str.next(BK * ldq); s_res = s_str.next(BK * lds); }
+        if (i == 0) { q_res = q_str.next(G * BK * ldq); s_res = s_str.next(G * BK * lds); }
         const unsigned off = q_off + (unsigned)(RQ * i) * ldq;
         if (VEC) r.q[i] = __builtin_amdgcn_raw_buffer_load_b128(q_res, off, 0, 0);
         else {
@@ -239,25 +243,42 @@ __global__ __launch_bounds__(256, WT == 8 ? 1 : 2) void gemm_tn8_kernel(Tn8Param
                 for (int j = 0; j < WT; ++j) asm volatile("s_nop 15" : "+a"(acc[i][j]));
         }
     }
-    if (p.colsum != nullptr) {                                                            // the RA threads of a column, in row order
-        float* buf = (float*)smem;
+    if constexpr (G == 2) {
+        // the other group's half of the accumulators goes to it through LDS: group 0 ends with the first half of the rows, group 1 with the second
+        f32x4* buf = (f32x4*)smem_all + tid;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) buf[(ra0 * CA + ca) * 8 + j] = db[j];
+        for (int i = 0; i < WT; ++i)
+#pragma unroll
+            for (int j = 0; j < WT / 2; ++j) buf[((group * WT + i) * (WT / 2) + j) * 256] = group ? acc[i][j] : acc[i][WT / 2 + j];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WT; ++i)
+#pragma unroll
+            for (int j = 0; j < WT / 2; ++j) {
+                const f32x4 other = buf[(((group ^ 1) * WT + i) * (WT / 2) + j) * 256];
+                acc[i][j] = group ? acc[i][WT / 2 + j] + other : acc[i][j] + other;      // (the sum of two, the same in either order)
+            }
+    }
+    if (p.colsum != nullptr) {                                                            // the G RA threads of a column, in the order of groups and rows
+        float* buf = (float*)smem_all;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) buf[((group * RA + ra0) * CA + ca) * 8 + j] = db[j];
         __syncthreads();
         const int m = m0 + tid;
-        if (tid < BLOCK && m < p.M) {
+        if (group == 0 && tid < BLOCK && m < p.M) {
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < RA; ++i) sum += buf[i * BLOCK + tid];
+            for (int i = 0; i < G * RA; ++i) sum += buf[i * BLOCK + tid];
             p.colsum[((int64_t)split * p.tiles_n + tile_n) * p.M + m] = sum;
         }
     }
     const int mr = lane & 15;
     float* Cp = p.C + (int64_t)split * p.M * p.N;
 #pragma unroll
-    for (int tm = 0; tm < WT; ++tm) {
-        const int m = m0 + wm * 16 * WT + tm * 16 + mr;
+    for (int tm = 0; tm < WT / G; ++tm) {
+        const int m = m0 + wm * 16 * WT + (group * (WT / G) + tm) * 16 + mr;
         if (m >= p.M) continue;
 #pragma unroll
         for (int tn = 0; tn < WT; ++tn) {
@@ -318,7 +339,7 @@ static Tn8Plan tn8_plan(int M, int N, int64_t K) {
     q.tiles_m = (M + block - 1) / block;
     q.tiles_n = (N + block - 1) / block;
     const int64_t tiles = (int64_t)q.tiles_m * q.tiles_n;
-    int64_t s = (q.wt == 8 ? 256 : 512) / tiles;
+    int64_t s = 256 / tiles;
     // no slice below 512 tokens: every slice leaves a plane of dW to write and to add (2464 x 768 x 768: 10 slices 25.4 us, 5 slices 21.3)
     const int64_t most = (K + 511) / 512;
     if (s > most) s = most;
@@ -349,19 +370,21 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
     Tn8Params p;
     p.A = (const bf16_t*)dy; p.lda = ld_dy; p.q = (const unsigned char*)q; p.ldq = ldq; p.scale = scale;
     p.M = M; p.N = N; p.K = K; p.groups = (N + 127) / 128; p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.splits = pl.splits;
-    const int tokens = 32;
+    const int tokens = pl.wt == 8 ? 32 : 64;                                    // (a tile for each group)
     p.k_per_split = ((K + tokens - 1) / tokens + pl.splits - 1) / pl.splits * tokens;
     p.C = pl.splits == 1 ? dw : (float*)workspace;
     float* cs = (float*)workspace + (pl.splits == 1 ? 0 : (n * pl.splits + 3) / 4 * 4);
     p.colsum = db == nullptr ? nullptr : cs;
     const bool vec = M % 8 == 0 && ld_dy % 8 == 0 && HH_ALIGNED16(dy) && N % 16 == 0 && ldq % 16 == 0 && HH_ALIGNED16(q);
     const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n * pl.splits));
-    const int lds = 4 * 2 * 32 * 64 * pl.wt;
-    if (pl.wt == 8) {
+    const int lds = 128 * 1024;
+    {
         static std::atomic<uint64_t> attr{0};
         if (hh_attr_needed(attr)) {
             hipError_t e = hipFuncSetAttribute((const void*)gemm_tn8_kernel<8, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
             if (e == hipSuccess) e = hipFuncSetAttribute((const void*)gemm_tn8_kernel<8, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            if (e == hipSuccess) e = hipFuncSetAttribute((const void*)gemm_tn8_kernel<4, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            if (e == hipSuccess) e = hipFuncSetAttribute((const void*)gemm_tn8_kernel<4, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
             HH_REQUIRE(e == hipSuccess, HH_ERR_LAUNCH, "hh_gemm_tn_act8: %s", hipGetErrorString(e));
             hh_attr_done(attr);
         }
@@ -370,8 +393,8 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
         if (vec) hipLaunchKernelGGL((gemm_tn8_kernel<8, true>), grid, dim3(256), lds, s, p);
         else hipLaunchKernelGGL((gemm_tn8_kernel<8, false>), grid, dim3(256), lds, s, p);
     } else {
-        if (vec) hipLaunchKernelGGL((gemm_tn8_kernel<4, true>), grid, dim3(256), lds, s, p);
-        else hipLaunchKernelGGL((gemm_tn8_kernel<4, false>), grid, dim3(256), lds, s, p);
+        if (vec) hipLaunchKernelGGL((gemm_tn8_kernel<4, true>), grid, dim3(512), lds, s, p);
+        else hipLaunchKernelGGL((gemm_tn8_kernel<4, false>), grid, dim3(512), lds, s, p);
     }
     if (pl.splits > 1 || db) {
         const int wide = n % 4 == 0;
