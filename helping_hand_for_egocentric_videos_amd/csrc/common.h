@@ -15,6 +15,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+// wide accesses at any element's address (of fp32, of bf16, of bytes): the same instructions, which take every byte address
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4), may_alias));
+typedef unsigned int u32x4_any __attribute__((ext_vector_type(4), aligned(2), may_alias));
+typedef unsigned int u32x2_any __attribute__((ext_vector_type(2), aligned(1), may_alias));
 
 void hh_set_error(const char* fmt, ...);
 int hh_check_launch(const char* what);

@@ -30,8 +30,9 @@ struct Tn8Params {
     const unsigned char* q; int64_t ldq;
     const float* scale;                    // [K][groups]
     float* C;                              // [splits][M][N]
-    float* colsum;                         // [splits * tiles_n][M] or NULL
+    float* colsum;                         // [splits * db_planes][M] or NULL
     int M, N, groups, tiles_m, tiles_n, splits;
+    int db_planes;                         // column tiles that share the tokens of a slice for db
     int64_t K, k_per_split;                // k_per_split: a multiple of the tile's tokens
 };
 
@@ -42,8 +43,9 @@ struct Tn8Params {
 // WT = 8 (256 x 256, one wave to a SIMD, 256 accumulators): 16 KB of fragments feed 64 instructions of 16 cycles; the four waves' reads take 512 of those
 //   1024 cycles of LDS, the writes 256.  Bound by the matrix core and the power that it may draw: 65 552 tokens x 1024 x 4096 with db 449 us = 1224 TFLOP/s, where a
 //   library product of 8192^3 in bf16 reaches 1263 on the same card, and its product of this shape and layout, from operands that are bf16 already, 818.
-// WT = 4 (128 x 128, two workgroups to a CU) for outputs and lengths that give the other too few workgroups; bound by latencies (7 us of a launch with one step,
-//   0.3 us for each further one): 2464 x 768 x 768 takes 20 us with the launch that joins its five slices.
+// WT = 4 (128 x 128) for outputs and lengths that give the other too few workgroups: bound by a step's latencies (0.3 us with one wave to a SIMD, where its products take
+//   0.1), so that two groups of four waves take every second tile each and add their sums at the end (12 320 x 768 x 768 35.9 -> 31.5 us).  2464 x 768 x 768 takes
+//   19 us with the launch that joins its five slices.
 template <int WT, bool VEC>
 __global__ __launch_bounds__(WT == 8 ? 256 : 512) void gemm_tn8_kernel(Tn8Params p) {
     constexpr int G = WT == 8 ? 1 : 2;                                                    // groups of four waves: every G-th tile of the slice to each
@@ -70,70 +72,80 @@ __global__ __launch_bounds__(WT == 8 ? 256 : 512) void gemm_tn8_kernel(Tn8Params
     // Buffer loads: a resource ends with the slice, and what lies behind reads as zero -- the rows that fill up the last tile, and the tiles behind it.  Columns behind
     // the last belong to the next row or are zero; their products are not stored.  The resource moves with the tile that is requested, so that offsets stay
     // below 2^31 whatever the slice's length.
+    //
+    // Any alignment and width (not VEC): the resources begin at a multiple of four bytes at or before the operand and end at one at or behind its end (never in
+    // another page than a byte of the operand), a piece is read as the five dwords that hold it and shifted into place; the rows of a thread and its tiles lie a
+    // multiple of four bytes apart, so that it has one shift.  Rows behind the last are asked for behind the end, so that they are zeros here too.
     const int ra0 = tid / CA, rq0 = tid / CQ, ca = tid % CA, cq = tid % CQ;
     const unsigned lda = (unsigned)p.lda * 2, ldq = (unsigned)p.ldq, lds = (unsigned)p.groups * 4;      // bytes
-    const unsigned a_off = (unsigned)ra0 * lda + (unsigned)(m0 + ca * 8) * 2, q_off = (unsigned)rq0 * ldq + (unsigned)(n0 + cq * 16);
+    const char* a_at = (const char*)(p.A + k0 * p.lda);
+    const char* q_at = (const char*)(p.q + k0 * p.ldq);
+    const unsigned a_mis = VEC ? 0 : (unsigned)(uintptr_t)a_at & 3, q_mis = VEC ? 0 : (unsigned)(uintptr_t)q_at & 3;
+    const unsigned a_row = a_mis + (unsigned)ra0 * lda, q_row = q_mis + (unsigned)rq0 * ldq;
+    const unsigned a_off = a_row + (unsigned)(m0 + ca * 8) * 2, q_off = q_row + (unsigned)(n0 + cq * 16);
     const unsigned s_off = (unsigned)rq0 * lds + (unsigned)((n0 + cq * 16) / 128) * 4;
     struct Stream {
-        const char* at; int64_t left;
+        const char* at; int64_t left; int end;
         __device__ __amdgpu_buffer_rsrc_t next(unsigned bytes) {                          // the resource of this tile; moves on to the next
-            const int64_t n = left < 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left;
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, (int)n, 0x27000);
+            end = left < 0 ? 0 : left > 0x7ffffffc ? 0x7ffffffc : (int)left;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, VEC ? end : (end + 3) & ~3, 0x27000);
             at += bytes; left -= bytes;
             return r;
         }
     };
     const int64_t len = k1 - k0;
-    Stream a_str = {(const char*)(p.A + k0 * p.lda), len * (int64_t)lda}, q_str = {(const char*)(p.q + k0 * p.ldq), len * (int64_t)ldq},
-           s_str = {(const char*)(p.scale + k0 * p.groups), len * (int64_t)lds};
+    Stream a_str = {a_at - a_mis, len * (int64_t)lda + a_mis, 0}, q_str = {q_at - q_mis, len * (int64_t)ldq + q_mis, 0},
+           s_str = {(const char*)(p.scale + k0 * p.groups), len * (int64_t)lds, 0};
     // (the last row of a strided operand ends where its columns do, not where a next row would begin)
     a_str.left -= (int64_t)(p.lda - p.M) * 2;
     q_str.left -= p.ldq - p.N;
     if (group) { a_str.next(BK * lda); q_str.next(BK * ldq); s_str.next(BK * lds); }
-    struct Regs { u32x4 a[NA], q[NQ]; float s[NQ]; };
+    struct Regs { u32x4 a[NA], q[NQ]; unsigned a5[VEC ? 1 : NA], q5[VEC ? 1 : NQ]; float s[NQ]; };
     __amdgpu_buffer_rsrc_t a_res, q_res, s_res;
     // piece i of the next tile's rows of dY / of q: pieces in order, tiles in order
     auto fetch_a = [&](int i, Regs& r) {
         if (i == 0) a_res = a_str.next(G * BK * lda);
         const unsigned off = a_off + (unsigned)(RA * i) * lda;
-        if (VEC) r.a[i] = __builtin_amdgcn_raw_buffer_load_b128(a_res, off, 0, 0);
+        if constexpr (VEC) r.a[i] = __builtin_amdgcn_raw_buffer_load_b128(a_res, off, 0, 0);
         else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                r.a[i][j] = (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(a_res, off + 4 * j, 0, 0) |
-                            (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(a_res, off + 4 * j + 2, 0, 0) << 16;
+            const unsigned at = a_row + (unsigned)(RA * i) * lda < (unsigned)a_str.end ? off & ~3u : 0x80000000u;
+            r.a[i] = __builtin_amdgcn_raw_buffer_load_b128(a_res, at, 0, 0);
+            r.a5[i] = __builtin_amdgcn_raw_buffer_load_b32(a_res, at + 16, 0, 0);
         }
     };
     auto fetch_q = [&](int i, Regs& r) {
         if (i == 0) { q_res = q_str.next(G * BK * ldq); s_res = s_str.next(G * BK * lds); }
         const unsigned off = q_off + (unsigned)(RQ * i) * ldq;
-        if (VEC) r.q[i] = __builtin_amdgcn_raw_buffer_load_b128(q_res, off, 0, 0);
+        if constexpr (VEC) r.q[i] = __builtin_amdgcn_raw_buffer_load_b128(q_res, off, 0, 0);
         else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                unsigned w = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w |= (unsigned)(unsigned char)__builtin_amdgcn_raw_buffer_load_b8(q_res, off + 4 * j + k, 0, 0) << (8 * k);
-                r.q[i][j] = w;
-            }
+            const unsigned at = q_row + (unsigned)(RQ * i) * ldq < (unsigned)q_str.end ? off & ~3u : 0x80000000u;
+            r.q[i] = __builtin_amdgcn_raw_buffer_load_b128(q_res, at, 0, 0);
+            r.q5[i] = __builtin_amdgcn_raw_buffer_load_b32(q_res, at + 16, 0, 0);
         }
         r.s[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(s_res, s_off + (unsigned)(RQ * i) * lds, 0, 0));
+    };
+    auto shifted = [](const u32x4& v, unsigned v5, unsigned byte) -> u32x4 {             // 16 bytes from byte 0 .. 3 of five dwords
+        return (u32x4){__builtin_amdgcn_alignbyte(v[1], v[0], byte), __builtin_amdgcn_alignbyte(v[2], v[1], byte), __builtin_amdgcn_alignbyte(v[3], v[2], byte),
+                       __builtin_amdgcn_alignbyte(v5, v[3], byte)};
     };
     float db[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) db[j] = 0.f;
-    int db_tile = p.colsum != nullptr ? tile_n : -1;     // db: the column tiles share the tokens, each adds up every tiles_n-th tile's rows on their way into LDS
+    // db: db_planes of the column tiles share the tokens, each adds up every db_planes-th tile's rows on their way into LDS
+    int db_tile = p.colsum != nullptr && tile_n < p.db_planes ? tile_n : -1;
     auto put_a = [&](int t, int i, Regs& r) {
         const int row = ra0 + RA * i;
+        if constexpr (!VEC) r.a[i] = shifted(r.a[i], r.a5[i], a_off & 3);
         if (t == db_tile) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) { db[2 * j] += bf16_lo_to_f32(r.a[i][j]); db[2 * j + 1] += bf16_hi_to_f32(r.a[i][j]); }
-            if (i == NA - 1) db_tile += p.tiles_n;
+            if (i == NA - 1) db_tile += p.db_planes;
         }
         *(u32x4*)(smem + (t & (BUFS - 1)) * 2 * HALF + row * ROW + ((ca ^ tn8_key(row)) << 4)) = r.a[i];
     };
-    auto put_q = [&](int t, int i, int h, const Regs& r) {                                // half h of piece i: 8 values, 16 bytes of bf16
+    auto put_q = [&](int t, int i, int h, Regs& r) {                                // half h of piece i: 8 values, 16 bytes of bf16
         const int row = rq0 + RQ * i;
+        if constexpr (!VEC) { if (h == 0) r.q[i] = shifted(r.q[i], r.q5[i], q_off & 3); }
         u32x4 w;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -260,7 +272,7 @@ __global__ __launch_bounds__(WT == 8 ? 256 : 512) void gemm_tn8_kernel(Tn8Params
                 acc[i][j] = group ? acc[i][WT / 2 + j] + other : acc[i][j] + other;      // (the sum of two, the same in either order)
             }
     }
-    if (p.colsum != nullptr) {                                                            // the G RA threads of a column, in the order of groups and rows
+    if (p.colsum != nullptr && tile_n < p.db_planes) {                                                            // the G RA threads of a column, in the order of groups and rows
         float* buf = (float*)smem_all;
         __syncthreads();
 #pragma unroll
@@ -271,7 +283,7 @@ __global__ __launch_bounds__(WT == 8 ? 256 : 512) void gemm_tn8_kernel(Tn8Params
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < G * RA; ++i) sum += buf[i * BLOCK + tid];
-            p.colsum[((int64_t)split * p.tiles_n + tile_n) * p.M + m] = sum;
+            p.colsum[((int64_t)split * p.db_planes + tile_n) * p.M + m] = sum;
         }
     }
     const int mr = lane & 15;
@@ -283,7 +295,7 @@ __global__ __launch_bounds__(WT == 8 ? 256 : 512) void gemm_tn8_kernel(Tn8Params
 #pragma unroll
         for (int tn = 0; tn < WT; ++tn) {
             const int n = n0 + wn * 16 * WT + tn * 16 + 4 * g;
-            if (n + 4 <= p.N && p.N % 4 == 0) *(f32x4*)(Cp + (int64_t)m * p.N + n) = acc[tn][tm];
+            if (n + 4 <= p.N) *(f32x4_any*)(Cp + (int64_t)m * p.N + n) = acc[tn][tm];
             else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -293,26 +305,23 @@ __global__ __launch_bounds__(WT == 8 ? 256 : 512) void gemm_tn8_kernel(Tn8Params
     }
 }
 
-// dW and db from their planes, added in order: blockIdx.x < blocks: dW, a piece of 4 (wide) or 1 to a thread;  behind them 64 channels of db to a workgroup, whose
+// dW and db from their planes, added in order: blockIdx.x < blocks: dW, four values to a thread;  behind them 64 channels of db to a workgroup, whose
 // waves take a quarter of the planes each
 __global__ __launch_bounds__(256) void tn8_join_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, int splits, const float* __restrict__ cs_part, float* __restrict__ cs,
-                                                       int m, int cs_planes, int wide, int blocks) {
+                                                       int m, int cs_planes, int blocks) {
     if ((int)blockIdx.x < blocks) {
         const int64_t stride = (int64_t)blocks * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-        if (wide) {
-            for (int64_t i = first; i < n / 4; i += stride) {
-                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t i = first; i < n / 4; i += stride) {
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-                for (int s = 0; s < splits; ++s) a += *((const f32x4*)(part + s * n) + i);
-                *((f32x4*)out + i) = a;
-            }
-        } else {
-            for (int64_t i = first; i < n; i += stride) {
-                float a = 0.f;
-#pragma unroll 8
-                for (int s = 0; s < splits; ++s) a += part[s * n + i];
-                out[i] = a;
-            }
+            for (int s = 0; s < splits; ++s) a += *(const f32x4_any*)(part + s * n + 4 * i);
+            *((f32x4*)out + i) = a;
+        }
+        if (first < n % 4) {
+            const int64_t i = n / 4 * 4 + first;
+            float a = 0.f;
+            for (int s = 0; s < splits; ++s) a += part[s * n + i];
+            out[i] = a;
         }
         return;
     }
@@ -354,7 +363,7 @@ extern "C" int64_t hh_workspace_bytes_gemm_tn_act8(int M, int N, int64_t K) {
     if (!tn8_shape_ok(M, N, K)) return -1;
     const Tn8Plan q = tn8_plan(M, N, K);
     const int64_t db = (int64_t)q.splits * q.tiles_n * M;
-    return (q.splits == 1 ? db : ((int64_t)q.splits * M * N + 3) / 4 * 4 + db) * 4;
+    return q.splits == 1 ? 0 : (((int64_t)q.splits * M * N + 3) / 4 * 4 + db) * 4;
 }
 
 extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int64_t ldq, const float* scale, float* dw, float* db, int M, int N, int64_t K, void* workspace,
@@ -363,9 +372,9 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
     HH_REQUIRE(ld_dy <= (1 << 24) && ldq <= (1 << 24), HH_ERR_SHAPE, "hh_gemm_tn_act8: leading dimensions up to 2^24");
     HH_REQUIRE(dw != nullptr && (K == 0 || (dy != nullptr && q != nullptr && scale != nullptr)), HH_ERR_ALIGN, "hh_gemm_tn_act8: NULL pointer");
     HH_REQUIRE((((uintptr_t)dw) & 15) == 0, HH_ERR_ALIGN, "hh_gemm_tn_act8: dw must be 16-byte aligned");
-    HH_REQUIRE(workspace != nullptr && HH_ALIGNED16(workspace), HH_ERR_ALIGN, "hh_gemm_tn_act8: a 16-byte aligned workspace is needed");
-    hipStream_t s = (hipStream_t)stream;
     const Tn8Plan pl = tn8_plan(M, N, K);
+    HH_REQUIRE(pl.splits == 1 || (workspace != nullptr && HH_ALIGNED16(workspace)), HH_ERR_ALIGN, "hh_gemm_tn_act8: a 16-byte aligned workspace is needed");
+    hipStream_t s = (hipStream_t)stream;
     const int64_t n = (int64_t)M * N;
     Tn8Params p;
     p.A = (const bf16_t*)dy; p.lda = ld_dy; p.q = (const unsigned char*)q; p.ldq = ldq; p.scale = scale;
@@ -373,8 +382,9 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
     const int tokens = pl.wt == 8 ? 32 : 64;                                    // (a tile for each group)
     p.k_per_split = ((K + tokens - 1) / tokens + pl.splits - 1) / pl.splits * tokens;
     p.C = pl.splits == 1 ? dw : (float*)workspace;
-    float* cs = (float*)workspace + (pl.splits == 1 ? 0 : (n * pl.splits + 3) / 4 * 4);
-    p.colsum = db == nullptr ? nullptr : cs;
+    // one slice: no sums are left to join, and the first column tile's workgroups write db
+    p.db_planes = pl.splits == 1 ? 1 : pl.tiles_n;
+    p.colsum = db == nullptr ? nullptr : pl.splits == 1 ? db : (float*)workspace + (n * pl.splits + 3) / 4 * 4;
     const bool vec = M % 8 == 0 && ld_dy % 8 == 0 && HH_ALIGNED16(dy) && N % 16 == 0 && ldq % 16 == 0 && HH_ALIGNED16(q);
     const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n * pl.splits));
     const int lds = 128 * 1024;
@@ -396,11 +406,10 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
         if (vec) hipLaunchKernelGGL((gemm_tn8_kernel<4, true>), grid, dim3(512), lds, s, p);
         else hipLaunchKernelGGL((gemm_tn8_kernel<4, false>), grid, dim3(512), lds, s, p);
     }
-    if (pl.splits > 1 || db) {
-        const int wide = n % 4 == 0;
-        int64_t blocks = ((pl.splits > 1 ? (wide ? n / 4 : n) : 0) + 255) / 256;
-        if (blocks > 4096) blocks = 4096;
-        hipLaunchKernelGGL(tn8_join_kernel, dim3((unsigned)(blocks + (db ? (M + 63) / 64 : 0))), dim3(256), 0, s, p.C, dw, n, pl.splits, p.colsum, db, M, pl.splits * pl.tiles_n, wide, (int)blocks);
+    if (pl.splits > 1) {
+        int64_t blocks = (n / 4 + 255) / 256;
+        blocks = blocks < 1 ? 1 : blocks > 4096 ? 4096 : blocks;
+        hipLaunchKernelGGL(tn8_join_kernel, dim3((unsigned)(blocks + (db ? (M + 63) / 64 : 0))), dim3(256), 0, s, p.C, dw, n, pl.splits, p.colsum, db, M, pl.splits * pl.tiles_n, (int)blocks);
     }
     return hh_check_launch("hh_gemm_tn_act8");
 }

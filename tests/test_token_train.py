@@ -64,7 +64,7 @@ def test_act8_refusals():
     g = lambda dy=16, ld=8, q=16, ldq=16, s=16, dw=16, M=8, N=16, K=64, ws=16: L.hh_gemm_tn_act8(dy, ld, q, ldq, s, dw, None, M, N, K, ws, None)  # noqa: E731
     assert g(M=0) == -1 and g(N=0) == -1 and g(K=-1) == -1 and g(ld=7) == -1 and g(ldq=15) == -1 and g(ld=(1 << 24) + 8) == -1 and g(K=(1 << 30) + 1) == -1
     assert g(dy=None) == -5 and g(q=None) == -5 and g(s=None) == -5 and g(dw=None) == -5 and g(dw=8) == -5 and g(K=4096, ws=None) == -5
-    assert L.hh_workspace_bytes_gemm_tn_act8(0, 16, 64) == -1 and L.hh_workspace_bytes_gemm_tn_act8(8, 16, 64) == 4 * 8      # (a row of db)
+    assert L.hh_workspace_bytes_gemm_tn_act8(0, 16, 64) == -1 and L.hh_workspace_bytes_gemm_tn_act8(8, 16, 64) == 0      # (one slice)
     assert L.hh_workspace_bytes_gemm_tn_act8(128, 128, 1 << 16) >= 2 * 128 * 128 * 4
 
 

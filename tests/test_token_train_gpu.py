@@ -193,7 +193,7 @@ def norm_error(v, e, n, rms, ref):
     return n[0].abs() * (r * de + xh * dr) + 8 * U * (n[0].abs() * xh + ref.abs())
 
 
-CASES = [(1, 1, "none"), (3, 5, "scalar"), (7, 64, "channel"), (37, 255, "group"), (64, 256, "none"), (40, 257, "group"), (416, 512, "scalar"), (130, 768, "group"),
+CASES = [(1, 1, "none"), (9, 2, "channel"), (12, 3, "group"), (33, 6, "scalar"), (50, 1023, "channel"), (5, 4093, "none"), (3, 5, "scalar"), (7, 64, "channel"), (37, 255, "group"), (64, 256, "none"), (40, 257, "group"), (416, 512, "scalar"), (130, 768, "group"),
          (77, 1000, "channel"), (33, 1024, "channel"), (9, 1025, "scalar"), (12, 2048, "group"), (5, 2051, "channel"), (3, 4096, "none"), (2, 4095, "group")]
 
 
@@ -285,10 +285,11 @@ def test_residual_norm_bwd(rows, cols, gate, post, pre, rms, xt, yt, ht):
                 within(v, ref, 2 * N * (mag() * torch.ones_like(rx)).sum(0) + 1e-30, "residual_norm " + name)
 
 
-@pytest.mark.parametrize("rows,cols,groups", [(16504, 1024, 4), (17003, 1000, 1), (8402, 2048, 2), (33500, 512, 1)])
+@pytest.mark.parametrize("rows,cols,groups", [(16504, 1024, 4), (17003, 1000, 1), (8402, 2048, 2), (33500, 512, 1), (16801, 1023, 1), (24002, 770, 2),
+                                              (104002, 1024, 2), (215000, 512, 1), (430001, 256, 1)])
 @pytest.mark.parametrize("post,pre", [(True, True), (False, True), (True, False)])
 def test_residual_norm_of_large_calls(rows, cols, groups, post, pre):
-    """Over 96 MB of outputs: the non-temporal kernels and four rows at a time, against the same rows in calls of a few thousand (whose kernels the tests above hold to their
+    """Over 96 MB of outputs the non-temporal kernels, over 600 MB of gradients four rows at a time, against the same rows in calls of a few thousand (whose kernels the tests above hold to their
     definition).  Rows are independent, so that they agree bit for bit up to the order of a sum over a row's waves, which is the same; column sums to their bound."""
     gate = "group" if groups > 1 else "channel"
     s = make_block(rows, cols, gate, post, pre, False, F32, BF16, groups=groups)
@@ -561,6 +562,49 @@ def test_gemm_tn_act8_views_bounds_and_empty():
     pad = torch.full((M + 1, N), 3.0, device=DEV)
     ops.gemm_tn_act8(dy, big, sc, out=pad[:M])
     assert (pad[M] == 3).all()
+
+
+def placed(t, offset, junk):
+    """t's values in a buffer that is `junk` before and behind them, `offset` elements from its (aligned) begin."""
+    raw = torch.full((t.numel() + offset + 32,), junk, dtype=torch.uint8 if t.element_size() == 1 else torch.int16, device=DEV)
+    raw[offset:offset + t.numel()] = t.contiguous().view(-1).view(raw.dtype)
+    return raw[offset:offset + t.numel()].view(t.dtype).view(t.shape)
+
+
+@pytest.mark.parametrize("K,M,N", [(1, 3, 5), (33, 7, 21), (63, 129, 131), (101, 40, 1001), (1101, 77, 145), (11003, 1031, 1037)])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_gemm_tn_act8_any_address_and_nan_around_the_operands(K, M, N, offset):
+    """Rows that begin at every byte, in buffers whose other bytes are NaN: nothing but the operands counts."""
+    _, q, s = ops.act8(rnd(K, N, seed=1, dtype=BF16), want_out=False)
+    dy = rnd(K, M, seed=3, dtype=BF16)
+    want = check_wgrad(dy, q, s, "act8 wgrad")
+    got = ops.gemm_tn_act8(placed(dy, offset, 0x7fff), placed(q, offset, 0x7f), s, colsum=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 3), (9, 130), (33, 1001), (64, 768)])
+def test_act8_at_any_address(rows, cols):
+    for dt in (F32, BF16):
+        u, da = rnd(rows * cols + 1, seed=4, dtype=dt), rnd(rows * cols + 1, seed=5, dtype=dt)
+        a, q, s = ops.act8(u[1:].view(rows, cols), ops.ACT_QUICKGELU)
+        for x, y in zip((a, q, s), ops.act8(u[1:].clone().view(rows, cols), ops.ACT_QUICKGELU)):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+        du, b = ops.act8_bwd(placed(q, 1, 0x7f), s, da[1:].view(rows, cols), ops.ACT_QUICKGELU, want_out=True)
+        for x, y in zip((du, b), ops.act8_bwd(q, s, da[1:].clone().view(rows, cols), ops.ACT_QUICKGELU, want_out=True)):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("S,L,V,dim", [(3, 50, 9, 2), (5, 77, 30, 7), (40, 60, 12, 541), (64, 77, 40, 1031)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_embed_tokens_bwd_adds_once_where_pieces_share_channels(S, L, V, dim, dt):
+    """Whole numbers, whose sums are exact in any order: rows of a width that no wide access divides, added to what is there, equal the stock sum."""
+    ids, dy = rints(0, V, (S, L), seed=4), rints(-8, 9, (S, L, dim), seed=5).to(dt)
+    out = rints(-100, 100, (V, dim), seed=6).to(F32)
+    want = out.double().index_add(0, ids.view(-1), dy.view(-1, dim).double())
+    assert torch.equal(ops.embed_tokens_bwd(ids, dy, V, out=out).double(), want)
+    dw, dpos = ops.embed_tokens_bwd(ids, dy, V, pos_grad=True)
+    assert torch.equal(dw.double(), torch.zeros(V, dim, dtype=torch.float64, device=DEV).index_add(0, ids.view(-1), dy.view(-1, dim).double()))
+    assert torch.equal(dpos.double(), dy.double().sum(0))
 
 
 # ---- streams, graphs, the operators together -------------------------------------------------------------------------------------------
