@@ -31,19 +31,16 @@ __device__ __forceinline__ float act_slope(float v, int act) {
     return 1.f;
 }
 
-template <bool NT, typename V>
-__device__ __forceinline__ void put(V* p, const V& v) { if (NT) __builtin_nontemporal_store(v, p); else *p = v; }
-
 template <typename T, bool NT>
 __device__ __forceinline__ void load8(const T* p, bool whole, int n, float (&v)[8]) {
     if (whole) {
         if constexpr (sizeof(T) == 4) {
-            const f32x4 a = NT ? __builtin_nontemporal_load((const f32x4*)p) : *(const f32x4*)p;
-            const f32x4 b = NT ? __builtin_nontemporal_load((const f32x4*)(p + 4)) : *(const f32x4*)(p + 4);
+            const f32x4 a = NT ? __builtin_nontemporal_load((const f32x4_any*)p) : *(const f32x4_any*)p;
+            const f32x4 b = NT ? __builtin_nontemporal_load((const f32x4_any*)(p + 4)) : *(const f32x4_any*)(p + 4);
 #pragma unroll
             for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
         } else {
-            const u32x4 t = NT ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
+            const u32x4 t = NT ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p;
 #pragma unroll
             for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_lo_to_f32(t[j]); v[2 * j + 1] = bf16_hi_to_f32(t[j]); }
         }
@@ -56,12 +53,13 @@ template <typename T, bool NT>
 __device__ __forceinline__ void store8(T* p, bool whole, int n, const float (&v)[8]) {
     if (whole) {
         if constexpr (sizeof(T) == 4) {
-            const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-            put<NT>((f32x4*)p, a);
-            put<NT>((f32x4*)(p + 4), b);
+            const f32x4_any a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+            f32x4_any* o = (f32x4_any*)p;
+            if (NT) { __builtin_nontemporal_store(a, o); __builtin_nontemporal_store(b, (f32x4_any*)(p + 4)); } else { *o = a; *(f32x4_any*)(p + 4) = b; }
         } else {
-            const u32x4 t = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
-            put<NT>((u32x4*)p, t);
+            const u32x4_any t = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+            u32x4_any* o = (u32x4_any*)p;
+            if (NT) __builtin_nontemporal_store(t, o); else *o = t;
         }
     } else {
 #pragma unroll
@@ -92,18 +90,20 @@ __device__ __forceinline__ Act8Place act8_place(int per_row, int cols, int log_p
     q.group = row * per_row + gi;
     q.at = row * cols + gi * ACT8_GROUP + c0;
     q.left = cols - gi * ACT8_GROUP - c0;                            // may be <= 0
+    // the piece in which the row ends is moved back to be whole, inside its group: what it shares with the piece before is worked out twice, to the same values
+    if (q.left > 0 && q.left < 8 && c0 > 0) { q.at -= 8 - q.left; q.left = 8; }
     return q;
 }
 
 template <typename T, bool NT>
 __global__ __launch_bounds__(256) void act8_fwd_kernel(const T* __restrict__ u, T* __restrict__ a, unsigned char* __restrict__ q, float* __restrict__ scale, int64_t rows, int per_row,
-                                                       int cols, int log_p, int parts, int act, int aligned) {
+                                                       int cols, int log_p, int parts, int act) {
     bool on;
     const Act8Place place = act8_place(per_row, cols, log_p, parts, rows, &on);
     if (!on) return;                                                     // (16 lanes at a time: the exchange below stays inside them)
     const int64_t g = place.group, at = place.at;
     const int n = place.left;
-    const bool whole = aligned && n >= 8;
+    const bool whole = n >= 8;
     float v[8];
     load8<T, NT>(u + at, whole, n, v);
     float top = 0.f;
@@ -132,8 +132,9 @@ __global__ __launch_bounds__(256) void act8_fwd_kernel(const T* __restrict__ u, 
             if (!(fabsf(v[4 * h + j]) <= 3.402823466e38f)) w[h] |= 0x7fu << (8 * j);
     }
     if (whole) {
-        const u32x2 t = {w[0], w[1]};
-        put<NT>((u32x2*)(q + at), t);
+        const u32x2_any t = {w[0], w[1]};
+        u32x2_any* o = (u32x2_any*)(q + at);
+        if (NT) __builtin_nontemporal_store(t, o); else *o = t;
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -148,16 +149,16 @@ __global__ __launch_bounds__(256) void act8_fwd_kernel(const T* __restrict__ u, 
 
 template <typename T, bool NT>
 __global__ __launch_bounds__(256) void act8_bwd_kernel(const unsigned char* __restrict__ q, const float* __restrict__ scale, const T* __restrict__ da, T* __restrict__ du, T* __restrict__ a,
-                                                       int64_t rows, int per_row, int cols, int log_p, int parts, int act, int aligned) {
+                                                       int64_t rows, int per_row, int cols, int log_p, int parts, int act) {
     bool on;
     const Act8Place place = act8_place(per_row, cols, log_p, parts, rows, &on);
     if (!on) return;
     const int64_t g = place.group, at = place.at;
     const int n = place.left;
-    const bool whole = aligned && n >= 8;
+    const bool whole = n >= 8;
     unsigned w[2] = {0u, 0u};
     if (whole) {
-        const u32x2 t = NT ? __builtin_nontemporal_load((const u32x2*)(q + at)) : *(const u32x2*)(q + at);
+        const u32x2 t = NT ? __builtin_nontemporal_load((const u32x2_any*)(q + at)) : *(const u32x2_any*)(q + at);
         w[0] = t[0]; w[1] = t[1];
     } else {
 #pragma unroll
@@ -210,9 +211,8 @@ extern "C" int hh_act8_fwd(const void* u, int u_dtype, void* a, void* q, float* 
     HH_REQUIRE(rows < (1ll << 40) && blocks <= 0x7fffffff, HH_ERR_SHAPE, "hh_act8_fwd: too many rows");
     if (rows == 0) return HH_OK;
     HH_REQUIRE(u != nullptr && q != nullptr && scale != nullptr, HH_ERR_ALIGN, "hh_act8_fwd: NULL pointer");
-    const int al = cols % 8 == 0 && HH_ALIGNED16(u) && HH_ALIGNED16(a) && (((uintptr_t)q) & 7) == 0;
     const bool f32 = u_dtype == HH_F32, nt = rows * cols * (1 + (a ? (f32 ? 4 : 2) : 0)) > HH_STREAM_BYTES;
-#define AF(T, N) hipLaunchKernelGGL((act8_fwd_kernel<T, N>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T*)u, (T*)a, (unsigned char*)q, scale, rows, per_row, cols, g.log_p, g.parts, act, al)
+#define AF(T, N) hipLaunchKernelGGL((act8_fwd_kernel<T, N>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T*)u, (T*)a, (unsigned char*)q, scale, rows, per_row, cols, g.log_p, g.parts, act)
     if (f32) { if (nt) AF(float, true); else AF(float, false); }
     else { if (nt) AF(bf16_t, true); else AF(bf16_t, false); }
 #undef AF
@@ -229,9 +229,8 @@ extern "C" int hh_act8_bwd(const void* q, const float* scale, const void* da, vo
     HH_REQUIRE(rows < (1ll << 40) && blocks <= 0x7fffffff, HH_ERR_SHAPE, "hh_act8_bwd: too many rows");
     if (rows == 0) return HH_OK;
     HH_REQUIRE(q != nullptr && scale != nullptr && da != nullptr && du != nullptr, HH_ERR_ALIGN, "hh_act8_bwd: NULL pointer");
-    const int al = cols % 8 == 0 && HH_ALIGNED16(da) && HH_ALIGNED16(du) && HH_ALIGNED16(a) && (((uintptr_t)q) & 7) == 0;
     const bool f32 = dtype == HH_F32, nt = rows * cols * (f32 ? 4 : 2) * (a ? 2 : 1) > HH_STREAM_BYTES;
-#define AB(T, N) hipLaunchKernelGGL((act8_bwd_kernel<T, N>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const unsigned char*)q, scale, (const T*)da, (T*)du, (T*)a, rows, per_row, cols, g.log_p, g.parts, act, al)
+#define AB(T, N) hipLaunchKernelGGL((act8_bwd_kernel<T, N>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const unsigned char*)q, scale, (const T*)da, (T*)du, (T*)a, rows, per_row, cols, g.log_p, g.parts, act)
     if (f32) { if (nt) AB(float, true); else AB(float, false); }
     else { if (nt) AB(bf16_t, true); else AB(bf16_t, false); }
 #undef AB

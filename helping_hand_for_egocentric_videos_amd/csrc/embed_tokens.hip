@@ -13,7 +13,7 @@ typedef unsigned int u32;
 // ---- forward ---------------------------------------------------------------------------------------------------------------------------
 template <int E> struct fvec { float v[E]; };
 
-// E consecutive elements as fp32; `whole`: the address is aligned for one wide access and all E exist, else `n` of them one by one
+// E consecutive elements as fp32, in wide accesses where all E exist (`whole`), else `n` of them one by one
 template <int E, typename T, bool NT = false>
 __device__ __forceinline__ fvec<E> load_e(const T* p, bool whole, int n) {
     fvec<E> r;
@@ -21,16 +21,16 @@ __device__ __forceinline__ fvec<E> load_e(const T* p, bool whole, int n) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < E; i += 4) {
-                const f32x4 t = NT ? __builtin_nontemporal_load((const f32x4*)(p + i)) : *(const f32x4*)(p + i);
+                const f32x4 t = NT ? __builtin_nontemporal_load((const f32x4_any*)(p + i)) : *(const f32x4_any*)(p + i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) r.v[i + j] = t[j];
             }
         } else if constexpr (E == 8) {
-            const u32x4 t = NT ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
+            const u32x4 t = NT ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p;
 #pragma unroll
             for (int j = 0; j < 4; ++j) { r.v[2 * j] = bf16_lo_to_f32(t[j]); r.v[2 * j + 1] = bf16_hi_to_f32(t[j]); }
         } else {
-            const u32x2 t = *(const u32x2*)p;
+            const u32x2 t = *(const u32x2_any*)p;
 #pragma unroll
             for (int j = 0; j < 2; ++j) { r.v[2 * j] = bf16_lo_to_f32(t[j]); r.v[2 * j + 1] = bf16_hi_to_f32(t[j]); }
         }
@@ -45,13 +45,13 @@ __device__ __forceinline__ void store_e(T* p, const fvec<E>& r, bool whole, int 
     if (whole) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < E; i += 4) { f32x4 t = {r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]}; if (NT) __builtin_nontemporal_store(t, (f32x4*)(p + i)); else *(f32x4*)(p + i) = t; }
+            for (int i = 0; i < E; i += 4) { const f32x4_any t = {r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]}; if (NT) __builtin_nontemporal_store(t, (f32x4_any*)(p + i)); else *(f32x4_any*)(p + i) = t; }
         } else if constexpr (E == 8) {
             u32x4 t = {pack_bf16(r.v[0], r.v[1]), pack_bf16(r.v[2], r.v[3]), pack_bf16(r.v[4], r.v[5]), pack_bf16(r.v[6], r.v[7])};
-            *(u32x4*)p = t;
+            *(u32x4_any*)p = t;
         } else {
             u32x2 t = {pack_bf16(r.v[0], r.v[1]), pack_bf16(r.v[2], r.v[3])};
-            *(u32x2*)p = t;
+            *(u32x2_any*)p = t;
         }
     } else {
 #pragma unroll
@@ -60,6 +60,11 @@ __device__ __forceinline__ void store_e(T* p, const fvec<E>& r, bool whole, int 
     }
 }
 
+// where a lane's piece c .. c + E - 1 of a row begins: the piece in which the row ends is moved back to be whole, and what it shares with the piece before is
+// worked out twice, to the same values
+template <int E>
+__device__ __forceinline__ int piece_at(int c, int dim) { return c + E > dim && dim >= E ? dim - E : c; }
+
 __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t i) {
     return wide ? ((const int64_t*)ids)[i] : (int64_t)((const int*)ids)[i];
 }
@@ -67,7 +72,7 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t i)
 // lpr lanes (a power of two) share a row, each takes every lpr-th piece of E elements; 64 / lpr rows to a wave
 template <typename TW, typename TO, int E, bool NT>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__ ids, int wide, const TW* __restrict__ w, const float* __restrict__ pos, TO* __restrict__ out,
-                                                        int64_t n, int length, int64_t rows, int dim, float scale, int lpr_log2, int aligned) {
+                                                        int64_t n, int length, int64_t rows, int dim, float scale, int lpr_log2) {
     const int lane = threadIdx.x & 63;
     const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int64_t r = (wave << (6 - lpr_log2)) + (lane >> lpr_log2);
@@ -77,8 +82,9 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__
     const TW* wr = w + (known ? id : 0) * dim;
     const float* pr = pos ? pos + (r % length) * (int64_t)dim : nullptr;
     TO* o = out + r * dim;
-    for (int c = (lane & ((1 << lpr_log2) - 1)) * E; c < dim; c += E << lpr_log2) {
-        const bool whole = aligned && c + E <= dim;
+    const bool whole = dim >= E;
+    for (int first = (lane & ((1 << lpr_log2) - 1)) * E; first < dim; first += E << lpr_log2) {
+        const int c = piece_at<E>(first, dim);
         fvec<E> v;
         if (known) {
             v = load_e<E, TW>(wr + c, whole, dim - c);
@@ -342,7 +348,7 @@ struct RunList {
     float* part;                                     // [chunks][2][dim]: a chunk's first run where it began earlier, its last where it goes on
     unsigned char* flags;                            // [chunks]: what crosses the border behind the chunk
     int64_t rows;
-    int accumulate, aligned;
+    int accumulate;
     float scale;
 };
 struct RunParams {
@@ -353,12 +359,19 @@ struct RunParams {
 __device__ __forceinline__ u32 run_key(const RunParams& p, const RunList& l, int j) { return l.keys ? l.keys[j] : (u32)(j / p.seqs); }
 __device__ __forceinline__ int64_t run_from(const RunParams& p, const RunList& l, int j) { return l.keys ? (int64_t)l.from[j] : (int64_t)(j % p.seqs) * p.length + j / p.seqs; }
 
+// (own: the first channel of the piece that is not the piece before's too; only those can be added to what is there)
 template <int E>
-__device__ __forceinline__ void put_row(const RunParams& p, const RunList& l, u32 key, int c, bool whole, fvec<E> v) {
+__device__ __forceinline__ void put_row(const RunParams& p, const RunList& l, u32 key, int c, int own, bool whole, fvec<E> v) {
     float* o = l.out + (int64_t)key * p.dim + c;
 #pragma unroll
     for (int i = 0; i < E; ++i) v.v[i] *= l.scale;
     if (l.accumulate) {
+        if (own > c) {
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (c + i >= own) o[i] += v.v[i];
+            return;
+        }
         const fvec<E> t = load_e<E, float>(o, whole, p.dim - c);
 #pragma unroll
         for (int i = 0; i < E; ++i) v.v[i] += t.v[i];
@@ -369,7 +382,7 @@ __device__ __forceinline__ void put_row(const RunParams& p, const RunList& l, u3
 // 16 bytes of dy as they lie in memory (E = 4 of fp32, 8 of bf16): turned into fp32 when they are added, so that eight rows on their way take 32 registers
 template <typename T, bool NT>
 __device__ __forceinline__ u32x4 raw16(const T* p, bool whole, int n) {
-    if (whole) return NT ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
+    if (whole) return NT ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p;
     u32x4 r = {0u, 0u, 0u, 0u};
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -397,9 +410,9 @@ __device__ __forceinline__ void add_raw16(fvec<E>& acc, const u32x4& r) {
 template <typename T, int E, bool NT>
 __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
     const RunList& l = p.list[blockIdx.z];
-    const int c = (blockIdx.y * 256 + threadIdx.x) * E;
-    if (c >= p.dim) return;
-    const bool whole = l.aligned && c + E <= p.dim;
+    const int own = (blockIdx.y * 256 + threadIdx.x) * E, c = piece_at<E>(own, p.dim);
+    if (own >= p.dim) return;
+    const bool whole = p.dim >= E;
     const int j0 = blockIdx.x * p.chunk, j1 = j0 + p.chunk < p.n ? j0 + p.chunk : p.n;
     u32 key = run_key(p, l, j0);
     bool head = j0 > 0 && run_key(p, l, j0 - 1) == key;          // this run began in an earlier chunk
@@ -407,7 +420,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
 #pragma unroll
     for (int i = 0; i < E; ++i) acc.v[i] = 0.f;
     float* part = l.part + (int64_t)blockIdx.x * 2 * p.dim + c;
-    if (c == 0) {
+    if (own == 0) {
         const u32 at_end = run_key(p, l, j1 - 1);
         const bool cross = j1 < p.n && (int64_t)at_end < l.rows && run_key(p, l, j1) == at_end;
         l.flags[blockIdx.x] = (unsigned char)(!cross ? RUN_ENDS : head && key == at_end ? RUN_COVERS : RUN_STARTS);
@@ -428,7 +441,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
                 if (next[i] != key || j + i + 1 == j1) {
                     if (head) store_e<E, float>(part, acc, whole, p.dim - c);
                     else if (next[i] == key) store_e<E, float>(part + p.dim, acc, whole, p.dim - c);
-                    else put_row<E>(p, l, key, c, whole, acc);
+                    else put_row<E>(p, l, key, c, own, whole, acc);
 #pragma unroll
                     for (int k = 0; k < E; ++k) acc.v[k] = 0.f;
                     head = false;
@@ -448,8 +461,8 @@ __global__ __launch_bounds__(1024) void run_join_kernel(RunParams p) {
     __shared__ float buf[16][256];
     const RunList& l = p.list[blockIdx.z];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int c = (blockIdx.y * 64 + lane) * 4;
-    const bool mine = c < p.dim, whole = l.aligned && c + 4 <= p.dim;
+    const int own = (blockIdx.y * 64 + lane) * 4, c = piece_at<4>(own, p.dim);
+    const bool mine = own < p.dim, whole = p.dim >= 4;
     const int b = blockIdx.x * 16 + wave;
     int heads = 0;                                               // chunks b + 1 .. b + heads belong to the run that starts in chunk b
     if (b < p.chunks && l.flags[b] == RUN_STARTS) {
@@ -489,7 +502,7 @@ __global__ __launch_bounds__(1024) void run_join_kernel(RunParams p) {
             if (u < heads)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc.v[e] += v[u].v[e];
-        put_row<4>(p, l, run_key(p, l, (b + 1) * p.chunk), c, whole, acc);
+        put_row<4>(p, l, run_key(p, l, (b + 1) * p.chunk), c, own, whole, acc);
     }
     __syncthreads();
     for (int i = 0; i < 16; ++i) {
@@ -518,7 +531,7 @@ __global__ __launch_bounds__(1024) void run_join_kernel(RunParams p) {
             for (int q = 1; q < 16; ++q)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc.v[e] += buf[q][lane * 4 + e];
-            put_row<4>(p, l, run_key(p, l, (from + 1) * p.chunk), c, whole, acc);
+            put_row<4>(p, l, run_key(p, l, (from + 1) * p.chunk), c, own, whole, acc);
         }
         __syncthreads();
     }
@@ -552,10 +565,8 @@ extern "C" int hh_embed_tokens_fwd(const void* ids, int id_bytes, const void* we
     if (n == 0) return HH_OK;
     HH_REQUIRE(ids != nullptr && weight != nullptr && out != nullptr, HH_ERR_ALIGN, "hh_embed_tokens_fwd: NULL pointer");
     hipStream_t s = (hipStream_t)stream;
-    const bool al = HH_ALIGNED16(weight) && HH_ALIGNED16(out) && HH_ALIGNED16(pos);
 #define EFL(TW, TO, E, NT)                                                                                                                       \
-    hipLaunchKernelGGL((embed_fwd_kernel<TW, TO, E, NT>), dim3((unsigned)blocks), dim3(256), 0, s, ids, id_bytes == 8, (const TW*)weight, pos, (TO*)out, n, length, rows, dim, scale, l, \
-                       (int)(al && dim % E == 0))
+    hipLaunchKernelGGL((embed_fwd_kernel<TW, TO, E, NT>), dim3((unsigned)blocks), dim3(256), 0, s, ids, id_bytes == 8, (const TW*)weight, pos, (TO*)out, n, length, rows, dim, scale, l)
 #define EF(TW, TO, E)                                                                                                                            \
     do {                                                                                                                                         \
         int l = 0;                                                                                                                               \
@@ -642,8 +653,8 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     }
     RunParams p;
     p.dy = dy; p.n = (int)n; p.chunk = run_chunk(n, run_waves(dim, e)); p.chunks = (int)chunks; p.dim = dim; p.length = length; p.seqs = (int)seqs;
-    p.list[0] = RunList{keys[sorted], from[sorted], dweight, (float*)part, flags, rows, accumulate != 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dweight), scale};
-    p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), flags + flag_bytes, length, 0, dim % e == 0 && HH_ALIGNED16(dy) && HH_ALIGNED16(dpos), 1.f};
+    p.list[0] = RunList{keys[sorted], from[sorted], dweight, (float*)part, flags, rows, accumulate != 0, scale};
+    p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), flags + flag_bytes, length, 0, 1.f};
     const int need = (dim + e - 1) / e;
     const int threads = need >= 256 ? 256 : (need + 63) / 64 * 64;
     const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), dpos ? 2u : 1u);

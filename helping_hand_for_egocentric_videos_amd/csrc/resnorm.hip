@@ -41,7 +41,9 @@ template <int DT, typename T>
 __device__ __forceinline__ T* rn_row(T* base, int dt, int64_t off) { return base + off * (rn_f32<DT>(dt) ? 4 : 2); }
 
 // four channels as they lie in memory: 4 dwords of fp32, 2 of bf16; turned into fp32 only when all loads of a step have been issued (a conversion behind
-// each load would wait for it).  Channels behind the row's end are zero (VEC: the caller asks with c < cols).
+// each load would wait for it).  Rows of any width and alignment (not VEC): the four in which the row ends are read whole, from up to three channels before, and
+// shifted into place by rn_cvt; only a row of fewer than four is read one by one.
+__device__ __forceinline__ int rn_behind(int c, int cols) { return c + 4 > cols && cols >= 4 ? c + 4 - cols : 0; }
 template <bool VEC, int DT, bool NT = false>
 __device__ __forceinline__ u32x4 rn_raw(const char* row, int dt, int c, int cols) {
     u32x4 r = {0u, 0u, 0u, 0u};
@@ -51,6 +53,16 @@ __device__ __forceinline__ u32x4 rn_raw(const char* row, int dt, int c, int cols
             r = NT ? __builtin_nontemporal_load(at) : *at;
         } else {
             const u32x2* at = (const u32x2*)(row + (unsigned)(c * 2));
+            const u32x2 t = NT ? __builtin_nontemporal_load(at) : *at;
+            r[0] = t[0]; r[1] = t[1];
+        }
+    } else if (cols >= 4) {
+        c -= rn_behind(c, cols);
+        if (rn_f32<DT>(dt)) {
+            const u32x4_any* at = (const u32x4_any*)(row + (unsigned)(c * 4));
+            r = NT ? __builtin_nontemporal_load(at) : *at;
+        } else {
+            const u32x2_any* at = (const u32x2_any*)(row + (unsigned)(c * 2));
             const u32x2 t = NT ? __builtin_nontemporal_load(at) : *at;
             r[0] = t[0]; r[1] = t[1];
         }
@@ -64,8 +76,8 @@ __device__ __forceinline__ u32x4 rn_raw(const char* row, int dt, int c, int cols
     }
     return r;
 }
-template <int DT>
-__device__ __forceinline__ Q4 rn_cvt(const u32x4& r, int dt) {
+template <bool VEC, int DT>
+__device__ __forceinline__ Q4 rn_cvt(const u32x4& r, int dt, int behind) {
     Q4 q;
     if (rn_f32<DT>(dt)) {
 #pragma unroll
@@ -74,12 +86,16 @@ __device__ __forceinline__ Q4 rn_cvt(const u32x4& r, int dt) {
         q.v[0] = bf16_lo_to_f32(r[0]); q.v[1] = bf16_hi_to_f32(r[0]);
         q.v[2] = bf16_lo_to_f32(r[1]); q.v[3] = bf16_hi_to_f32(r[1]);
     }
+    if (!VEC && behind) {
+        if (behind & 1) { q.v[0] = q.v[1]; q.v[1] = q.v[2]; q.v[2] = q.v[3]; q.v[3] = 0.f; }
+        if (behind & 2) { q.v[0] = q.v[2]; q.v[1] = q.v[3]; q.v[2] = q.v[3] = 0.f; }
+    }
     return q;
 }
 template <bool VEC>
 __device__ __forceinline__ Q4 rn_param(const float* base, int64_t off, int c, int cols) {
-    if (VEC && c >= cols) return Q4{{0.f, 0.f, 0.f, 0.f}};
-    return rn_cvt<HH_F32>(rn_raw<VEC, HH_F32>((const char*)(base + off), HH_F32, c, cols), HH_F32);
+    if (c >= cols) return Q4{{0.f, 0.f, 0.f, 0.f}};
+    return rn_cvt<VEC, HH_F32>(rn_raw<VEC, HH_F32>((const char*)(base + off), HH_F32, c, cols), HH_F32, rn_behind(c, cols));
 }
 
 template <bool VEC, bool NT, int DT>
@@ -94,9 +110,19 @@ __device__ __forceinline__ void rn_store(const Q4& q, char* row, int dt, int c, 
             u32x2* o = (u32x2*)(row + (unsigned)(c * 2));
             if (NT) __builtin_nontemporal_store(t, o); else *o = t;
         }
+    } else if (c + 4 <= cols) {
+        if (rn_f32<DT>(dt)) {
+            const f32x4_any t = {q.v[0], q.v[1], q.v[2], q.v[3]};
+            f32x4_any* o = (f32x4_any*)(row + (unsigned)(c * 4));
+            if (NT) __builtin_nontemporal_store(t, o); else *o = t;
+        } else {
+            const u32x2_any t = {pack_bf16(q.v[0], q.v[1]), pack_bf16(q.v[2], q.v[3])};
+            u32x2_any* o = (u32x2_any*)(row + (unsigned)(c * 2));
+            if (NT) __builtin_nontemporal_store(t, o); else *o = t;
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 3; ++j)
             if (c + j < cols) {
                 if (rn_f32<DT>(dt)) ((float*)row)[c + j] = q.v[j];
                 else ((bf16_t*)row)[c + j] = (bf16_t)q.v[j];
@@ -105,7 +131,7 @@ __device__ __forceinline__ void rn_store(const Q4& q, char* row, int dt, int c, 
 }
 template <bool VEC>
 __device__ __forceinline__ void rn_put(const Q4& q, float* row, int c, int cols) {
-    if (!VEC || c < cols) rn_store<VEC, false, HH_F32>(q, (char*)row, HH_F32, c, cols);
+    if (c < cols) rn_store<VEC, false, HH_F32>(q, (char*)row, HH_F32, c, cols);
 }
 
 __device__ __forceinline__ float add_swapped32(float a, float b) {     // lanes 0..31: a over both halves, lanes 32..63: b
@@ -221,8 +247,8 @@ __device__ __forceinline__ Q4 rn_gate(const RnParams& p, int64_t group, int c) {
 template <int R, bool VEC, bool NT, int XT, int YT, int HT>
 __global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
     __shared__ RnRed red;
-    const int waves = blockDim.x >> 6, c = threadIdx.x * 4;
-    const bool on = !VEC || c < p.cols;
+    const int waves = blockDim.x >> 6, c = threadIdx.x * 4, behind = rn_behind(c, p.cols);
+    const bool on = c < p.cols;
     const float inv = 1.f / (float)p.cols;
     const Q4 zero = {{0.f, 0.f, 0.f, 0.f}};
     const int64_t r0 = (int64_t)blockIdx.x * R;
@@ -256,7 +282,7 @@ __global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
     Q4 x[R], y[R];
     float mean[R], rstd[R], eps[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) { x[i] = rn_cvt<XT>(rx[i], p.x_dt); y[i] = rn_cvt<YT>(ry[i], p.y_dt); }
+    for (int i = 0; i < R; ++i) { x[i] = rn_cvt<VEC, XT>(rx[i], p.x_dt, behind); y[i] = rn_cvt<VEC, YT>(ry[i], p.y_dt, behind); }
     if (p.g1) {
 #pragma unroll
         for (int i = 0; i < R; ++i) eps[i] = p.eps1;
@@ -289,8 +315,8 @@ __global__ __launch_bounds__(1024) void resnorm_fwd_kernel(RnParams p) {
 template <int R, bool POST, bool PRE, bool VEC, bool NT, int XT, int YT, int HT>
 __global__ __launch_bounds__(R == 4 ? 256 : 1024) void resnorm_bwd_kernel(RnParams p) {
     __shared__ RnRed red;
-    const int waves = blockDim.x >> 6, c = threadIdx.x * 4;
-    const bool on = !VEC || c < p.cols;
+    const int waves = blockDim.x >> 6, c = threadIdx.x * 4, behind = rn_behind(c, p.cols);
+    const bool on = c < p.cols;
     const float inv = 1.f / (float)p.cols;
     const Q4 zero = {{0.f, 0.f, 0.f, 0.f}};
     const u32x4 none = {0u, 0u, 0u, 0u};
@@ -334,7 +360,7 @@ __global__ __launch_bounds__(R == 4 ? 256 : 1024) void resnorm_bwd_kernel(RnPara
                     float eps[2 * R];
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
-                        xy[i] = rn_cvt<XT>(rx[i], p.x_dt); xy[R + i] = rn_cvt<YT>(ry[i], p.y_dt);
+                        xy[i] = rn_cvt<VEC, XT>(rx[i], p.x_dt, behind); xy[R + i] = rn_cvt<VEC, YT>(ry[i], p.y_dt, behind);
                         eps[i] = p.eps2; eps[R + i] = p.eps1;
                     }
                     rn_stats<VEC, true, 2 * R>(xy, c, p.cols, inv, p.rms, eps, red, turn, waves, mean, rstd);
@@ -343,7 +369,7 @@ __global__ __launch_bounds__(R == 4 ? 256 : 1024) void resnorm_bwd_kernel(RnPara
                 } else {
                     float eps[R], m[R], q[R];
 #pragma unroll
-                    for (int i = 0; i < R; ++i) { x[i] = rn_cvt<XT>(rx[i], p.x_dt); y[i] = rn_cvt<YT>(ry[i], p.y_dt); eps[i] = p.eps2; }
+                    for (int i = 0; i < R; ++i) { x[i] = rn_cvt<VEC, XT>(rx[i], p.x_dt, behind); y[i] = rn_cvt<VEC, YT>(ry[i], p.y_dt, behind); eps[i] = p.eps2; }
                     rn_stats<VEC, true, R>(x, c, p.cols, inv, p.rms, eps, red, turn, waves, m, q);
 #pragma unroll
                     for (int i = 0; i < R; ++i) { mean[i] = m[i]; rstd[i] = q[i]; }
@@ -351,8 +377,8 @@ __global__ __launch_bounds__(R == 4 ? 256 : 1024) void resnorm_bwd_kernel(RnPara
                 Q4 k[R];
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
-                    k[i] = rn_cvt<HT>(rh[i], p.h_dt);
-                    d[i] = rn_cvt<XT>(rd[i], p.x_dt);
+                    k[i] = rn_cvt<VEC, HT>(rh[i], p.h_dt, behind);
+                    d[i] = rn_cvt<VEC, XT>(rd[i], p.x_dt, behind);
                     s[i] = s[R + i] = 0.f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -374,7 +400,7 @@ __global__ __launch_bounds__(R == 4 ? 256 : 1024) void resnorm_bwd_kernel(RnPara
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < R; ++i) { y[i] = rn_cvt<YT>(ry[i], p.y_dt); d[i] = rn_cvt<XT>(rd[i], p.x_dt); }
+                for (int i = 0; i < R; ++i) { y[i] = rn_cvt<VEC, YT>(ry[i], p.y_dt, behind); d[i] = rn_cvt<VEC, XT>(rd[i], p.x_dt, behind); }
                 if constexpr (POST) {
                     float eps[R], m[R], q[R];
 #pragma unroll
@@ -533,17 +559,17 @@ __global__ __launch_bounds__(1024) void resnorm_reduce_kernel(RnReduce p) {
 }
 
 // ---- entry points ------------------------------------------------------------------------------------------------------------------------
-#ifndef RN_FWD_MANY
+// rows from which the forward pass takes four at a time (4097 x 1024: 10.8 us, one at a time 11.7; 32 776 x 1024: 66 and 75) and below which it takes one, where a
+// call is all latency (416 x 512: 3.6 us, four at a time 4.3)
 #define RN_FWD_MANY 4096
-#endif
 static int rn_waves(int cols) { return (cols + 255) / 256; }
 
 struct RnPlan { int64_t chunks, units, per_block, blocks; };
-// about 4096 waves (four to a SIMD) in workgroups that take whole units of one gate group's rows; a unit leaves four partial rows, so it has 16 rows if there are
-// (12 320 x 768: 8 rows 38.3 us, 16 rows 34.5, 32 rows 38.8)
-static RnPlan rn_plan(int64_t rows, int cols, int64_t groups) {
+// Workgroups that are on the chip at once (two rows at a time: 16 waves to a CU, four rows: 8), which take whole units of one gate group's rows; a unit leaves four
+// partial rows, so it has 16 rows if there are (12 320 x 768: 8 rows 38.3 us, 16 rows 34.5, 32 rows 38.8)
+static RnPlan rn_plan(int64_t rows, int cols, int64_t groups, int at_once) {
     RnPlan q;
-    const int64_t blocks = 4096 / rn_waves(cols);
+    const int64_t blocks = 256 * ((at_once == 4 ? 8 : 16) / rn_waves(cols));
     const int64_t most = (rows / groups + 15) / 16;
     q.chunks = (blocks + groups - 1) / groups;
     if (q.chunks > most) q.chunks = most;
@@ -598,8 +624,7 @@ extern "C" int hh_residual_norm_fwd(const hh_residual_norm* d, hh_stream_t strea
 #define RF(R, V, N, X, Y, H) hipLaunchKernelGGL((resnorm_fwd_kernel<R, V, N, X, Y, H>), dim3((unsigned)((d->rows + R - 1) / R)), dim3(threads), 0, s, p)
 #define RFN(X, Y, H) do { if (d->rows < RN_FWD_MANY) RF(1, true, false, X, Y, H); else if (nt) RF(4, true, true, X, Y, H); else RF(4, true, false, X, Y, H); } while (0)
 #define RFH(X, Y) do { if (p.h_dt == HH_F32) RFN(X, Y, HH_F32); else RFN(X, Y, HH_BF16); } while (0)
-    // four rows to a workgroup where that still leaves work for every CU, one where a short call is all latency
-    if (!vec) { if (d->rows >= RN_FWD_MANY) RF(4, false, false, RN_ANY, RN_ANY, RN_ANY); else RF(1, false, false, RN_ANY, RN_ANY, RN_ANY); }
+    if (!vec) { if (d->rows < RN_FWD_MANY) RF(1, false, false, RN_ANY, RN_ANY, RN_ANY); else if (nt) RF(4, false, true, RN_ANY, RN_ANY, RN_ANY); else RF(4, false, false, RN_ANY, RN_ANY, RN_ANY); }
     else if (p.x_dt == HH_F32) { if (p.y_dt == HH_F32) RFH(HH_F32, HH_F32); else RFH(HH_F32, HH_BF16); }
     else { if (p.y_dt == HH_F32) RFH(HH_BF16, HH_F32); else RFH(HH_BF16, HH_BF16); }
 #undef RFH
@@ -611,8 +636,9 @@ extern "C" int hh_residual_norm_fwd(const hh_residual_norm* d, hh_stream_t strea
 extern "C" int64_t hh_workspace_bytes_residual_norm_bwd(int64_t rows, int cols, int64_t groups) {
     if (rows < 0 || cols <= 0 || cols > 4096 || groups < 1 || groups > 65000 || rows % groups) return -1;
     if (rows == 0) return 0;
-    const RnPlan q = rn_plan(rows, cols, groups);
-    return (4 * q.blocks + q.units) * cols * 4;
+    const RnPlan q = rn_plan(rows, cols, groups, 2), q4 = cols <= 1024 ? rn_plan(rows, cols, groups, 4) : q;
+    const int64_t lines = 4 * q.blocks + q.units, lines4 = 4 * q4.blocks + q4.units;
+    return (lines > lines4 ? lines : lines4) * cols * 4;
 }
 
 extern "C" int hh_residual_norm_bwd(const hh_residual_norm* d, hh_stream_t stream) {
@@ -626,18 +652,21 @@ extern "C" int hh_residual_norm_bwd(const hh_residual_norm* d, hh_stream_t strea
                HH_ERR_ALIGN, "hh_residual_norm_bwd: a gradient's pointer comes with its parameter's");
     RnPlan q = {0, 0, 0, 0};                                     // (no rows: every sum is over nothing, and the second launch writes zeros)
     if (d->rows > 0) {
-        q = rn_plan(d->rows, p.cols, d->groups);
+        // two rows at a time, and four for the largest calls of up to 1024 channels: their requests are larger, but their workgroups fill the chip only where they have
+        // one, two or four waves, and a few hundred MB of gradients have to be written before that pays (1024 channels: 35 807 rows 138 us, four 141; 65 104 rows 238
+        // and 242; 130 208 rows 497 and 473.  768 channels: 173 611 rows 491 and 533)
+        const int64_t bytes = d->rows * p.cols * (rn_size(p.x_dt) + rn_size(p.y_dt));
+        const bool nt = bytes > HH_STREAM_BYTES;
+        const int waves = rn_waves(p.cols), threads = waves * 64, at_once = vec && bytes > (600ll << 20) && (waves == 1 || waves == 2 || waves == 4) ? 4 : 2;
+        q = rn_plan(d->rows, p.cols, d->groups, at_once);
         HH_REQUIRE(d->workspace != nullptr && HH_ALIGNED16(d->workspace), HH_ERR_ALIGN, "hh_residual_norm_bwd: a 16-byte aligned workspace is needed");
         p.part = (float*)d->workspace;
         p.gate_part = p.part + 4 * q.blocks * p.cols;
         p.chunks = q.chunks; p.units = q.units; p.per_block = q.per_block;
-        const bool nt = d->rows * p.cols * (rn_size(p.x_dt) + rn_size(p.y_dt)) > HH_STREAM_BYTES;
-        const int threads = rn_waves(p.cols) * 64;
-// four rows at a time for large calls (131 104 x 1024: 500 -> 472 us with two -> four), two for the others (12 320 x 768: 34.5, four 39.4)
 #define RB(R, PO, PR, V, N, X, Y, H) hipLaunchKernelGGL((resnorm_bwd_kernel<R, PO, PR, V, N, X, Y, H>), dim3((unsigned)q.blocks), dim3(threads), 0, s, p)
-#define RBN(PO, PR, X, Y, H) do { if (!nt) RB(2, PO, PR, true, false, X, Y, H); else if (threads <= 256) RB(4, PO, PR, true, true, X, Y, H); else RB(2, PO, PR, true, true, X, Y, H); } while (0)
+#define RBN(PO, PR, X, Y, H) do { if (at_once == 4) RB(4, PO, PR, true, true, X, Y, H); else if (nt) RB(2, PO, PR, true, true, X, Y, H); else RB(2, PO, PR, true, false, X, Y, H); } while (0)
 #define RBY(PO, PR, X, H) do { if (p.y_dt == HH_F32) RBN(PO, PR, X, HH_F32, H); else RBN(PO, PR, X, HH_BF16, H); } while (0)
-#define RBX(PO, PR, H) do { if (!vec) RB(2, PO, PR, false, false, RN_ANY, RN_ANY, RN_ANY); else if (p.x_dt == HH_F32) RBY(PO, PR, HH_F32, H); else RBY(PO, PR, HH_BF16, H); } while (0)
+#define RBX(PO, PR, H) do { if (!vec) { if (nt) RB(2, PO, PR, false, true, RN_ANY, RN_ANY, RN_ANY); else RB(2, PO, PR, false, false, RN_ANY, RN_ANY, RN_ANY); } else if (p.x_dt == HH_F32) RBY(PO, PR, HH_F32, H); else RBY(PO, PR, HH_BF16, H); } while (0)
         if (p.g1 && p.g2) { if (p.h_dt == HH_F32) RBX(true, true, HH_F32); else RBX(true, true, HH_BF16); }
         else if (p.g2) { if (p.h_dt == HH_F32) RBX(false, true, HH_F32); else RBX(false, true, HH_BF16); }
         else if (p.g1) RBX(true, false, HH_F32);
