@@ -337,7 +337,7 @@ __global__ __launch_bounds__(256) void tn8_join_kernel(const float* __restrict__
     if (wave == 0 && c < m) cs[c] = (buf[0][lane] + buf[1][lane]) + (buf[2][lane] + buf[3][lane]);
 }
 
-struct Tn8Plan { int wt, tiles_m, tiles_n, splits; };
+struct Tn8Plan { int wt, tiles_m, tiles_n, splits, db_planes; };
 static Tn8Plan tn8_plan(int M, int N, int64_t K) {
     Tn8Plan q;
     const int64_t large = ((int64_t)(M + 255) / 256) * ((N + 255) / 256);
@@ -353,6 +353,9 @@ static Tn8Plan tn8_plan(int M, int N, int64_t K) {
     const int64_t most = (K + 511) / 512;
     if (s > most) s = most;
     q.splits = (int)(s < 1 ? 1 : s);
+    // one short slice: nothing is left to join, and the workgroups of the first column tile write db (500 x 1024 x 4096 18.4 -> 15.9 us); in a long one the others would
+    // wait for them (4096 x 4096 x 4096 134 us either way, 16 384 x 4096 x 4096 shared 442 us, 470 not)
+    q.db_planes = q.splits == 1 && K <= 4096 ? 1 : q.tiles_n;
     return q;
 }
 static bool tn8_shape_ok(int M, int N, int64_t K) {
@@ -362,8 +365,9 @@ static bool tn8_shape_ok(int M, int N, int64_t K) {
 extern "C" int64_t hh_workspace_bytes_gemm_tn_act8(int M, int N, int64_t K) {
     if (!tn8_shape_ok(M, N, K)) return -1;
     const Tn8Plan q = tn8_plan(M, N, K);
-    const int64_t db = (int64_t)q.splits * q.tiles_n * M;
-    return q.splits == 1 ? 0 : (((int64_t)q.splits * M * N + 3) / 4 * 4 + db) * 4;
+    const int64_t db = (int64_t)q.splits * q.db_planes * M;
+    if (q.splits == 1) return q.db_planes == 1 ? 0 : db * 4;
+    return (((int64_t)q.splits * M * N + 3) / 4 * 4 + db) * 4;
 }
 
 extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int64_t ldq, const float* scale, float* dw, float* db, int M, int N, int64_t K, void* workspace,
@@ -373,7 +377,8 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
     HH_REQUIRE(dw != nullptr && (K == 0 || (dy != nullptr && q != nullptr && scale != nullptr)), HH_ERR_ALIGN, "hh_gemm_tn_act8: NULL pointer");
     HH_REQUIRE((((uintptr_t)dw) & 15) == 0, HH_ERR_ALIGN, "hh_gemm_tn_act8: dw must be 16-byte aligned");
     const Tn8Plan pl = tn8_plan(M, N, K);
-    HH_REQUIRE(pl.splits == 1 || (workspace != nullptr && HH_ALIGNED16(workspace)), HH_ERR_ALIGN, "hh_gemm_tn_act8: a 16-byte aligned workspace is needed");
+    const bool joined = pl.splits > 1 || (db != nullptr && pl.db_planes > 1);
+    HH_REQUIRE(!joined || (workspace != nullptr && HH_ALIGNED16(workspace)), HH_ERR_ALIGN, "hh_gemm_tn_act8: a 16-byte aligned workspace is needed");
     hipStream_t s = (hipStream_t)stream;
     const int64_t n = (int64_t)M * N;
     Tn8Params p;
@@ -382,9 +387,8 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
     const int tokens = pl.wt == 8 ? 32 : 64;                                    // (a tile for each group)
     p.k_per_split = ((K + tokens - 1) / tokens + pl.splits - 1) / pl.splits * tokens;
     p.C = pl.splits == 1 ? dw : (float*)workspace;
-    // one slice: no sums are left to join, and the first column tile's workgroups write db
-    p.db_planes = pl.splits == 1 ? 1 : pl.tiles_n;
-    p.colsum = db == nullptr ? nullptr : pl.splits == 1 ? db : (float*)workspace + (n * pl.splits + 3) / 4 * 4;
+    p.db_planes = pl.db_planes;
+    p.colsum = db == nullptr ? nullptr : !joined ? db : (float*)workspace + (pl.splits == 1 ? 0 : (n * pl.splits + 3) / 4 * 4);
     const bool vec = M % 8 == 0 && ld_dy % 8 == 0 && HH_ALIGNED16(dy) && N % 16 == 0 && ldq % 16 == 0 && HH_ALIGNED16(q);
     const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n * pl.splits));
     const int lds = 128 * 1024;
@@ -406,10 +410,10 @@ extern "C" int hh_gemm_tn_act8(const void* dy, int64_t ld_dy, const void* q, int
         if (vec) hipLaunchKernelGGL((gemm_tn8_kernel<4, true>), grid, dim3(512), lds, s, p);
         else hipLaunchKernelGGL((gemm_tn8_kernel<4, false>), grid, dim3(512), lds, s, p);
     }
-    if (pl.splits > 1) {
-        int64_t blocks = (n / 4 + 255) / 256;
-        blocks = blocks < 1 ? 1 : blocks > 4096 ? 4096 : blocks;
-        hipLaunchKernelGGL(tn8_join_kernel, dim3((unsigned)(blocks + (db ? (M + 63) / 64 : 0))), dim3(256), 0, s, p.C, dw, n, pl.splits, p.colsum, db, M, pl.splits * pl.tiles_n, (int)blocks);
+    if (joined) {
+        int64_t blocks = pl.splits == 1 ? 0 : (n / 4 + 255) / 256;
+        if (pl.splits > 1) blocks = blocks < 1 ? 1 : blocks > 4096 ? 4096 : blocks;
+        hipLaunchKernelGGL(tn8_join_kernel, dim3((unsigned)(blocks + (db ? (M + 63) / 64 : 0))), dim3(256), 0, s, p.C, dw, n, pl.splits, p.colsum, db, M, pl.splits * pl.db_planes, (int)blocks);
     }
     return hh_check_launch("hh_gemm_tn_act8");
 }

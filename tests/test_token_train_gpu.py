@@ -523,7 +523,7 @@ def test_gemm_tn_act8(K, M, N):
     check_wgrad(rnd(K, M, seed=3, dtype=BF16), q, s, "act8 wgrad")
 
 
-@pytest.mark.parametrize("K,M,N", [(66000, 264, 272), (132001, 136, 400), (11003, 1030, 1037), (45000, 512, 520), (40961, 768, 1024)])
+@pytest.mark.parametrize("K,M,N", [(66000, 264, 272), (132001, 136, 400), (11003, 1030, 1037), (45000, 512, 520), (40961, 768, 1024), (4200, 4100, 4099)])
 def test_gemm_tn_act8_in_large_tiles(K, M, N):
     """Enough tokens and outputs for the 256 x 256 tiles: slices that end inside a tile, slices without a token, ragged outputs, unaligned rows."""
     assert -(-M // 256) * -(-N // 256) * -(-K // 1024) >= 256
