@@ -565,14 +565,17 @@ __global__ __launch_bounds__(1024) void resnorm_reduce_kernel(RnReduce p) {
 static int rn_waves(int cols) { return (cols + 255) / 256; }
 
 struct RnPlan { int64_t chunks, units, per_block, blocks; };
-// Workgroups that are on the chip at once (two rows at a time: 16 waves to a CU, four rows: 8), which take whole units of one gate group's rows; a unit leaves four
-// partial rows, so it has 16 rows if there are (12 320 x 768: 8 rows 38.3 us, 16 rows 34.5, 32 rows 38.8)
+// Workgroups that are on the chip at once (two rows at a time: 16 waves to a CU, four rows: 8), which take whole units of one gate group's rows.  A unit leaves four
+// partial rows, so it has 8 rows (12 320 x 768: 4 rows 35.1 us, 8 rows 35.2, 16 rows 37.0; the caller's other operands matter as much: 33.0 and 34.6 us for 8 and 16) --
+// fewer where that gives less than a workgroup to a CU, down to the two that are worked on at once (416 x 512: 8 rows 12.6 us, 2 rows 8.6; 1024 x 1024: 2 rows 19.0,
+// 4 rows 14.0, 8 rows 15.5).
 static RnPlan rn_plan(int64_t rows, int cols, int64_t groups, int at_once) {
     RnPlan q;
     const int64_t blocks = 256 * ((at_once == 4 ? 8 : 16) / rn_waves(cols));
-    const int64_t most = (rows / groups + 15) / 16;
+    const int64_t each = rows / groups, few = (255 + groups) / groups, pairs = (each + 1) / 2;
+    const int64_t most = (each + 7) / 8, least = pairs < few ? pairs : few;
     q.chunks = (blocks + groups - 1) / groups;
-    if (q.chunks > most) q.chunks = most;
+    if (q.chunks > most) q.chunks = most > least ? most : least;
     q.units = q.chunks * groups;
     q.per_block = (q.units + blocks - 1) / blocks;
     q.blocks = (q.units + q.per_block - 1) / q.per_block;
