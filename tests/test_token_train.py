@@ -16,8 +16,9 @@ def test_embed_tokens_refusals():
     assert f(idb=2) == -2 and f(wd=2) == -2 and f(od=7) == -2
     assert f(ids=None) == -5 and f(w=None) == -5 and f(o=None) == -5
     b = lambda ids=16, idb=8, dy=16, dd=0, dw=16, s=2, n=3, v=5, d=8, ws=16: L.hh_embed_tokens_bwd(ids, idb, dy, dd, dw, 1, None, s, n, v, d, 1.0, -1, ws, None)  # noqa: E731
-    assert b(d=0) == -1 and b(idb=1) == -2 and b(dd=3) == -2 and b(dw=None) == -5 and b(ids=None) == -5 and b(dy=None) == -5 and b(ws=None) == -5 and b(ws=8) == -5
+    assert b(d=0) == -1 and b(idb=1) == -2 and b(dd=3) == -2 and b(dw=None) == -5 and b(ids=None) == -5 and b(dy=None) == -5 and b(s=2000, ws=None) == -5 and b(s=2000, ws=8) == -5
     assert L.hh_workspace_bytes_embed_tokens_bwd(2, 0, 5, 8) == -1 and L.hh_workspace_bytes_embed_tokens_bwd(1 << 30, 1, 5, 8) == -1
+    assert L.hh_workspace_bytes_embed_tokens_bwd(2, 3, 5, 8) == 0         # few tokens: one launch
     assert L.hh_workspace_bytes_embed_tokens_bwd(160, 77, 49408, 768) >= 4 * 4 * 160 * 77
 
 

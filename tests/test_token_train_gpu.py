@@ -607,6 +607,26 @@ def test_embed_tokens_bwd_adds_once_where_pieces_share_channels(S, L, V, dim, dt
     assert torch.equal(dpos.double(), dy.double().sum(0))
 
 
+@pytest.mark.parametrize("S,L,V,dim", [(1, 512, 40, 768), (512, 1, 3, 2052), (16, 32, 49408, 12), (7, 73, 33000, 1), (3, 171, 700000, 3), (2, 9, 4, 70000), (1, 1, 40000000, 4)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_embed_tokens_bwd_of_few_tokens(S, L, V, dim, dt):
+    """Up to and just over 512 tokens, tables of many rows or wide ones: whole numbers, so that the stock sums are exact."""
+    ids = rints(-2, V + 2, (S, L), seed=4)
+    ids[0, 0] = V - 1
+    if S * L > 100:
+        ids[:, L // 2:] = min(5, V - 1)                             # one id has most of the tokens
+    dy = rints(-8, 9, (S, L, dim), seed=5).to(dt)
+    known = (ids >= 0) & (ids < V) & (ids != 1)
+    want = torch.zeros(V, dim, device=DEV)
+    want.index_add_(0, ids[known], dy[known].float() * 0.5)
+    for i in (ids, ids.int()):
+        dw, dpos = ops.embed_tokens_bwd(i, dy, V, scale=0.5, skip_id=1, pos_grad=True)
+        assert torch.equal(dw, want) and torch.equal(dpos, dy.float().sum(0))
+    out = torch.full((V, dim), 3.0, device=DEV)
+    ops.embed_tokens_bwd(ids, dy, V, scale=0.5, skip_id=1, out=out)
+    assert torch.equal(out, want + 3)
+
+
 # ---- streams, graphs, the operators together -------------------------------------------------------------------------------------------
 def one_pass(t):
     """Embedding, the end of a block, an activation and its checkpoint, and their backward passes: every output."""
