@@ -341,15 +341,16 @@ struct Tn8Plan { int wt, tiles_m, tiles_n, splits, db_planes; };
 static Tn8Plan tn8_plan(int M, int N, int64_t K) {
     Tn8Plan q;
     const int64_t large = ((int64_t)(M + 255) / 256) * ((N + 255) / 256);
-    // 256 x 256 tiles (one workgroup to a CU) where slices of 1024 tokens or more of them fill the chip: 32 776 x 512 x 2048 86 us (94 in tiles of 128), but
-    // 12 320 x 768 x 768, 117 of them, 44 us (36)
-    q.wt = large * ((K + 1023) / 1024) >= 256 && M > 128 && N > 128 ? 8 : 4;
+    // 256 x 256 tiles (one workgroup to a CU) where they nearly fill the chip by themselves (500 x 4096 x 3584: 29.5 us, tiles of 128 45.3; but 2048 x 2560 x 2560, 100
+    // of them, 54.2 and 47.3), or with slices of 1024 tokens (65 552 x 1024 x 4096: 465 and 604; 4097 x 2048 x 4096: 85 and 96; 8194 x 1536 x 2048, 432 of
+    // them, 69 and 79; 3000 x 2048 x 4096, 384, 71 either way; 4097 x 2048 x 2048, 320, 58 and 48; 12 320 x 768 x 768, 117, 42 and 32)
+    q.wt = (large >= 192 || large * ((K + 1023) / 1024) >= 400) && M > 128 && N > 128 ? 8 : 4;
     const int block = 32 * q.wt;
     q.tiles_m = (M + block - 1) / block;
     q.tiles_n = (N + block - 1) / block;
     const int64_t tiles = (int64_t)q.tiles_m * q.tiles_n;
     int64_t s = 256 / tiles;
-    // no slice below 512 tokens: every slice leaves a plane of dW to write and to add (2464 x 768 x 768: 10 slices 25.4 us, 5 slices 21.3)
+    // no slice below 512 tokens: every slice leaves a plane of dW to write and to add (2464 x 768 x 768: slices of 352 tokens 20.6 us, 512 19.4, 832 20.9)
     const int64_t most = (K + 511) / 512;
     if (s > most) s = most;
     q.splits = (int)(s < 1 ? 1 : s);

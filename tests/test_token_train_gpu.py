@@ -523,10 +523,11 @@ def test_gemm_tn_act8(K, M, N):
     check_wgrad(rnd(K, M, seed=3, dtype=BF16), q, s, "act8 wgrad")
 
 
-@pytest.mark.parametrize("K,M,N", [(66000, 264, 272), (132001, 136, 400), (11003, 1030, 1037), (45000, 512, 520), (40961, 768, 1024), (4200, 4100, 4099)])
+@pytest.mark.parametrize("K,M,N", [(102000, 264, 272), (205001, 136, 400), (16503, 1030, 1037), (68000, 512, 520), (40961, 768, 1024), (4200, 4100, 4099), (700, 3600, 3500)])
 def test_gemm_tn_act8_in_large_tiles(K, M, N):
     """Enough tokens and outputs for the 256 x 256 tiles: slices that end inside a tile, slices without a token, ragged outputs, unaligned rows."""
-    assert -(-M // 256) * -(-N // 256) * -(-K // 1024) >= 256
+    tiles = -(-M // 256) * -(-N // 256)
+    assert tiles >= 192 or tiles * -(-K // 1024) >= 400
     u = rnd(K, N, seed=1, dtype=BF16) * torch.exp(rnd(K, 1, seed=2)).to(BF16)
     _, q, s = ops.act8(u, want_out=False)
     check_wgrad(rnd(K, M, seed=3, dtype=BF16), q, s, "act8 wgrad, large tiles")
@@ -571,7 +572,7 @@ def placed(t, offset, junk):
     return raw[offset:offset + t.numel()].view(t.dtype).view(t.shape)
 
 
-@pytest.mark.parametrize("K,M,N", [(1, 3, 5), (33, 7, 21), (63, 129, 131), (101, 40, 1001), (1101, 77, 145), (11003, 1031, 1037)])
+@pytest.mark.parametrize("K,M,N", [(1, 3, 5), (33, 7, 21), (63, 129, 131), (101, 40, 1001), (1101, 77, 145), (16503, 1031, 1037)])
 @pytest.mark.parametrize("offset", [1, 2, 3])
 def test_gemm_tn_act8_any_address_and_nan_around_the_operands(K, M, N, offset):
     """Rows that begin at every byte, in buffers whose other bytes are NaN: nothing but the operands counts."""
