@@ -4,6 +4,7 @@ bits.  The reference trains none of its towers (run/train.py:89 freezes the back
 package would: `CLIP.encode_text`'s lookup (LaviLa.py:660-663), the tanh-gated residual of `SpaceTimeBlock` (LaviLa.py:305-390), `Mlp` (LaviLa.py:175-190)."""
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -19,6 +20,7 @@ class _EmbedTokens(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
         want_pos = ctx.pos_rows is not None and ctx.needs_input_grad[2]
@@ -51,6 +53,7 @@ class _ResidualNorm(torch.autograd.Function):
         return x_new, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dx_new, dh):
         x_new, y, gate, pg, pb, ng, nb = ctx.saved_tensors
         if dx_new is None and dh is None:
@@ -63,10 +66,19 @@ class _ResidualNorm(torch.autograd.Function):
         return (g.dx, g.dy, *(None if t is None else t.to(d) for t, d in zip(g[2:], ctx.dtypes)), None)
 
 
+def _norm_of(m, rms, which):
+    if m is None:
+        return None, None, 0.0
+    if isinstance(m, nn.RMSNorm) != rms:
+        raise TypeError("residual_norm: %s is a %s, with rms=%s" % (which, type(m).__name__, rms))
+    if m.weight is None:
+        raise ValueError("residual_norm: %s has no weight (elementwise_affine=False)" % which)
+    return m.weight, getattr(m, "bias", None), torch.finfo(torch.float32).eps if m.eps is None else m.eps
+
+
 def residual_norm(x, y, gate=None, post=None, pre=None, *, gate_tanh=False, res_scale=1.0, rms=False, out_dtype=torch.bfloat16):
-    """(x_new, h) of ops.residual_norm with every gradient; post / pre: nn.LayerNorm or nn.RMSNorm (with rms) modules, or None."""
-    norm = lambda m: (None, None, 0.0) if m is None else (m.weight, getattr(m, "bias", None), torch.finfo(torch.float32).eps if m.eps is None else m.eps)  # noqa: E731
-    (pg, pb, pe), (ng, nb, ne) = norm(post), norm(pre)
+    """(x_new, h) of ops.residual_norm with every gradient; post / pre: nn.LayerNorm (nn.RMSNorm with rms) modules with weights, or None."""
+    (pg, pb, pe), (ng, nb, ne) = _norm_of(post, rms, "post"), _norm_of(pre, rms, "pre")
     opts = {"gate_tanh": gate_tanh, "res_scale": float(res_scale), "rms": rms, "out_dtype": out_dtype, "post_eps": pe, "pre_eps": ne}
     return _ResidualNorm.apply(x, y, gate, pg, pb, ng, nb, opts)
 
@@ -85,6 +97,7 @@ class _MlpAct8(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         qx, sx, qu, su, w1, w2 = ctx.saved_tensors
         dyb = ops.to_bf16(dy.contiguous())
@@ -97,8 +110,8 @@ class _MlpAct8(torch.autograd.Function):
 
 
 def mlp_act8(x, fc1, fc2, act=ops.ACT_QUICKGELU):
-    """fc2(act(fc1(x))) for x fp32 / bf16 [rows, D] -> fp32 [rows, D_out] with bf16 products, keeping x and fc1's output as 8-bit checkpoints for the backward pass (2.06
-    bytes for an element pair instead of 6: fc2's input is taken again from the second).  fc1, fc2: nn.Linear whose widths are multiples of 128 (ops.gemm, ops.gemm_tn)."""
+    """fc2(act(fc1(x))) for x fp32 / bf16 [rows, D] -> fp32 [rows, D_out] with bf16 products, keeping x and fc1's output as 8-bit checkpoints for the backward pass (1.03
+    bytes for a value of either; fc2's input, which has the width of fc1's output, is taken again from that and not kept).  fc1, fc2: nn.Linear whose widths are multiples of 128 (ops.gemm, ops.gemm_tn)."""
     if x.dim() != 2:
         raise ValueError("mlp_act8: x must be [rows, D]")
     return _MlpAct8.apply(x, fc1.weight, fc1.bias, fc2.weight, fc2.bias, act)

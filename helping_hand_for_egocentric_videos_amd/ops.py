@@ -1075,7 +1075,7 @@ def embed_tokens_bwd(ids, dy, num_rows, scale=1.0, skip_id=None, pos_grad=False,
 
     ids int64 / int32 [..., L], dy fp32 / bf16 [..., L, D].  skip_id: an id without a gradient (nn.Embedding's padding_idx); ids outside [0, num_rows) have
     none either.  out: a fp32 [num_rows, D] buffer that the gradient is ACCUMULATED into (a parameter's slice of the gradient arena), a fresh one by
-    default.  Equal inputs give equal bits (the ids are sorted, no floating-point atomics)."""
+    default.  Equal inputs give equal bits (equal ids are added in an order that the ids alone decide, without floating-point atomics)."""
     stream = _here(ids, dy, out)
     length, seqs = _ids_of(ids, "embed_tokens_bwd")
     if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] == 0:
@@ -1224,7 +1224,8 @@ def act8_bwd(q, scale, da, act, want_out=False):
 def gemm_tn_act8(dy, q, scale, colsum=False, out=None):
     """Weight gradient from an 8-bit checkpoint: dy bf16 [K, M], (q, scale) = act8's of the layer's input [K, N] -> fp32 [M, N] = dy^T @ (q * scale), written
     into `out` when given; colsum=True also returns sum_k dy[k, :] (fp32 [M]: the bias gradient)   (include/hh.h: hh_gemm_tn_act8).  dy and q may be
-    row-strided views with unit inner stride; any K, M, N."""
+    row-strided views with unit inner stride (columns of a wider checkpoint from a multiple of 128, with their scales); any K <= 2^30, M, N; rows up to 2^24 elements
+    apart.  scale counts as a power of two: its exponent alone is used."""
     for t in (dy, q):
         if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
             raise ValueError("gemm_tn_act8: dy and q must be 2-D with unit inner stride and rows that do not overlap")

@@ -131,3 +131,17 @@ def test_pinned_matrix_products_keep_their_distances(tmp_path):
         for op, args in insts[at[-1] + 1:nops[0]]:              # (the zeros of a slice without tokens are written here)
             assert not any(regs(t) and t.startswith("a") for t in args[1:]), (op, args)
     assert found == 2
+
+
+def test_norm_modules_that_the_residual_does_not_take_are_refused():
+    """A norm without weights would be left out, one of the other kind computed as if it were not."""
+    from torch import nn
+    from helping_hand_for_egocentric_videos_amd.model import token_stream as ts
+    x = torch.zeros(2, 8)
+    for norm, rms in ((nn.LayerNorm(8, elementwise_affine=False), False), (nn.RMSNorm(8, elementwise_affine=False), True)):
+        with pytest.raises(ValueError, match="no weight"):
+            ts.residual_norm(x, x, post=norm, rms=rms)
+    for norm, rms in ((nn.RMSNorm(8), False), (nn.LayerNorm(8), True)):
+        for where in ("post", "pre"):
+            with pytest.raises(TypeError, match=where):
+                ts.residual_norm(x, x, rms=rms, **{where: norm})
