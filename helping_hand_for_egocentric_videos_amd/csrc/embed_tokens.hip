@@ -246,97 +246,63 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const u32* __r
     }
 }
 
-// A short list is sorted whole by one workgroup, four items to a thread: one launch instead of two for each digit.  Whole call, two launches a digit -> one: 32 ids of
-// 512 rows 28.0 -> 17.8 us, 2048 of 49 408 51.5 -> 43.0 us, 4096 of 49 408 53.1 -> 43.8 us (of 69 rows, one digit: 23.8 -> 24.4 us).
-#define SORT_SMALL 4096
-struct SmallSort { int n, passes; SortPass pass[4]; };
-__global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const void* __restrict__ ids, int wide, int64_t rows, int64_t skip, u32* __restrict__ keys_out, u32* __restrict__ from_out,
-                                                                  SmallSort q, ZeroPart z) {
-    if (blockIdx.x > 0) { zero_part(z, blockIdx.x - 1, gridDim.x - 1); return; }
-    __shared__ u32 base[256], wcount[16][256], part[4], list[SORT_SMALL];
-    __shared__ unsigned short list_from[SORT_SMALL];
+// A list that is not long is sorted by counting, in one launch: an entry's place is the number of entries with a smaller key, and of those before it with the same
+// key.  A workgroup places TOK entries, a lane each (and 64 / TOK lanes share an entry's comparisons); its 16 waves share the list, which goes through LDS in pieces of
+// 4096 keys.  n^2 comparisons, some three instructions for 64 of them.  Whole call with dpos, radix passes -> this:  of 800 rows of 512, 600 tokens 29.2 -> 19.2 us, 4000
+// 29.6 -> 19.8, 8000 36.8 -> 28.7, but 12 320 37.7 -> 44.5;  of 49 408 rows of 768 (the zeros are the most of it) 600 tokens 45.1 -> 37.4, 8000 52.4 -> 52.2.
+#define RANK_TOKENS 8192
+#define RANK_PIECE 4096
+template <int TOK>
+__global__ __launch_bounds__(SORT_THREADS) void rank_kernel(const void* __restrict__ ids, int wide, int64_t rows, int64_t skip, u32* __restrict__ keys_out, u32* __restrict__ from_out, int n,
+                                                            int rank_blocks, ZeroPart z) {
+    if ((int)blockIdx.x >= rank_blocks) { zero_part(z, blockIdx.x - rank_blocks, gridDim.x - rank_blocks); return; }
+    constexpr int J = 64 / TOK;
+    __shared__ u32x4 piece[RANK_PIECE / 4];
+    __shared__ u32 count[16 * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int rounds = (q.n + SORT_THREADS - 1) / SORT_THREADS;
-    u32 key[4], from[4], at[4];
+    const int i = blockIdx.x * TOK + lane % TOK, share = lane / TOK;
+    const int home = blockIdx.x * TOK & ~63;         // the 64 entries that the workgroup's are among
+    const auto key_of = [&](int j) -> u32 {          // (behind the list: larger than any key)
+        if (j >= n) return ~0u;
+        const int64_t id = load_id(ids, wide, j);
+        return id >= 0 && id < rows && id != skip ? (u32)id : (u32)rows;
+    };
+    const u32 key = key_of(i);
+    u32 place = 0;
+    for (int j0 = 0; j0 < n; j0 += RANK_PIECE) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int i = r * SORT_THREADS + tid;
-        key[r] = 0;
-        from[r] = (u32)i;
-        if (i < q.n) {
-            const int64_t id = load_id(ids, wide, i);
-            key[r] = id >= 0 && id < rows && id != skip ? (u32)id : (u32)rows;
-        }
-    }
-    for (int pass = 0; pass < q.passes; ++pass) {
-        const int shift = q.pass[pass].shift, bits = q.pass[pass].bits;
-        const u32 mask = (1u << bits) - 1;
-        if (tid < 256) base[tid] = 0;
+        for (int r = 0; r < RANK_PIECE / SORT_THREADS; ++r) ((u32*)piece)[r * SORT_THREADS + tid] = key_of(j0 + r * SORT_THREADS + tid);
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (r * SORT_THREADS + tid < q.n) atomicAdd(&base[(key[r] >> shift) & mask], 1u);
-        __syncthreads();
-        u32 total = 0, incl = 0;
-        if (tid < 256) {
-            incl = total = base[tid];
+        for (int b = 0; b < RANK_PIECE / (16 * 64); ++b) {
+            const int at = (b * 16 + wave) * 64;     // 64 keys: all before the workgroup's entries, all behind, or the ones that those are among
+            if (j0 + at >= n) break;
+            if (j0 + at != home) {
+                const u32 limit = j0 + at < home ? key + 1 : key;
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const u32 t = __shfl_up(incl, o, 64);
-                if (lane >= o) incl += t;
-            }
-            if (lane == 63) part[wave] = incl;
-        }
-        __syncthreads();
-        if (tid < 256) {
-            for (int w = 0; w < wave; ++w) incl += part[w];
-            base[tid] = incl - total;
-        }
+                for (int k = 0; k < 16 / J; ++k) {
+                    const u32x4 v = piece[at / 4 + k * J + share];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (r >= rounds) break;                          // (the same for the whole workgroup)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ((u32*)wcount)[tid + SORT_THREADS * i] = 0;
-            __syncthreads();
-            const bool valid = r * SORT_THREADS + tid < q.n;
-            const u32 digit = (key[r] >> shift) & mask;
-            uint64_t same = __ballot(valid);
-            for (int b = 0; b < bits; ++b) {
-                const uint64_t set = __ballot((digit >> b) & 1);
-                same &= ((digit >> b) & 1) ? set : ~set;
-            }
-            const u32 rank = (u32)__popcll(same & ((1ull << lane) - 1));
-            if (valid && rank == 0) wcount[wave][digit] = (u32)__popcll(same);
-            __syncthreads();
-            if (tid < 256) {
-                u32 a = base[tid];
-#pragma unroll
-                for (int w = 0; w < 16; ++w) {
-                    const u32 c = wcount[w][tid];
-                    wcount[w][tid] = a;
-                    a += c;
+                    for (int e = 0; e < 4; ++e) place += v[e] < limit;
                 }
-                base[tid] = a;
+            } else {
+                for (int k = 0; k < 16 / J; ++k) {
+                    const u32x4 v = piece[at / 4 + k * J + share];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) place += v[e] < key || (v[e] == key && j0 + at + (k * J + share) * 4 + e < i);
+                }
             }
-            __syncthreads();
-            at[r] = wcount[wave][digit] + rank;
-            __syncthreads();
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (r * SORT_THREADS + tid < q.n) { list[at[r]] = key[r]; list_from[at[r]] = (unsigned short)from[r]; }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = r * SORT_THREADS + tid;
-            if (i < q.n) { key[r] = list[i]; from[r] = list_from[i]; }
         }
         __syncthreads();
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int i = r * SORT_THREADS + tid;
-        if (i < q.n) { keys_out[i] = key[r]; from_out[i] = from[r]; }
+    count[tid] = place;
+    __syncthreads();
+    if (tid < TOK && i < n) {
+        u32 sum = 0;
+#pragma unroll 16
+        for (int k = 0; k < 16 * J; ++k) sum += count[k * TOK + tid];
+        keys_out[sum] = key;
+        from_out[sum] = (u32)i;
     }
 }
 
@@ -758,11 +724,12 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     char* part = (char*)flags + 2 * flag_bytes;
     const SortPlan sp = sort_plan(n, rows);
     int sorted = sp.passes & 1;                                                   // the buffers that hold the sorted list
-    if (n <= SORT_SMALL) {
-        SmallSort q = {(int)n, sp.passes, {}};
-        for (int i = 0; i < sp.passes; ++i) q.pass[i] = sp.pass[i];
+    if (n <= RANK_TOKENS) {
+        const int tok = n <= 4096 ? 16 : 32, blocks = (int)((n + tok - 1) / tok);          // about a workgroup to a CU
         const ZeroPart z = zero_share(zero, rows * dim, 0, 1, &zb);
-        hipLaunchKernelGGL(sort_small_kernel, dim3(1 + zb), dim3(SORT_THREADS), 0, s, ids, id_bytes == 8, rows, skip_id, keys[0], from[0], q, z);
+#define RANK(T) hipLaunchKernelGGL((rank_kernel<T>), dim3(blocks + zb), dim3(SORT_THREADS), 0, s, ids, id_bytes == 8, rows, skip_id, keys[0], from[0], (int)n, blocks, z)
+        if (tok == 16) RANK(16); else RANK(32);
+#undef RANK
         sorted = 0;
     } else {
         for (int i = 0; i < sp.passes; ++i) {
