@@ -5,7 +5,12 @@
 // ascending order; the sorted list is cut into chunks, a workgroup sums the runs of equal ids of its chunk in registers (fp32), writes the runs
 // that lie inside the chunk to dW and leaves the sums of runs that cross a border in the workspace; a second launch joins those in chunk order.
 // No floating-point atomics: the order of every sum depends on the ids alone, so that equal inputs give equal bits, and a row named by most
-// of the tokens (padding, start and end marks) is summed by as many workgroups as its share of the list.
+// of the tokens (padding, start and end marks) is summed by as many workgroups as its share of the list.  Up to 512 tokens need no list at all (direct_kernel).
+//
+// Measured:  forward 2048 x 77 of 768 fp32 with pos 81 us, 6.6 TB/s, bound by the writes (a fill: 6.8).  Gradient 160 x 77 of 49 408 x 768 fp32 with dpos 60 us: four
+// launches of 7.4 us that sort and, for the most of their time, fill dweight with zeros (152 MB), 20 us of sums (dy read twice, the second time from the cache), 12 us
+// for the runs that cross chunks.  64 x 2048 of 49 408 x 1024 bf16 137-144 us: sort and zeros 42 us, sums 91 us at 4.2
+// TB/s (rows gathered, 2 KB each), 14 us for the crossing runs.
 #include "common.h"
 
 typedef unsigned int u32;
