@@ -9,8 +9,8 @@
 //
 // Measured:  forward 2048 x 77 of 768 fp32 with pos 81 us, 6.6 TB/s, bound by the writes (a fill: 6.8).  Gradient 160 x 77 of 49 408 x 768 fp32 with dpos 60 us: four
 // launches of 7.4 us that sort and, for the most of their time, fill dweight with zeros (152 MB), 20 us of sums (dy read twice, the second time from the cache), 12 us
-// for the runs that cross chunks.  64 x 2048 of 49 408 x 1024 bf16 137-144 us: sort and zeros 42 us, sums 91 us at 4.2
-// TB/s (rows gathered, 2 KB each), 14 us for the crossing runs.
+// for the runs that cross chunks.  64 x 2048 of 49 408 x 1024 bf16 137 us, nearly all of it the sums (rows gathered, 2 KB
+// each, at 4.2 TB/s) with the zeros of the rows that no id names.
 #include "common.h"
 
 typedef unsigned int u32;
@@ -326,6 +326,7 @@ struct RunParams {
     RunList list[2];                                 // dweight, and dpos if there is one
     const void* dy;
     int n, chunk, chunks, dim, length, seqs;         // dpos: entry j is row t = j / seqs of the sequence j % seqs
+    int zeros;                                       // this launch zeroes the rows of dweight that no id names
 };
 __device__ __forceinline__ u32 run_key(const RunParams& p, const RunList& l, int j) { return l.keys ? l.keys[j] : (u32)(j / p.seqs); }
 __device__ __forceinline__ int64_t run_from(const RunParams& p, const RunList& l, int j) { return l.keys ? (int64_t)l.from[j] : (int64_t)(j % p.seqs) * p.length + j / p.seqs; }
@@ -377,9 +378,37 @@ __device__ __forceinline__ void add_raw16(fvec<E>& acc, const u32x4& r) {
     }
 }
 
-// blockIdx.x: a chunk of the list blockIdx.z;  eight rows are requested before the first is added (the gather's latency is what there is to hide)
+// 16 rows to a wave: each is looked for in the sorted list, and zeroed where it is not
+#define ZERO_ROWS 16
+__device__ __forceinline__ void zero_unnamed(const RunParams& p) {
+    const RunList& l = p.list[0];
+    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int64_t wave = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * waves + (threadIdx.x >> 6), stride = (int64_t)gridDim.x * gridDim.y * waves * ZERO_ROWS;
+    const fvec<4> zero = {{0.f, 0.f, 0.f, 0.f}};
+    for (int64_t r0 = wave * ZERO_ROWS; r0 < l.rows; r0 += stride) {
+        const int64_t r = r0 + (lane & (ZERO_ROWS - 1));
+        int lo = 0, hi = p.n;                        // the first entry whose key is not smaller than r
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if ((int64_t)l.keys[mid] < r) lo = mid + 1; else hi = mid;
+        }
+        const bool named = lo < p.n && (int64_t)l.keys[lo] == r;
+        unsigned todo = (unsigned)__ballot(lane < ZERO_ROWS && r < l.rows && !named);
+        while (todo) {
+            float* row = l.out + (r0 + __builtin_ctz(todo)) * p.dim;
+            todo &= todo - 1;
+            for (int own = lane * 4; own < p.dim; own += 256) {
+                const int c = piece_at<4>(own, p.dim);
+                store_e<4, float>(row + c, zero, p.dim >= 4, p.dim - c);
+            }
+        }
+    }
+}
+
+// blockIdx.x: a chunk of the list blockIdx.z (the last blockIdx.z: zeros, if this launch has them);  eight rows are requested before the first is added (the gather's latency is what there is to hide)
 template <typename T, int E, bool NT>
 __global__ __launch_bounds__(256) void run_sum_kernel(RunParams p) {
+    if (p.zeros && blockIdx.z == gridDim.z - 1) { zero_unnamed(p); return; }
     const RunList& l = p.list[blockIdx.z];
     const int own = (blockIdx.y * 256 + threadIdx.x) * E, c = piece_at<E>(own, p.dim);
     if (own >= p.dim) return;
@@ -700,6 +729,10 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
                "hh_embed_tokens_bwd: ids, dy and a 16-byte aligned workspace are needed");
     int zb = 0;
     float* zero = accumulate ? nullptr : dweight;
+    // zeros beside the sort, for all of dweight, or beside the sums, for the rows that no id names: where there are as many tokens as rows most rows are named, and are
+    // not written twice (131 072 tokens of 49 408 x 1024, spread evenly 153 -> 136 us, by Zipf's law 144 -> 138, all of one id 144 -> 153; 50 000 of 49 408 x 768
+    // 90.5 -> 81.6, 87 -> 84, 97 -> 105; 12 320 of 10 000 x 768 no difference)
+    const bool late = zero != nullptr && n > RANK_TOKENS && n >= rows;
     if (n == 0) {
         ZeroPart z = zero_share(zero, rows * dim, 0, 1, &zb);
         if (zb) hipLaunchKernelGGL(zero_kernel, dim3(zb), dim3(SORT_THREADS), 0, s, z);
@@ -738,21 +771,22 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
         sorted = 0;
     } else {
         for (int i = 0; i < sp.passes; ++i) {
-            ZeroPart z = zero_share(zero, rows * dim, 2 * i, 2 * sp.passes, &zb);
+            ZeroPart z = zero_share(late ? nullptr : zero, rows * dim, 2 * i, 2 * sp.passes, &zb);
             hipLaunchKernelGGL(sort_count_kernel, dim3(sp.blocks + zb), dim3(SORT_THREADS), 0, s, i == 0 ? ids : nullptr, id_bytes == 8, rows, skip_id, keys[i & 1], hist, (int)n, sp.per_block,
                                sp.pass[i].shift, sp.pass[i].bits, sp.blocks, z);
-            z = zero_share(zero, rows * dim, 2 * i + 1, 2 * sp.passes, &zb);
+            z = zero_share(late ? nullptr : zero, rows * dim, 2 * i + 1, 2 * sp.passes, &zb);
             hipLaunchKernelGGL(sort_place_kernel, dim3(sp.blocks + zb), dim3(SORT_THREADS), 0, s, keys[i & 1], i == 0 ? nullptr : from[i & 1], hist, keys[(i + 1) & 1], from[(i + 1) & 1], (int)n,
                                sp.per_block, sp.pass[i].shift, sp.pass[i].bits, sp.blocks, z);
         }
     }
     RunParams p;
     p.dy = dy; p.n = (int)n; p.chunk = run_chunk(n, run_waves(dim, e)); p.chunks = (int)chunks; p.dim = dim; p.length = length; p.seqs = (int)seqs;
+    p.zeros = late;
     p.list[0] = RunList{keys[sorted], from[sorted], dweight, (float*)part, flags, rows, accumulate != 0, scale};
     p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), flags + flag_bytes, length, 0, 1.f};
     const int need = (dim + e - 1) / e;
     const int threads = need >= 256 ? 256 : (need + 63) / 64 * 64;
-    const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), dpos ? 2u : 1u);
+    const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), (dpos ? 2u : 1u) + (late ? 1u : 0u));
     // dy past the caches where it is read once (64 x 2048 x 1024 bf16: 210 -> 190 us) or does not fit there; with dpos it is read twice, and 160 x 77 x 768 fp32
     // stay in the cache between (61.5 us, 65.3 past it)
     const bool nt = !dpos || n * dim * (e == 4 ? 4 : 2) > HH_STREAM_BYTES;
