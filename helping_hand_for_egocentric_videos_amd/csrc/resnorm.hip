@@ -479,11 +479,11 @@ __global__ __launch_bounds__(R == 4 ? 256 : 1024) void resnorm_bwd_kernel(RnPara
     float* out = p.part + blockIdx.x * (int64_t)p.cols;
     if constexpr (POST) {
         rn_put<VEC>(ag1, out, c, p.cols);
-        rn_put<VEC>(ab1, out + plane, c, p.cols);
+        if (p.b1) rn_put<VEC>(ab1, out + plane, c, p.cols);             // (a norm without beta: no plane of its gradient)
     }
     if constexpr (PRE) {
         rn_put<VEC>(ag2, out + 2 * plane, c, p.cols);
-        rn_put<VEC>(ab2, out + 3 * plane, c, p.cols);
+        if (p.b2) rn_put<VEC>(ab2, out + 3 * plane, c, p.cols);
     }
 }
 
