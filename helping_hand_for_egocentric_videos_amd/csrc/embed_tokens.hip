@@ -7,9 +7,9 @@
 // No floating-point atomics: the order of every sum depends on the ids alone, so that equal inputs give equal bits, and a row named by most
 // of the tokens (padding, start and end marks) is summed by as many workgroups as its share of the list.  Up to 512 tokens need no list at all (direct_kernel).
 //
-// Measured:  forward 2048 x 77 of 768 fp32 with pos 81 us, 6.6 TB/s, bound by the writes (a fill: 6.8).  Gradient 160 x 77 of 49 408 x 768 fp32 with dpos 60 us: four
-// launches of 7.4 us that sort and, for the most of their time, fill dweight with zeros (152 MB), 20 us of sums (dy read twice, the second time from the cache), 12 us
-// for the runs that cross chunks.  64 x 2048 of 49 408 x 1024 bf16 137 us, nearly all of it the sums (rows gathered, 2 KB
+// Measured:  forward 2048 x 77 of 768 fp32 with pos 81 us, 6.6 TB/s, bound by the writes (a fill: 6.8).  Gradient 160 x 77 of 49 408 x 768 fp32 with dpos 58 us: four
+// launches of 7 us that sort and, for the most of their time, fill dweight with zeros (152 MB), 20 us of sums (dy read twice, the second time from the cache), 12 us
+// for the runs that cross chunks.  64 x 2048 of 49 408 x 1024 bf16 142 us, nearly all of it the sums (rows gathered, 2 KB
 // each, at 4.2 TB/s) with the zeros of the rows that no id names.
 #include "common.h"
 
@@ -136,14 +136,15 @@ static SortPlan sort_plan(int64_t n, int64_t rows) {
 
 // A fresh gradient's zeros ride along: the sort keeps few CUs busy and waits for latencies, so that each of its launches carries, in the workgroups
 // behind its own, an equal part of the fill (152 MB for 49 408 x 768: 20 us at the card's 6.9 TB/s of a fill alone, spread over four launches here).
-struct ZeroPart { float* p; int64_t begin, end; int wide; };
+struct ZeroPart { float* p; int64_t begin, end; int wide, nt; };
 
 __device__ __forceinline__ void zero_part(const ZeroPart& z, int block, int blocks) {
     const int64_t first = z.begin + ((int64_t)block * SORT_THREADS + threadIdx.x) * (z.wide ? 4 : 1);
     const int64_t stride = (int64_t)blocks * SORT_THREADS * (z.wide ? 4 : 1);
     if (z.wide) {                                    // begin, end: multiples of 4
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t i = first; i < z.end; i += stride) *(f32x4*)(z.p + i) = zero;
+        if (z.nt) for (int64_t i = first; i < z.end; i += stride) __builtin_nontemporal_store(zero, (f32x4*)(z.p + i));
+        else for (int64_t i = first; i < z.end; i += stride) *(f32x4*)(z.p + i) = zero;
     } else {
         for (int64_t i = first; i < z.end; i += stride) z.p[i] = 0.f;
     }
@@ -326,7 +327,7 @@ struct RunParams {
     RunList list[2];                                 // dweight, and dpos if there is one
     const void* dy;
     int n, chunk, chunks, dim, length, seqs;         // dpos: entry j is row t = j / seqs of the sequence j % seqs
-    int zeros;                                       // this launch zeroes the rows of dweight that no id names
+    int zeros;                                       // this launch zeroes the rows of dweight that no id names (2: past the caches)
 };
 __device__ __forceinline__ u32 run_key(const RunParams& p, const RunList& l, int j) { return l.keys ? l.keys[j] : (u32)(j / p.seqs); }
 __device__ __forceinline__ int64_t run_from(const RunParams& p, const RunList& l, int j) { return l.keys ? (int64_t)l.from[j] : (int64_t)(j % p.seqs) * p.length + j / p.seqs; }
@@ -399,7 +400,7 @@ __device__ __forceinline__ void zero_unnamed(const RunParams& p) {
             todo &= todo - 1;
             for (int own = lane * 4; own < p.dim; own += 256) {
                 const int c = piece_at<4>(own, p.dim);
-                store_e<4, float>(row + c, zero, p.dim >= 4, p.dim - c);
+                if (p.zeros > 1) store_e<4, float, true>(row + c, zero, p.dim >= 4, p.dim - c); else store_e<4, float>(row + c, zero, p.dim >= 4, p.dim - c);
             }
         }
     }
@@ -701,9 +702,10 @@ extern "C" int64_t hh_workspace_bytes_embed_tokens_bwd(int64_t seqs, int length,
     return 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4) + 2 * align256(chunks) + 2 * align256(chunks * 2 * (int64_t)dim * 4);
 }
 
-// part i of `parts` of the zeros of out, and the workgroups that write it
+// part i of `parts` of the zeros of out, and the workgroups that write it.  Large gradients are zeroed past the caches: 160 x 77 of 49 408 x 768 fp32 with a few outputs in
+// turn 67.5 -> 58.3 us (59.4 -> 57.9 with one output's memory over and over), 64 x 2048 of 49 408 x 1024 bf16 147.4 -> 141.5 (137.5 -> 140.7).
 static ZeroPart zero_share(float* out, int64_t total, int i, int parts, int* blocks) {
-    ZeroPart z = {out, 0, 0, 0};
+    ZeroPart z = {out, 0, 0, 0, total * 4 > HH_STREAM_BYTES};
     *blocks = 0;
     if (out == nullptr) return z;
     z.wide = HH_ALIGNED16(out) && total % 4 == 0;
@@ -781,7 +783,7 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     }
     RunParams p;
     p.dy = dy; p.n = (int)n; p.chunk = run_chunk(n, run_waves(dim, e)); p.chunks = (int)chunks; p.dim = dim; p.length = length; p.seqs = (int)seqs;
-    p.zeros = late;
+    p.zeros = !late ? 0 : rows * dim * 4 > HH_STREAM_BYTES ? 2 : 1;
     p.list[0] = RunList{keys[sorted], from[sorted], dweight, (float*)part, flags, rows, accumulate != 0, scale};
     p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), flags + flag_bytes, length, 0, 1.f};
     const int need = (dim + e - 1) / e;
