@@ -5,7 +5,7 @@
 // ascending order; the sorted list is cut into chunks, a workgroup sums the runs of equal ids of its chunk in registers (fp32), writes the runs
 // that lie inside the chunk to dW and leaves the sums of runs that cross a border in the workspace; a second launch joins those in chunk order.
 // No floating-point atomics: the order of every sum depends on the ids alone, so that equal inputs give equal bits, and a row named by most
-// of the tokens (padding, start and end marks) is summed by as many workgroups as its share of the list.  Up to 512 tokens need no list at all (direct_kernel).
+// of the tokens (padding, start and end marks) is summed by as many workgroups as its share of the list.  Up to 512 or 1024 tokens need no list at all (direct_kernel).
 //
 // Measured:  forward 2048 x 77 of 768 fp32 with pos 81 us, 6.6 TB/s, bound by the writes (a fill: 6.8).  Gradient 160 x 77 of 49 408 x 768 fp32 with dpos 58 us: four
 // launches of 7 us that sort and, for the most of their time, fill dweight with zeros (152 MB), 20 us of sums (dy read twice, the second time from the cache), 12 us
@@ -552,14 +552,16 @@ static int run_chunk(int64_t n, int waves) {
 static int64_t run_chunks(int64_t n, int waves) { return n ? (n + run_chunk(n, waves) - 1) / run_chunk(n, waves) : 0; }
 
 // ---- few tokens: one launch, no sort -----------------------------------------------------------------------------------------------------
-// Up to DIRECT_TOKENS tokens every workgroup can look at all ids itself.  Three kinds of workgroups, by blockIdx.x:
+// Up to DIRECT_TOKENS tokens (DIRECT_NARROW of rows that one workgroup spans) every workgroup can look at all ids itself.  Three kinds of workgroups, by blockIdx.x:
 //   [0, n): a token; the first one of its id finds the others (in ascending order) and sums their rows, the rest of them end
 //   then [0, length) if dpos is wanted: a position's rows
 //   then the zeros of the rows of dweight that no id names, a range of at most DIRECT_ROWS rows each.
 // A workgroup takes 128 pieces of 16 bytes of a row (blockIdx.y); the rows of a sum are dealt out to its 8 (at most 16) sets of threads, whose sums are added in
 // order.  All launches with dpos, sorted -> direct:  6 tokens x 512 fp32 9.4 -> 3.7 us, 64 x 768 bf16 18.9 -> 3.9, 512 x 768 fp32 18.4 -> 8.3 (all of one id
-// 18.0 -> 12.4);  1014 x 1024 fp32 19.2 -> 13.2, but of one id 19.3 -> 22.6, and 1000 x 2048 bf16 18.9 -> 22.0.
+// 18.0 -> 12.4);  1001 x 512 fp32 16.6 -> 7.9 (half of one id 17.7 -> 15.8, all of it 15.3 -> 19.5);  wider rows: 1014 x 1024 fp32 19.2 -> 13.2, but of one id
+// 19.3 -> 22.6, and 1000 x 2048 bf16 18.9 -> 22.0.
 #define DIRECT_TOKENS 512
+#define DIRECT_NARROW 1024
 #define DIRECT_ROWS 32768
 #define DIRECT_PIECES 128
 struct DirectParams {
@@ -690,14 +692,14 @@ extern "C" int hh_embed_tokens_fwd(const void* ids, int id_bytes, const void* we
 }
 
 // (1024 zeros' workgroups at most)
-static bool direct_fits(int64_t n, int64_t rows) { return n <= DIRECT_TOKENS && rows <= 1024ll * DIRECT_ROWS; }
+static bool direct_fits(int64_t n, int64_t rows, int dim, int e) { return n <= (dim <= DIRECT_PIECES * e ? DIRECT_NARROW : DIRECT_TOKENS) && rows <= 1024ll * DIRECT_ROWS; }
 
 static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 
 extern "C" int64_t hh_workspace_bytes_embed_tokens_bwd(int64_t seqs, int length, int64_t rows, int dim) {
     if (!embed_shape_ok(seqs, length, rows, dim)) return -1;
     const int64_t n = seqs * length;
-    if (direct_fits(n, rows)) return 0;
+    if (direct_fits(n, rows, dim, 4)) return 0;
     const int64_t chunks = run_chunks(n, run_waves(dim, 8));                         // (bf16; fp32 rows take more waves, and fewer chunks)
     return 4 * align256(4 * n) + align256(SORT_BLOCKS * 256 * 4) + 2 * align256(chunks) + 2 * align256(chunks * 2 * (int64_t)dim * 4);
 }
@@ -726,7 +728,8 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     HH_REQUIRE(dweight != nullptr, HH_ERR_ALIGN, "hh_embed_tokens_bwd: dweight is NULL");
     hipStream_t s = (hipStream_t)stream;
     const int64_t n = seqs * length;
-    const bool direct = direct_fits(n, rows);
+    const int e = dy_dtype == HH_F32 ? 4 : 8;
+    const bool direct = direct_fits(n, rows, dim, e);
     HH_REQUIRE(n == 0 || (ids != nullptr && dy != nullptr && (direct || (workspace != nullptr && HH_ALIGNED16(workspace)))), HH_ERR_ALIGN,
                "hh_embed_tokens_bwd: ids, dy and a 16-byte aligned workspace are needed");
     int zb = 0;
@@ -748,7 +751,7 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
         const int64_t least = accumulate ? 0 : (rows + DIRECT_ROWS - 1) / DIRECT_ROWS;
         if (zeros < least) zeros = least;
         DirectParams p = {ids, id_bytes == 8, rows, skip_id, dy, dweight, dpos, accumulate != 0, (int)n, dim, length, (int)seqs, scale, zeros ? (rows + zeros - 1) / zeros : 0};
-        const int across = (dy_dtype == HH_F32 ? 4 : 8) * DIRECT_PIECES;
+        const int across = e * DIRECT_PIECES;
         const dim3 grid((unsigned)(n + (dpos ? length : 0) + zeros), (unsigned)((dim + across - 1) / across));
         if (dy_dtype == HH_F32) hipLaunchKernelGGL((direct_kernel<float, 4>), grid, dim3(1024), 0, s, p);
         else hipLaunchKernelGGL((direct_kernel<bf16_t, 8>), grid, dim3(1024), 0, s, p);
@@ -759,7 +762,6 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     u32* from[2] = {(u32*)(ws + 2 * align256(4 * n)), (u32*)(ws + 3 * align256(4 * n))};
     u32* hist = (u32*)(ws + 4 * align256(4 * n));
     unsigned char* flags = (unsigned char*)hist + align256(SORT_BLOCKS * 256 * 4);
-    const int e = dy_dtype == HH_F32 ? 4 : 8;
     const int64_t chunks = run_chunks(n, run_waves(dim, e)), flag_bytes = align256(chunks), part_bytes = align256(chunks * 2 * (int64_t)dim * 4);
     char* part = (char*)flags + 2 * flag_bytes;
     const SortPlan sp = sort_plan(n, rows);

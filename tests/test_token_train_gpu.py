@@ -610,10 +610,10 @@ def test_embed_tokens_bwd_adds_once_where_pieces_share_channels(S, L, V, dim, dt
 
 @pytest.mark.parametrize("S,L,V,dim", [(1, 512, 40, 768), (512, 1, 3, 2052), (16, 32, 49408, 12), (7, 73, 33000, 1), (3, 171, 700000, 3), (2, 9, 4, 70000), (1, 1, 40000000, 4),
                                        (513, 1, 60, 5), (64, 64, 300, 33), (17, 241, 20, 8), (3, 1366, 49408, 16), (128, 64, 2000, 12), (8193, 1, 70, 4),
-                                       (91, 101, 9000, 5), (30, 1000, 29999, 3), (5, 2000, 9999, 770)])
+                                       (91, 101, 9000, 5), (30, 1000, 29999, 3), (8, 128, 700, 33), (1, 1024, 60, 512), (32, 32, 9, 1024), (13, 77, 60, 516), (41, 25, 90, 64), (5, 2000, 9999, 770)])
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_embed_tokens_bwd_of_few_tokens(S, L, V, dim, dt):
-    """One launch (up to 512 tokens), a sort by counting (8192) and just over, tables of many rows or wide ones: whole numbers, so that the stock sums are exact."""
+    """One launch (up to 512 or 1024 tokens), a sort by counting (8192) and just over, tables of many rows or wide ones: whole numbers, so that the stock sums are exact."""
     ids = rints(-2, V + 2, (S, L), seed=4)
     ids[0, 0] = V - 1
     if S * L > 100:
