@@ -644,15 +644,16 @@ def one_pass(t):
     return [x, xn, h, a, q.view(torch.uint8), s, du, dw, db, de, dpos, *g]
 
 
-def pass_inputs(seed):
-    S, L, V, D = 20, 77, 500, 256
+def pass_inputs(seed, S=20):
+    L, V, D = 77, 500, 256
     s = make_block(S * L, D, "group", True, True, False, F32, BF16, seed=seed, groups=S)
     return dict(ids=rints(0, V, (S, L), seed=seed), w=rnd(V, D, seed=seed + 1), pos=rnd(L, D, seed=seed + 2), y=s["y"], gate=s["gate"], post=s["post"], pre=s["pre"],
                 da=rnd(S * L, D, seed=seed + 3, dtype=BF16))
 
 
-def test_graph_replays_equal_eager_passes():
-    static = pass_inputs(0)
+@pytest.mark.parametrize("S", [5, 20, 130])                        # (a gradient without a sort, one by counting, one by digits with the zeros beside the sums)
+def test_graph_replays_equal_eager_passes(S):
+    static = pass_inputs(0, S)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -663,7 +664,7 @@ def test_graph_replays_equal_eager_passes():
     with torch.cuda.graph(graph):
         outs = one_pass(static)
     for seed in (0, 7, 3, 7):
-        new = pass_inputs(seed)
+        new = pass_inputs(seed, S)
         for k, v in new.items():
             for dst, src in zip(static[k], v) if isinstance(v, tuple) else ((static[k], v),):
                 if isinstance(dst, torch.Tensor):
@@ -678,8 +679,9 @@ def test_graph_replays_equal_eager_passes():
             assert torch.equal(a, b), (seed, i)
 
 
-def test_two_streams_at_once():
-    a, b = pass_inputs(1), pass_inputs(2)
+@pytest.mark.parametrize("S", [5, 20, 130])
+def test_two_streams_at_once(S):
+    a, b = pass_inputs(1, S), pass_inputs(2, S)
     want = [one_pass(a), one_pass(b)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
