@@ -541,7 +541,7 @@ __global__ __launch_bounds__(1024) void run_join_kernel(RunParams p) {
 __global__ __launch_bounds__(SORT_THREADS) void zero_kernel(ZeroPart z) { zero_part(z, blockIdx.x, gridDim.x); }
 
 // Rows of a chunk: as many workgroups as fit the chip at once (run_sum_kernel leaves room for 7 waves on each of 1024 SIMDs; a second round of them waits for the
-// first: 64 x 2048 x 1024 bf16 in chunks of 32 rows 165 us, 48 rows 142, 64 rows 154), whole batches of eight rows, and 16 rows at least, because every
+// first: 64 x 2048 x 1024 bf16 in chunks of 32 rows 166 us, 40 rows 142, 64 rows 162), whole batches of eight rows, and 16 rows at least, because every
 // border between chunks may leave two partial rows (160 x 77 x 768 fp32: 8 rows 68 us, 16 rows 61, 32 rows 65).
 #define RUN_WAVES 6600
 static int run_waves(int dim, int e) { return (dim + 64 * e - 1) / (64 * e); }
@@ -791,8 +791,8 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     const int need = (dim + e - 1) / e;
     const int threads = need >= 256 ? 256 : (need + 63) / 64 * 64;
     const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), (dpos ? 2u : 1u) + (late ? 1u : 0u));
-    // dy past the caches where it is read once (64 x 2048 x 1024 bf16: 210 -> 190 us) or does not fit there; with dpos it is read twice, and 160 x 77 x 768 fp32
-    // stay in the cache between (61.5 us, 65.3 past it)
+    // dy past the caches where it is read once (64 x 2048 x 1024 bf16: 150 -> 142 us) or does not fit there; with dpos it is read twice, and 160 x 77 x 768 fp32
+    // stay in the cache between (58.5 us, 64.7 past it)
     const bool nt = !dpos || n * dim * (e == 4 ? 4 : 2) > HH_STREAM_BYTES;
     if (e == 4 && nt) hipLaunchKernelGGL((run_sum_kernel<float, 4, true>), grid, dim3(threads), 0, s, p);
     else if (e == 4) hipLaunchKernelGGL((run_sum_kernel<float, 4, false>), grid, dim3(threads), 0, s, p);
