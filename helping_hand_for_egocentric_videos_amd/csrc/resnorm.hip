@@ -592,11 +592,12 @@ static int rn_check(const hh_residual_norm* d, bool bwd, const char* who) {
                "%s: %lld rows do not split into %lld gate groups (1 without a gate for each group, 65000 at most)", who, (long long)d->rows, (long long)d->groups);
     HH_REQUIRE((d->x_dtype == HH_F32 || d->x_dtype == HH_BF16) && (d->y_dtype == HH_F32 || d->y_dtype == HH_BF16) && (d->h_dtype == HH_F32 || d->h_dtype == HH_BF16), HH_ERR_DTYPE,
                "%s: bad dtype", who);
-    if (d->rows == 0) return HH_OK;
-    HH_REQUIRE(d->y != nullptr && d->x_new != nullptr && (bwd ? (d->dx != nullptr && d->dy != nullptr) : d->x != nullptr), HH_ERR_ALIGN, "%s: NULL pointer", who);
+    // (the parameters are read without rows too: the backward pass of none writes their gradients, a tanh gate's from its values)
     HH_REQUIRE((d->gate_kind == HH_GATE_NONE) == (d->gate == nullptr), HH_ERR_ALIGN, "%s: gate kind and pointer do not agree", who);
     HH_REQUIRE(d->post_gamma != nullptr || d->post_beta == nullptr, HH_ERR_ALIGN, "%s: post_beta without post_gamma", who);
     HH_REQUIRE(d->pre_gamma != nullptr || d->pre_beta == nullptr, HH_ERR_ALIGN, "%s: pre_beta without pre_gamma", who);
+    if (d->rows == 0) return HH_OK;
+    HH_REQUIRE(d->y != nullptr && d->x_new != nullptr && (bwd ? (d->dx != nullptr && d->dy != nullptr) : d->x != nullptr), HH_ERR_ALIGN, "%s: NULL pointer", who);
     if (bwd) HH_REQUIRE((d->dh != nullptr) == (d->pre_gamma != nullptr), HH_ERR_ALIGN, "%s: dh comes with pre_gamma", who);
     else HH_REQUIRE((d->h != nullptr) == (d->pre_gamma != nullptr), HH_ERR_ALIGN, "%s: h comes with pre_gamma", who);
     return HH_OK;

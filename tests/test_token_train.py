@@ -145,3 +145,18 @@ def test_norm_modules_that_the_residual_does_not_take_are_refused():
         for where in ("post", "pre"):
             with pytest.raises(TypeError, match=where):
                 ts.residual_norm(x, x, rms=rms, **{where: norm})
+
+
+def test_residual_norm_without_rows_still_needs_the_parameters_it_reads():
+    """The backward pass of no rows writes the parameters' gradients, a tanh gate's from the gate's values: a gate that is not there is refused as it is with rows."""
+    L = _lib.lib()
+    for gate_kind, dgate in ((1, 16), (2, 16), (3, 16)):
+        for tanh in (0, 1):
+            d = _lib.ResidualNorm()
+            d.rows, d.groups, d.cols, d.res_scale, d.gate_kind, d.gate_tanh, d.dgate = 0, 1, 64, 1.0, gate_kind, tanh, dgate
+            assert L.hh_residual_norm_bwd(ctypes.byref(d), None) == -5 and L.hh_residual_norm_fwd(ctypes.byref(d), None) == -5
+    for beta in ("post_beta", "pre_beta"):
+        d = _lib.ResidualNorm()
+        d.rows, d.groups, d.cols, d.res_scale = 0, 1, 64, 1.0
+        setattr(d, beta, 16)
+        assert L.hh_residual_norm_bwd(ctypes.byref(d), None) == -5 and L.hh_residual_norm_fwd(ctypes.byref(d), None) == -5
