@@ -29,7 +29,7 @@ __device__ __forceinline__ float act_slope(float v, int act) {
         const float s = sigmoid1702(v);
         return s * (1.f + 1.702f * v * (1.f - s));
     }
-    if (act == HH_ACT_RELU) return v > 0.f ? 1.f : 0.f;
+    if (act == HH_ACT_RELU) return v > 0.f ? 1.f : v <= 0.f ? 0.f : v;      // (keeps NaN)
     return 1.f;
 }
 

@@ -498,6 +498,28 @@ def test_act8_infinities_and_nan_touch_nothing_else():
     assert torch.equal(a, b) and torch.equal(q.view(torch.uint8), r.view(torch.uint8)) and torch.equal(s, t)
 
 
+@pytest.mark.parametrize("act", [ops.ACT_NONE, ops.ACT_QUICKGELU, ops.ACT_RELU])
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("cols", [128, 131, 5])
+def test_act8_bwd_shows_what_was_infinite_or_nan(act, dt, cols):
+    """A checkpoint holds infinities and NaN as NaN, and so does every gradient (and activation) that uses them, whatever the activation; their neighbours are as without them."""
+    u, da = rnd(6, cols, seed=1, dtype=dt), rnd(6, cols, seed=2, dtype=dt).abs() + 0.5
+    bad = torch.zeros(6, cols, dtype=torch.bool, device=DEV)
+    v = u.clone()
+    for r, c, t in ((0, 0, "inf"), (1, 3, "-inf"), (2, cols - 1, "nan"), (4, 2, "inf")):
+        v[r, c], bad[r, c], u[r, c] = float(t), True, 0              # (zero: counts for no scale either)
+    _, q, s = ops.act8(v, act)
+    _, q0, s0 = ops.act8(u, act)
+    assert torch.equal(s, s0)
+    du, a = ops.act8_bwd(q, s, da, act, want_out=True)
+    du0, a0 = ops.act8_bwd(q0, s0, da, act, want_out=True)
+    assert torch.isnan(du[bad]).all() or act == ops.ACT_NONE
+    assert torch.isnan(a[bad]).all()
+    assert torch.equal(du[~bad], du0[~bad]) and torch.equal(a[~bad], a0[~bad])
+    if act == ops.ACT_NONE:                                          # (a slope of one whatever the value)
+        assert torch.equal(du, da)
+
+
 def values(q, s):
     return q.double() * s.double().repeat_interleave(128, 1)[:, :q.shape[1]]
 
