@@ -5,7 +5,8 @@
 //              the largest e4m3 value; k is held in [-117, 120], and is 0 where all are zero);  q = u / s rounded to nearest, ties to even.
 //              A power of two, because then u / s and q * s are exact in fp32, and q * s (4 significant bits) is exact in bf16 too: the matrix core
 //              takes a checkpoint without a second rounding (gemm_tn8.hip), and the only error is e4m3's own half step, 2^-4 of the value
-//              (2^-10 of s below 2^-6 of s).  k >= -117 keeps the smallest step, 2^(k - 9), a normal number.
+//              (2^-10 of s below 2^-6 of s).  k >= -117 keeps the smallest step, 2^(k - 9), a normal number.  At the other end of the range |u| from 1.9375 * 2^127
+//              (3.29e38) on rounds to 2^128, the one q * s that fp32 and bf16 do not have: it is read back as infinity, as bf16 itself would round most of these.
 //              Infinities and NaN do not count for the scale; both are stored as e4m3's NaN, so that a gradient that uses them shows it.
 //   backward:  v = q * s;  du = da * act'(v), and on request act(v), the operand of the next product's weight gradient.
 //
@@ -26,11 +27,18 @@ __device__ __forceinline__ float act_value(float v, int act) {
 }
 __device__ __forceinline__ float act_slope(float v, int act) {
     if (act == HH_ACT_QUICKGELU) {
+        // s is 0 below -52 and 1 above 11 (to fp32): v no longer counts there, and 1.702 v, which is infinite from 2^127 / 0.851 on, stays finite.  s keeps NaN.
         const float s = sigmoid1702(v);
-        return s * (1.f + 1.702f * v * (1.f - s));
+        return s * (1.f + 1.702f * __builtin_amdgcn_fmed3f(v, -128.f, 128.f) * (1.f - s));
     }
     if (act == HH_ACT_RELU) return v > 0.f ? 1.f : v <= 0.f ? 0.f : v;      // (keeps NaN)
     return 1.f;
+}
+
+// act(v) of a checkpoint's value, which is infinite where a finite activation was rounded up to 2^128: QuickGELU of minus infinity is 0, not infinity * 0
+__device__ __forceinline__ float act_again(float v, int act) {
+    if (act == HH_ACT_QUICKGELU) return fmaxf(v, -3.402823466e38f) * sigmoid1702(v);
+    return act_value(v, act);
 }
 
 template <typename T, bool NT>
@@ -181,7 +189,7 @@ __global__ __launch_bounds__(256) void act8_bwd_kernel(const unsigned char* __re
     store8<T, NT>(du + at, whole, n, d);
     if (a != nullptr) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = act_value(v[j], act);
+        for (int j = 0; j < 8; ++j) v[j] = act_again(v[j], act);
         store8<T, NT>(a + at, whole, n, v);
     }
 }

@@ -1,7 +1,7 @@
 // Weight gradient from an 8-bit activation checkpoint:  dW[m, n] = sum_k dY[k, m] * q[k, n] * s[k, n / 128],  db[m] = sum_k dY[k, m],
 // dY bf16 [K tokens, M], q e4m3 [K, N] with a power-of-two scale for 128 channels of a token (act8.hip).
 //
-// q * s is exact in bf16 (4 significant bits times a power of two), so the operand is turned into bf16 on its way into LDS -- two values an
+// q * s is exact in bf16 (4 significant bits times a power of two; 2^128 alone is infinite, see act8.hip), so the operand is turned into bf16 on its way into LDS -- two values an
 // instruction, the scale inside it -- and the product runs on v_mfma_f32_16x16x32_bf16 with fp32 sums: the only roundings are those of the sums.
 // Both operands stand token-major in memory and in LDS (a row = 128 columns = 256 B); the transposing LDS read delivers the 8 consecutive
 // tokens that a lane of the matrix instruction wants.  16-byte chunk c of row r lies at c ^ tn8_key(r), which spreads the four rows x 32 B that

@@ -550,6 +550,7 @@ int hh_residual_norm_bwd(const hh_residual_norm* d, hh_stream_t stream);
 /* ---- activation checkpoints in 8 bits
  * hh_act8_fwd: a = act(u) (NULL: not wanted), q = e4m3(u / s) [rows, cols], scale = s = 2^k fp32 [rows, ceil(cols / 128)]: k is the smallest whole number in
  *   [-117, 120] with max |u| <= 448 * 2^k over the 128 channels (0 where all are zero; infinities and NaN do not count and are stored as NaN).
+ *   A finite |u| of 1.9375 * 2^127 or more is rounded to 2^128, which the readers of a checkpoint take as infinity; all other values of q * s are exact.
  * hh_act8_bwd: v = q * s, du = da * act'(v), a = act(v) (NULL: not wanted); da, du and a have `dtype`.
  * hh_gemm_tn_act8: dw fp32 [M, N] = dy^T (q * s) and db fp32 [M] = sum_k dy[k,:] (or NULL) over K tokens, dy bf16 [K, M] (ld_dy), q [K, N] (ldq), scale
  *   [K, ceil(N / 128)] whose entries are powers of two (only their exponents are used); q * s is exact in the matrix core's bf16, sums are fp32 and in a fixed

@@ -520,6 +520,32 @@ def test_act8_bwd_shows_what_was_infinite_or_nan(act, dt, cols):
         assert torch.equal(du, da)
 
 
+@pytest.mark.parametrize("act", [ops.ACT_NONE, ops.ACT_QUICKGELU, ops.ACT_RELU])
+def test_act8_bwd_at_the_ends_of_the_range(act):
+    """Finite activations up to fp32's largest.  From 1.9375 * 2^127 on (248 of a scale of 2^120: e4m3's middle between 240 and 256) a value rounds to 2^128, infinity in fp32;
+    the slope there is that of the far end, 1 or 0, and no other value is infinite."""
+    top = 3.402823466e38
+    border = 1.9375 * 2.0 ** 127
+    below = float(torch.tensor(border).nextafter(torch.tensor(0.0)))
+    vals = [top, border, below, 3e38, 2.9e38, 2.5e38, 2e38, 1.9e38, 1e38, 2.0 ** 100, 1e10, 200.0, 128.0, 60.0, 52.0]
+    u = torch.tensor([[v, -v] for v in vals], device=DEV)
+    da = torch.full_like(u, 0.75)
+    _, q, s = ops.act8(u, act)
+    qr, sr = act8_ref(u)
+    assert torch.equal(q.double().cpu(), qr) and torch.equal(s.double().cpu(), sr)
+    du, a = ops.act8_bwd(q, s, da, act, want_out=True)
+    v = (qr * sr).to(DEV)                                            # 64 bits: finite
+    assert (v.abs() >= 2.0 ** 128).sum() == 4
+    rv, slope = act_ref(v, act)
+    pos = torch.where(v.abs() >= 2.0 ** 128, float("inf"), rv.abs()) * torch.sign(v)
+    if act == ops.ACT_NONE:
+        assert torch.equal(du, da) and torch.equal(a.double(), pos)
+    else:
+        assert torch.equal(du[:, 0], da[:, 0])                       # (the slope at 52 and above is 1 to fp32)
+        assert (du[:, 1].abs() <= 2.0 ** -60).all()                  # e^(-1.702 * 52) < 2^-127, times 90
+        assert torch.equal(a[:, 0].double(), pos[:, 0]) and (a[:, 1].abs() <= 2.0 ** -60).all()
+
+
 def values(q, s):
     return q.double() * s.double().repeat_interleave(128, 1)[:, :q.shape[1]]
 
