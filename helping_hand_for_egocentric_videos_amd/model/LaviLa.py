@@ -30,6 +30,18 @@ def _require_gpu(x, who):
                            "there is no CPU fallback -- use oracle/ for CPU reference numbers")
 
 
+def _plain_f32(t):
+    """A contiguous fp32 tensor whose memory is its values (a subclass may hold them elsewhere)."""
+    return type(t) in (torch.Tensor, nn.Parameter) and t.dtype == torch.float32 and t.is_contiguous()
+
+
+def _looks_up_only(m):
+    """Whether calling the module does nothing but take rows of its table: an nn.Embedding as it is.  An adapter around a table, a module with hooks or with a bound on
+    its rows' norms has to be called."""
+    return (type(m) is nn.Embedding and "forward" not in vars(m) and m.max_norm is None and not m._forward_hooks and not m._forward_pre_hooks and
+            not nn.modules.module._has_any_global_hook() and _plain_f32(m.weight))
+
+
 class Mlp(nn.Module):
     def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=nn.GELU, drop=0.):
         super().__init__()
@@ -459,7 +471,8 @@ class CLIP(nn.Module):
         """LaviLa.py:660-670 (apply_project=False, as encode_image has it, skips the EOT-token projection: the training step only
         uses the feature map).  The backbone is frozen on this path (run/train.py:89,109-116; run/test_EgoMCQ.py:60 under no_grad):
         Linears and LayerNorms of the 12 text blocks run on libhh kernels (`Transformer.forward_frozen`), the 77 x 77 causal core on
-        hh_text_attn_fwd.  There is no stock-op branch: a text tower that wants gradients is not part of this path and raises."""
+        hh_text_attn_fwd.  There is no stock-op branch: a text tower that wants gradients is not part of this path and raises.  Token ids
+        must be in the table; one that is not gives NaN features from its position on (the stock lookup may read whatever lies there)."""
         _require_gpu(text, "CLIP.encode_text")
         if torch.is_grad_enabled() and any(p.requires_grad for p in self.transformer.parameters()):
             raise NotImplementedError("CLIP.encode_text: the text tower is frozen on the hot path (run/train.py:89 freezes the backbone; optim_policy, "
@@ -467,7 +480,7 @@ class CLIP(nn.Module):
                                       "no stock-op fallback -- call under torch.no_grad() or freeze the parameters")
         with torch.no_grad(), ops.prof_role(ops.PROF_ROLE_TEXT):
             pos = self.positional_embedding[:text.shape[1]]
-            if self.token_embedding.weight.dtype == pos.dtype == torch.float32:      # one launch, and the bits of the two stock operations
+            if _looks_up_only(self.token_embedding) and _plain_f32(pos) and pos.shape[0] == text.shape[-1]:      # one launch, and the bits of the two stock operations
                 x = ops.embed_tokens(text.contiguous(), self.token_embedding.weight, pos=pos)
             else:
                 x = self.token_embedding(text) + pos
