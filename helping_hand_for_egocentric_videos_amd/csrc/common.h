@@ -52,8 +52,10 @@ void hh_prof_note_kernel(int klass, const char* name);    // runtime.cpp: the ke
 
 // Whether a kernel's output (or an input that it alone reads) of this many bytes goes past the caches (non-temporal accesses).  A plain store of a large output
 // leaves lines behind that are thrown out before the next kernel comes to them, and the copies back to HBM cost the rest of the kernel its bandwidth.
-// Token embedding in fp32, alone / with a LayerNorm of the result behind it, plain -> non-temporal:  61 MB 19.3 / 35.8 -> 19.2 / 37.8 us,
-// 121 MB 36.2 / 71.9 -> 35.9 / 68.9 us,  242 MB 92 / 160 -> 70 / 152 us,  484 MB 181 / 310 -> 136 / 288 us.
+// Token embedding, rows of 768 spread over a table of 49 408, alone / with a LayerNorm of the result behind it, us, plain -> non-temporal:
+//   fp32:  61 MB 18.9 / 36.0 either way,  121 MB 34.4 / 66.2 -> 33.8 / 66.5,  242 MB 90 / 160 -> 65 / 153,  484 MB 177 / 310 -> 128 / 289
+//   bf16:  61 MB 20.5 / 44.1 either way,  121 MB 36.7 / 93.0 -> 34.4 / 94.6,  242 MB 94 / 226 -> 64 / 221,  484 MB 193 / 438 -> 126 / 422
+// (captions, most of whose ids are one, read little of the table: 484 MB of fp32 take 82 us).
 #define HH_STREAM_BYTES (96ll << 20)
 
 #define HH_ALIGNED16(p) ((((uintptr_t)(p)) & 15) == 0)

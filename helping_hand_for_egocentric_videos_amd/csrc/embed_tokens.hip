@@ -19,19 +19,19 @@ typedef unsigned int u32;
 template <int E> struct fvec { float v[E]; };
 
 // E consecutive elements as fp32, in wide accesses where all E exist (`whole`), else `n` of them one by one
-template <int E, typename T, bool NT = false>
+template <int E, typename T>
 __device__ __forceinline__ fvec<E> load_e(const T* p, bool whole, int n) {
     fvec<E> r;
     if (whole) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < E; i += 4) {
-                const f32x4 t = NT ? __builtin_nontemporal_load((const f32x4_any*)(p + i)) : *(const f32x4_any*)(p + i);
+                const f32x4 t = *(const f32x4_any*)(p + i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) r.v[i + j] = t[j];
             }
         } else if constexpr (E == 8) {
-            const u32x4 t = NT ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p;
+            const u32x4 t = *(const u32x4_any*)p;
 #pragma unroll
             for (int j = 0; j < 4; ++j) { r.v[2 * j] = bf16_lo_to_f32(t[j]); r.v[2 * j + 1] = bf16_hi_to_f32(t[j]); }
         } else {
@@ -52,11 +52,11 @@ __device__ __forceinline__ void store_e(T* p, const fvec<E>& r, bool whole, int 
 #pragma unroll
             for (int i = 0; i < E; i += 4) { const f32x4_any t = {r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]}; if (NT) __builtin_nontemporal_store(t, (f32x4_any*)(p + i)); else *(f32x4_any*)(p + i) = t; }
         } else if constexpr (E == 8) {
-            u32x4 t = {pack_bf16(r.v[0], r.v[1]), pack_bf16(r.v[2], r.v[3]), pack_bf16(r.v[4], r.v[5]), pack_bf16(r.v[6], r.v[7])};
-            *(u32x4_any*)p = t;
+            const u32x4_any t = {pack_bf16(r.v[0], r.v[1]), pack_bf16(r.v[2], r.v[3]), pack_bf16(r.v[4], r.v[5]), pack_bf16(r.v[6], r.v[7])};
+            if (NT) __builtin_nontemporal_store(t, (u32x4_any*)p); else *(u32x4_any*)p = t;
         } else {
-            u32x2 t = {pack_bf16(r.v[0], r.v[1]), pack_bf16(r.v[2], r.v[3])};
-            *(u32x2_any*)p = t;
+            const u32x2_any t = {pack_bf16(r.v[0], r.v[1]), pack_bf16(r.v[2], r.v[3])};
+            if (NT) __builtin_nontemporal_store(t, (u32x2_any*)p); else *(u32x2_any*)p = t;
         }
     } else {
 #pragma unroll

@@ -244,3 +244,22 @@ def test_encode_text_takes_tables_that_the_operator_does_not(monkeypatch):
     assert torch.equal(run(), clip.token_embedding(text) + pos[:1]) and not calls
     clip.positional_embedding = nn.Parameter(pos, requires_grad=False)
     assert torch.equal(run(), want) and calls == [1]
+
+
+def test_non_temporal_embedding_kernels_store_past_the_caches(tmp_path):
+    """embed_tokens.hip's forward kernels for large outputs, of every type: in what hipcc makes of them each wide store is non-temporal, and none in the kernels for small outputs."""
+    import os
+    import re
+    import subprocess
+    from helping_hand_for_egocentric_videos_amd import build
+    if not os.path.exists(build.HIPCC):
+        pytest.skip("no hipcc")
+    out = str(tmp_path / "embed_tokens.s")
+    subprocess.run([build.HIPCC] + build.FLAGS + ["--cuda-device-only", "-S", os.path.join(build.CSRC, "embed_tokens.hip"), "-o", out], check=True, capture_output=True)
+    found = set()
+    for name, body in re.findall(r"^(_Z16embed_fwd_kernel\w+):(.*?)\.end_amdhsa_kernel", open(out).read(), re.S | re.M):
+        nt = re.search(r"Lb([01])E", name)[1] == "1"
+        wide = re.findall(r"global_store_dwordx[24][^\n]*", body)
+        assert wide and all((" nt" in line) == nt for line in wide), (name, wide)
+        found.add(name)
+    assert len(found) == 8
