@@ -324,7 +324,7 @@ struct RunList {
     float scale;
 };
 struct RunParams {
-    RunList list[2];                                 // dweight, and dpos if there is one
+    RunList list[2];                                 // dweight and dpos, or the one that is wanted
     const void* dy;
     int n, chunk, chunks, dim, length, seqs;         // dpos: entry j is row t = j / seqs of the sequence j % seqs
     int zeros;                                       // this launch zeroes the rows of dweight that no id names (2: past the caches)
@@ -553,7 +553,7 @@ static int64_t run_chunks(int64_t n, int waves) { return n ? (n + run_chunk(n, w
 
 // ---- few tokens: one launch, no sort -----------------------------------------------------------------------------------------------------
 // Up to DIRECT_TOKENS tokens (DIRECT_NARROW of rows that one workgroup spans) every workgroup can look at all ids itself.  Three kinds of workgroups, by blockIdx.x:
-//   [0, n): a token; the first one of its id finds the others (in ascending order) and sums their rows, the rest of them end
+//   [0, n) if dweight is wanted: a token; the first one of its id finds the others (in ascending order) and sums their rows, the rest of them end
 //   then [0, length) if dpos is wanted: a position's rows
 //   then the zeros of the rows of dweight that no id names, a range of at most DIRECT_ROWS rows each.
 // A workgroup takes 128 pieces of 16 bytes of a row (blockIdx.y); the rows of a sum are dealt out to its 8 (at most 16) sets of threads, whose sums are added in
@@ -570,6 +570,7 @@ struct DirectParams {
     const void* dy;
     float* dweight; float* dpos;
     int accumulate, n, dim, length, seqs;
+    int tokens;                                      // workgroups of tokens: n, or 0 without dweight
     float scale;
     int64_t zero_rows;                               // rows of a zeros' workgroup
 };
@@ -615,7 +616,7 @@ __global__ __launch_bounds__(1024) void direct_kernel(DirectParams p) {
     __shared__ float join[1024 * E];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int block = blockIdx.x;
-    if (block < p.n) {
+    if (block < p.tokens) {
         const int64_t id = direct_id(p, block);
         if (id < 0) return;
         const bool match = tid < p.n && direct_id(p, tid) == id;
@@ -631,7 +632,7 @@ __global__ __launch_bounds__(1024) void direct_kernel(DirectParams p) {
         direct_sum<T, E>(p, list, 0, 0, m, p.dweight + id * p.dim, p.scale, p.accumulate, join);
         return;
     }
-    block -= p.n;
+    block -= p.tokens;
     if (p.dpos != nullptr) {
         if (block < p.length) {
             direct_sum<T, E>(p, nullptr, block, p.length, p.seqs, p.dpos + (int64_t)block * p.dim, 1.f, 0, join);
@@ -725,12 +726,12 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
                (long long)seqs, length, (long long)rows, dim);
     HH_REQUIRE(id_bytes == 4 || id_bytes == 8, HH_ERR_DTYPE, "hh_embed_tokens_bwd: ids are 4 or 8 bytes wide");
     HH_REQUIRE(dy_dtype == HH_F32 || dy_dtype == HH_BF16, HH_ERR_DTYPE, "hh_embed_tokens_bwd: bad dtype");
-    HH_REQUIRE(dweight != nullptr, HH_ERR_ALIGN, "hh_embed_tokens_bwd: dweight is NULL");
+    HH_REQUIRE(dweight != nullptr || dpos != nullptr, HH_ERR_ALIGN, "hh_embed_tokens_bwd: dweight and dpos are NULL");
     hipStream_t s = (hipStream_t)stream;
     const int64_t n = seqs * length;
     const int e = dy_dtype == HH_F32 ? 4 : 8;
     const bool direct = direct_fits(n, rows, dim, e);
-    HH_REQUIRE(n == 0 || (ids != nullptr && dy != nullptr && (direct || (workspace != nullptr && HH_ALIGNED16(workspace)))), HH_ERR_ALIGN,
+    HH_REQUIRE(n == 0 || ((ids != nullptr || dweight == nullptr) && dy != nullptr && (direct || (workspace != nullptr && HH_ALIGNED16(workspace)))), HH_ERR_ALIGN,
                "hh_embed_tokens_bwd: ids, dy and a 16-byte aligned workspace are needed");
     int zb = 0;
     float* zero = accumulate ? nullptr : dweight;
@@ -746,13 +747,13 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
         return hh_check_launch("hh_embed_tokens_bwd");
     }
     if (direct) {
-        int64_t zeros = accumulate ? 0 : (rows * dim + 16383) / 16384;
+        int64_t zeros = zero == nullptr ? 0 : (rows * dim + 16383) / 16384;
         zeros = zeros > 1024 ? 1024 : zeros;
-        const int64_t least = accumulate ? 0 : (rows + DIRECT_ROWS - 1) / DIRECT_ROWS;
+        const int64_t least = zero == nullptr ? 0 : (rows + DIRECT_ROWS - 1) / DIRECT_ROWS;
         if (zeros < least) zeros = least;
-        DirectParams p = {ids, id_bytes == 8, rows, skip_id, dy, dweight, dpos, accumulate != 0, (int)n, dim, length, (int)seqs, scale, zeros ? (rows + zeros - 1) / zeros : 0};
+        DirectParams p = {ids, id_bytes == 8, rows, skip_id, dy, dweight, dpos, accumulate != 0, (int)n, dim, length, (int)seqs, dweight ? (int)n : 0, scale, zeros ? (rows + zeros - 1) / zeros : 0};
         const int across = e * DIRECT_PIECES;
-        const dim3 grid((unsigned)(n + (dpos ? length : 0) + zeros), (unsigned)((dim + across - 1) / across));
+        const dim3 grid((unsigned)(p.tokens + (dpos ? length : 0) + zeros), (unsigned)((dim + across - 1) / across));
         if (dy_dtype == HH_F32) hipLaunchKernelGGL((direct_kernel<float, 4>), grid, dim3(1024), 0, s, p);
         else hipLaunchKernelGGL((direct_kernel<bf16_t, 8>), grid, dim3(1024), 0, s, p);
         return hh_check_launch("hh_embed_tokens_bwd");
@@ -766,14 +767,14 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     char* part = (char*)flags + 2 * flag_bytes;
     const SortPlan sp = sort_plan(n, rows);
     int sorted = sp.passes & 1;                                                   // the buffers that hold the sorted list
-    if (n <= RANK_TOKENS) {
+    if (dweight != nullptr && n <= RANK_TOKENS) {                                 // (dpos has its list without a sort)
         const int tok = n <= 4096 ? 16 : 32, blocks = (int)((n + tok - 1) / tok);          // about a workgroup to a CU
         const ZeroPart z = zero_share(zero, rows * dim, 0, 1, &zb);
 #define RANK(T) hipLaunchKernelGGL((rank_kernel<T>), dim3(blocks + zb), dim3(SORT_THREADS), 0, s, ids, id_bytes == 8, rows, skip_id, keys[0], from[0], (int)n, blocks, z)
         if (tok == 16) RANK(16); else RANK(32);
 #undef RANK
         sorted = 0;
-    } else {
+    } else if (dweight != nullptr) {
         for (int i = 0; i < sp.passes; ++i) {
             ZeroPart z = zero_share(late ? nullptr : zero, rows * dim, 2 * i, 2 * sp.passes, &zb);
             hipLaunchKernelGGL(sort_count_kernel, dim3(sp.blocks + zb), dim3(SORT_THREADS), 0, s, i == 0 ? ids : nullptr, id_bytes == 8, rows, skip_id, keys[i & 1], hist, (int)n, sp.per_block,
@@ -790,15 +791,17 @@ extern "C" int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy
     p.list[1] = RunList{nullptr, nullptr, dpos, (float*)(part + part_bytes), flags + flag_bytes, length, 0, 1.f};
     const int need = (dim + e - 1) / e;
     const int threads = need >= 256 ? 256 : (need + 63) / 64 * 64;
-    const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), (dpos ? 2u : 1u) + (late ? 1u : 0u));
-    // dy past the caches where it is read once (64 x 2048 x 1024 bf16: 150 -> 142 us) or does not fit there; with dpos it is read twice, and 160 x 77 x 768 fp32
+    const unsigned lists = (dweight ? 1u : 0u) + (dpos ? 1u : 0u);
+    if (dweight == nullptr) p.list[0] = p.list[1];
+    const dim3 grid((unsigned)p.chunks, (unsigned)((need + 255) / 256), lists + (late ? 1u : 0u));
+    // dy past the caches where it is read once (64 x 2048 x 1024 bf16: 150 -> 142 us) or does not fit there; with both gradients it is read twice, and 160 x 77 x 768 fp32
     // stay in the cache between (58.5 us, 64.7 past it)
-    const bool nt = !dpos || n * dim * (e == 4 ? 4 : 2) > HH_STREAM_BYTES;
+    const bool nt = lists == 1 || n * dim * (e == 4 ? 4 : 2) > HH_STREAM_BYTES;
     if (e == 4 && nt) hipLaunchKernelGGL((run_sum_kernel<float, 4, true>), grid, dim3(threads), 0, s, p);
     else if (e == 4) hipLaunchKernelGGL((run_sum_kernel<float, 4, false>), grid, dim3(threads), 0, s, p);
     else if (nt) hipLaunchKernelGGL((run_sum_kernel<bf16_t, 8, true>), grid, dim3(threads), 0, s, p);
     else hipLaunchKernelGGL((run_sum_kernel<bf16_t, 8, false>), grid, dim3(threads), 0, s, p);
     if (p.chunks > 1)
-        hipLaunchKernelGGL(run_join_kernel, dim3((unsigned)((p.chunks + 15) / 16), (unsigned)((dim + 255) / 256), dpos ? 2u : 1u), dim3(1024), 0, s, p);
+        hipLaunchKernelGGL(run_join_kernel, dim3((unsigned)((p.chunks + 15) / 16), (unsigned)((dim + 255) / 256), lists), dim3(1024), 0, s, p);
     return hh_check_launch("hh_embed_tokens_bwd");
 }

@@ -29,7 +29,7 @@ class _EmbedTokens(torch.autograd.Function):
         want_pos = ctx.pos_rows is not None and ctx.needs_input_grad[2]
         if not (ctx.needs_input_grad[1] or want_pos):
             return (None,) * 6
-        got = ops.embed_tokens_bwd(ids, dy.contiguous(), ctx.shape[0], scale=ctx.scale, skip_id=ctx.skip_id, pos_grad=want_pos)
+        got = ops.embed_tokens_bwd(ids, dy.contiguous(), ctx.shape[0], scale=ctx.scale, skip_id=ctx.skip_id, pos_grad=want_pos, weight_grad=ctx.needs_input_grad[1])
         dw, dpos = got if want_pos else (got, None)
         if want_pos and dpos.shape[0] < ctx.pos_rows:
             dpos = torch.cat([dpos, dpos.new_zeros((ctx.pos_rows - dpos.shape[0], dpos.shape[1]))])

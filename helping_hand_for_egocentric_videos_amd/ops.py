@@ -1069,14 +1069,17 @@ def embed_tokens(ids, weight, scale=1.0, pos=None, out_dtype=None):
     return out
 
 
-def embed_tokens_bwd(ids, dy, num_rows, scale=1.0, skip_id=None, pos_grad=False, out=None):
+def embed_tokens_bwd(ids, dy, num_rows, scale=1.0, skip_id=None, pos_grad=False, out=None, weight_grad=True):
     """Gradients of embed_tokens: dweight fp32 [num_rows, D] with dweight[v] = scale * the sum of dy over the places whose id is v, and with pos_grad also
     dpos fp32 [L, D] = dy summed over the sequences -> dweight or (dweight, dpos)   (include/hh.h: hh_embed_tokens_bwd).
 
     ids int64 / int32 [..., L], dy fp32 / bf16 [..., L, D].  skip_id: an id without a gradient (nn.Embedding's padding_idx); ids outside [0, num_rows) have
     none either.  out: a fp32 [num_rows, D] buffer that the gradient is ACCUMULATED into (a parameter's slice of the gradient arena), a fresh one by
-    default.  Equal inputs give equal bits (equal ids are added in an order that the ids alone decide, without floating-point atomics)."""
+    default.  weight_grad=False with pos_grad: (None, dpos), without a table's gradient (a frozen table).  Equal inputs give equal bits (equal ids are added in an
+    order that the ids alone decide, without floating-point atomics)."""
     stream = _here(ids, dy, out)
+    if not weight_grad and (out is not None or not pos_grad):
+        raise ValueError("embed_tokens_bwd: weight_grad=False takes pos_grad and no out")
     length, seqs = _ids_of(ids, "embed_tokens_bwd")
     if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] == 0:
         raise ValueError("embed_tokens_bwd: dy must be ids' shape and a last dimension D, got %s for ids %s" % (tuple(dy.shape), tuple(ids.shape)))
@@ -1086,8 +1089,12 @@ def embed_tokens_bwd(ids, dy, num_rows, scale=1.0, skip_id=None, pos_grad=False,
     dd = _dt(dy)
     L = _lib.lib()
     ws = _bytes(L.hh_workspace_bytes_embed_tokens_bwd(seqs, max(length, 1), V, D), "embed_tokens_bwd", dy.device)
-    dw = torch.empty((V, D), dtype=torch.float32, device=dy.device) if out is None else out
+    dw = out
+    if out is None and weight_grad:
+        dw = torch.empty((V, D), dtype=torch.float32, device=dy.device)
     dpos = torch.empty((length, D), dtype=torch.float32, device=dy.device) if pos_grad else None
+    if dw is None and not length:
+        return None, dpos
     _lib.check(L.hh_embed_tokens_bwd(_p(ids), ids.element_size(), _p(dy), dd, _p(dw), int(out is not None), _p(dpos) if length else None, seqs, max(length, 1), V, D,
                                      scale, -1 if skip_id is None else int(skip_id), _p(ws), stream), "hh_embed_tokens_bwd")
     return (dw, dpos) if pos_grad else dw

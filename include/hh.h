@@ -501,7 +501,7 @@ int hh_adamw_arena_step(float* p, float* g, float* m, float* v, int64_t n, const
  *   out[s,t,:] = scale * weight[ids[s,t],:] + pos[t,:]          ids [seqs, length] of id_bytes = 4 or 8; pos fp32 [length, dim] or NULL
  *   dweight[v,:] (+)= scale * sum over ids[s,t] == v of dy[s,t,:]      dpos[t,:] = sum_s dy[s,t,:] (or NULL)
  * An id outside [0, rows) gives a row of NaN forward and no gradient; neither does skip_id (pass -1 for none), like nn.Embedding's padding_idx.
- * accumulate != 0: dweight is added to and untouched where no id points; 0: written whole.  Rows of one id are added in an order that the ids alone
+ * dweight may be NULL where dpos is wanted alone (ids are not read then, and nothing is sorted).  accumulate != 0: dweight is added to and untouched where no id points; 0: written whole.  Rows of one id are added in an order that the ids alone
  * decide (by a sort of theirs, or for few tokens a search), without floating-point atomics: equal inputs give equal bits.  Any dim, pointers aligned to their
  * elements; dim <= 2^20, seqs * length < 2^30, rows < 2^31.  hh_workspace_bytes_embed_tokens_bwd may be 0; workspace may then be NULL. */
 int hh_embed_tokens_fwd(const void* ids, int id_bytes, const void* weight, int w_dtype, const float* pos, void* out, int out_dtype, int64_t seqs, int length, int64_t rows,

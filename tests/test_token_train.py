@@ -263,3 +263,16 @@ def test_non_temporal_embedding_kernels_store_past_the_caches(tmp_path):
         assert wide and all((" nt" in line) == nt for line in wide), (name, wide)
         found.add(name)
     assert len(found) == 8
+
+
+def test_positions_alone_refusals(monkeypatch):
+    """Without a place for the table's gradient there has to be one for the positions'; dy and the workspace are needed as ever, ids are not read."""
+    L = _lib.lib()
+    b = lambda ids=16, dy=16, dw=None, dpos=16, s=2, ws=16: L.hh_embed_tokens_bwd(ids, 8, dy, 0, dw, 0, dpos, s, 3, 5, 8, 1.0, -1, ws, None)  # noqa: E731
+    assert b(dpos=None) == -5 and b(dy=None) == -5 and b(s=2000, ws=None) == -5 and b(s=2000, ws=8) == -5
+    assert b(dw=16, ids=None) == -5
+    monkeypatch.setattr(ops, "_here", lambda *t: 0)
+    ids, dy = torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3, 8)
+    for kw in ({}, {"pos_grad": True, "out": torch.zeros(4, 8)}):
+        with pytest.raises(ValueError, match="weight_grad=False"):
+            ops.embed_tokens_bwd(ids, dy, 4, weight_grad=False, **kw)

@@ -148,6 +148,41 @@ def test_embed_tokens_bwd_infinities_stay_in_their_rows():
     assert torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("S,L,dim", [(1, 1, 3), (7, 73, 96), (60, 17, 516), (40, 60, 541), (9, 900, 64), (160, 77, 768), (3, 4100, 33), (0, 5, 8), (4, 0, 8)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_embed_tokens_bwd_of_the_positions_alone(S, L, dim, dt):
+    """A frozen table: the bits of the joint call's dpos, without its [V, D] gradient.  (One launch, both sorts' sizes, odd widths, no tokens.)"""
+    V = 49408
+    ids, dy = rints(-1, V + 1, (S, L), seed=1), rnd(S, L, dim, seed=2, dtype=dt)
+    _, want = ops.embed_tokens_bwd(ids, dy, V, pos_grad=True)
+    none, got = ops.embed_tokens_bwd(ids, dy, V, pos_grad=True, weight_grad=False)
+    assert none is None and torch.equal(got, want)
+    within(got, dy.double().sum(0), (S + 2) * U * dy.double().abs().sum(0), "pos grad alone")
+
+
+def test_a_frozen_table_with_trained_positions():
+    from torch import nn
+    from helping_hand_for_egocentric_videos_amd.model import token_stream as ts
+    V, D, S, L = 49408, 256, 40, 60
+    emb = ts.TokenEmbedding(V, D).to(DEV).requires_grad_(False)
+    pos, ids, cot = nn.Parameter(rnd(L + 3, D, seed=1)), rints(0, V, (S, L), seed=2), rnd(S, L, D, seed=3)
+    for trained in (False, True):
+        emb.weight.requires_grad_(trained)
+        emb.weight.grad = pos.grad = None
+        out = emb(ids, pos, scale=3.0)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out.backward(cot)
+        torch.cuda.synchronize()
+        assert trained or torch.cuda.max_memory_allocated() - before < V * D * 4 // 2
+        assert (emb.weight.grad is not None) == trained
+        within(pos.grad[:L], cot.double().sum(0), (S + 2) * U * cot.double().abs().sum(0), "frozen table, pos grad")
+        assert not pos.grad[L:].any()
+    ref, bound = embed_grad_ref(ids, cot, V, 3.0, None)
+    within(emb.weight.grad, ref, bound, "trained table")
+
+
 # ---- the end of a residual block -------------------------------------------------------------------------------------------------------
 def block_ref(x, y, gate, tanh, res, post, pre, rms, groups):
     """The definition in the inputs' type (64 bits): (x_new, h)."""
