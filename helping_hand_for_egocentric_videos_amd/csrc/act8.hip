@@ -216,9 +216,9 @@ extern "C" int hh_act8_fwd(const void* u, int u_dtype, void* a, void* q, float* 
     HH_REQUIRE(u_dtype == HH_F32 || u_dtype == HH_BF16, HH_ERR_DTYPE, "hh_act8_fwd: bad dtype");
     HH_REQUIRE(act8_ok(act), HH_ERR_UNSUPPORTED, "hh_act8_fwd: unknown activation %d", act);
     const int per_row = (cols + ACT8_GROUP - 1) / ACT8_GROUP;
+    HH_REQUIRE(rows < (1ll << 40) && hh_grid_fits(act8_grid(rows, cols).blocks, 256), HH_ERR_SHAPE, "hh_act8_fwd: too many rows for a launch (rows=%lld cols=%d)", (long long)rows, cols);
     const Act8Grid g = act8_grid(rows, cols);
     const int64_t blocks = g.blocks;
-    HH_REQUIRE(rows < (1ll << 40) && blocks <= 0x7fffffff, HH_ERR_SHAPE, "hh_act8_fwd: too many rows");
     if (rows == 0) return HH_OK;
     HH_REQUIRE(u != nullptr && q != nullptr && scale != nullptr, HH_ERR_ALIGN, "hh_act8_fwd: NULL pointer");
     const bool f32 = u_dtype == HH_F32, nt = rows * cols * (1 + (a ? (f32 ? 4 : 2) : 0)) > HH_STREAM_BYTES;
@@ -234,9 +234,9 @@ extern "C" int hh_act8_bwd(const void* q, const float* scale, const void* da, vo
     HH_REQUIRE(dtype == HH_F32 || dtype == HH_BF16, HH_ERR_DTYPE, "hh_act8_bwd: bad dtype");
     HH_REQUIRE(act8_ok(act), HH_ERR_UNSUPPORTED, "hh_act8_bwd: unknown activation %d", act);
     const int per_row = (cols + ACT8_GROUP - 1) / ACT8_GROUP;
+    HH_REQUIRE(rows < (1ll << 40) && hh_grid_fits(act8_grid(rows, cols).blocks, 256), HH_ERR_SHAPE, "hh_act8_bwd: too many rows for a launch (rows=%lld cols=%d)", (long long)rows, cols);
     const Act8Grid g = act8_grid(rows, cols);
     const int64_t blocks = g.blocks;
-    HH_REQUIRE(rows < (1ll << 40) && blocks <= 0x7fffffff, HH_ERR_SHAPE, "hh_act8_bwd: too many rows");
     if (rows == 0) return HH_OK;
     HH_REQUIRE(q != nullptr && scale != nullptr && da != nullptr && du != nullptr, HH_ERR_ALIGN, "hh_act8_bwd: NULL pointer");
     const bool f32 = dtype == HH_F32, nt = rows * cols * (f32 ? 4 : 2) * (a ? 2 : 1) > HH_STREAM_BYTES;

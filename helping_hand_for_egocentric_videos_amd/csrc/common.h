@@ -58,6 +58,9 @@ void hh_prof_note_kernel(int klass, const char* name);    // runtime.cpp: the ke
 // (captions, most of whose ids are one, read little of the table: 484 MB of fp32 take 82 us).
 #define HH_STREAM_BYTES (96ll << 20)
 
+// Whether a launch has room for so many workgroups: it counts its threads in 32 bits.
+static inline bool hh_grid_fits(int64_t blocks, int threads) { return blocks >= 0 && blocks <= 0x7fffffff && blocks * threads <= 0xffffffffll; }
+
 #define HH_ALIGNED16(p) ((((uintptr_t)(p)) & 15) == 0)
 
 __device__ __forceinline__ float bf16_lo_to_f32(unsigned int u) { return __uint_as_float(u << 16); }

@@ -681,6 +681,7 @@ extern "C" int hh_embed_tokens_fwd(const void* ids, int id_bytes, const void* we
         int l = 0;                                                                                                                               \
         while (l < 6 && ((int64_t)E << l) < dim) ++l;                                                                                            \
         const int64_t waves = (n + (64 >> l) - 1) / (64 >> l), blocks = (waves + 3) / 4;                                                         \
+        HH_REQUIRE(hh_grid_fits(blocks, 256), HH_ERR_SHAPE, "hh_embed_tokens_fwd: too many tokens for a launch (%lld of dim %d)", (long long)n, dim); \
         if (n * dim * (int64_t)sizeof(TO) > HH_STREAM_BYTES) EFL(TW, TO, E, true); else EFL(TW, TO, E, false);                                    \
     } while (0)
     if (w_dtype == HH_F32 && out_dtype == HH_F32) EF(float, float, 4);

@@ -586,7 +586,7 @@ static RnPlan rn_plan(int64_t rows, int cols, int64_t groups, int at_once) {
 
 static int rn_check(const hh_residual_norm* d, bool bwd, const char* who) {
     HH_REQUIRE(d != nullptr, HH_ERR_SHAPE, "%s: NULL description", who);
-    HH_REQUIRE(d->rows >= 0 && d->cols > 0 && d->cols <= 4096, HH_ERR_SHAPE, "%s: cols=%d must be in [1, 4096]", who, d->cols);
+    HH_REQUIRE(d->rows >= 0 && d->rows < (1ll << 40) && d->cols > 0 && d->cols <= 4096, HH_ERR_SHAPE, "%s: cols=%d must be in [1, 4096], rows=%lld below 2^40", who, d->cols, (long long)d->rows);
     HH_REQUIRE(d->gate_kind >= HH_GATE_NONE && d->gate_kind <= HH_GATE_GROUP, HH_ERR_UNSUPPORTED, "%s: unknown gate kind %d", who, d->gate_kind);
     HH_REQUIRE(d->groups >= 1 && d->groups <= 65000 && d->rows % d->groups == 0 && (d->groups == 1 || d->gate_kind == HH_GATE_GROUP), HH_ERR_SHAPE,
                "%s: %lld rows do not split into %lld gate groups (1 without a gate for each group, 65000 at most)", who, (long long)d->rows, (long long)d->groups);
@@ -621,12 +621,12 @@ static int64_t rn_size(int dtype) { return dtype == HH_F32 ? 4 : 2; }
 extern "C" int hh_residual_norm_fwd(const hh_residual_norm* d, hh_stream_t stream) {
     const int rc = rn_check(d, false, "hh_residual_norm_fwd");
     if (rc != HH_OK || d->rows == 0) return rc;
-    HH_REQUIRE(d->rows <= 0x7fffffff, HH_ERR_SHAPE, "hh_residual_norm_fwd: too many rows");
     hipStream_t s = (hipStream_t)stream;
     bool vec;
     const RnParams p = rn_params(d, &vec);
     const bool nt = d->rows * d->cols * (rn_size(p.x_dt) + (p.h ? rn_size(p.h_dt) : 0)) > HH_STREAM_BYTES;
     const int threads = rn_waves(p.cols) * 64;
+    HH_REQUIRE(hh_grid_fits(d->rows < RN_FWD_MANY ? d->rows : (d->rows + 3) / 4, threads), HH_ERR_SHAPE, "hh_residual_norm_fwd: too many rows for a launch (rows=%lld cols=%d)", (long long)d->rows, p.cols);
 #define RF(R, V, N, X, Y, H) hipLaunchKernelGGL((resnorm_fwd_kernel<R, V, N, X, Y, H>), dim3((unsigned)((d->rows + R - 1) / R)), dim3(threads), 0, s, p)
 #define RFN(X, Y, H) do { if (d->rows < RN_FWD_MANY) RF(1, true, false, X, Y, H); else if (nt) RF(4, true, true, X, Y, H); else RF(4, true, false, X, Y, H); } while (0)
 #define RFH(X, Y) do { if (p.h_dt == HH_F32) RFN(X, Y, HH_F32); else RFN(X, Y, HH_BF16); } while (0)

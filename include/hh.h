@@ -503,7 +503,8 @@ int hh_adamw_arena_step(float* p, float* g, float* m, float* v, int64_t n, const
  * An id outside [0, rows) gives a row of NaN forward and no gradient; neither does skip_id (pass -1 for none), like nn.Embedding's padding_idx.
  * dweight may be NULL where dpos is wanted alone (ids are not read then, and nothing is sorted).  accumulate != 0: dweight is added to and untouched where no id points; 0: written whole.  Rows of one id are added in an order that the ids alone
  * decide (by a sort of theirs, or for few tokens a search), without floating-point atomics: equal inputs give equal bits.  Any dim, pointers aligned to their
- * elements; dim <= 2^20, seqs * length < 2^30, rows < 2^31.  hh_workspace_bytes_embed_tokens_bwd may be 0; workspace may then be NULL. */
+ * elements; dim <= 2^20, seqs * length < 2^30, rows < 2^31; forward, a launch has room for fewer than
+ * 2^26 tokens at any dim, and for more of 128 channels or fewer.  hh_workspace_bytes_embed_tokens_bwd may be 0; workspace may then be NULL. */
 int hh_embed_tokens_fwd(const void* ids, int id_bytes, const void* weight, int w_dtype, const float* pos, void* out, int out_dtype, int64_t seqs, int length, int64_t rows,
                         int dim, float scale, hh_stream_t stream);
 int64_t hh_workspace_bytes_embed_tokens_bwd(int64_t seqs, int length, int64_t rows, int dim);
@@ -517,7 +518,8 @@ int hh_embed_tokens_bwd(const void* ids, int id_bytes, const void* dy, int dy_dt
  * x, x_new, dx_new, dx have x_dtype, y, dy y_dtype, h, dh h_dtype; parameters and their gradients are fp32.  x_new may be x.
  * hh_residual_norm_bwd reads x_new, y, dx_new (NULL: zeros) and dh (with pre) and writes dx, dy and the gradients of the parameters that there are
  * (dpost_beta / dpre_beta may be NULL); dx may be dx_new.  No floating-point atomics.  cols <= 4096, pointers aligned to their elements (the workspace
- * to 16 bytes); groups <= 65000 and rows % groups == 0. */
+ * to 16 bytes); groups <= 65000 and rows % groups == 0; forward, rows * cols below 2^36, cols
+ * rounded up to a multiple of 256. */
 enum hh_gate_kind { HH_GATE_NONE = 0, HH_GATE_SCALAR = 1, HH_GATE_CHANNEL = 2, HH_GATE_GROUP = 3 };
 typedef struct hh_residual_norm {
     int64_t rows, groups;
@@ -556,7 +558,8 @@ int hh_residual_norm_bwd(const hh_residual_norm* d, hh_stream_t stream);
  *   [K, ceil(N / 128)] whose entries are powers of two (only their exponents are used); q * s is exact in the matrix core's bf16, sums are fp32 and in a fixed
  *   order.  q may be columns of a wider checkpoint from a multiple of 128 on, with their scales.  dw and the workspace: 16-byte aligned; the workspace may be NULL
  *   where hh_workspace_bytes_gemm_tn_act8 is 0.  K <= 2^30, M, N, ld_dy, ldq <= 2^24.
- * act: HH_ACT_NONE, HH_ACT_QUICKGELU, HH_ACT_RELU.  Any cols / M / N / K, pointers aligned to their elements. */
+ * act: HH_ACT_NONE, HH_ACT_QUICKGELU, HH_ACT_RELU.  Any cols / M / N / K, pointers aligned to their elements; hh_act8_*: rows * cols below 2^35, cols
+ * rounded up to 128, 256, 512, 1024 or a multiple of 2048 (of 128 where 128 divides them). */
 int hh_act8_fwd(const void* u, int u_dtype, void* a, void* q, float* scale, int64_t rows, int cols, int act, hh_stream_t stream);
 int hh_act8_bwd(const void* q, const float* scale, const void* da, void* du, void* a, int dtype, int64_t rows, int cols, int act, hh_stream_t stream);
 int64_t hh_workspace_bytes_gemm_tn_act8(int M, int N, int64_t K);

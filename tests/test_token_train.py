@@ -276,3 +276,23 @@ def test_positions_alone_refusals(monkeypatch):
     for kw in ({}, {"pos_grad": True, "out": torch.zeros(4, 8)}):
         with pytest.raises(ValueError, match="weight_grad=False"):
             ops.embed_tokens_bwd(ids, dy, 4, weight_grad=False, **kw)
+
+
+def test_calls_that_a_launch_has_no_room_for_are_refused_as_shapes():
+    """A launch counts its threads in 32 bits.  One row under the limit is not tried here: it would be launched."""
+    L = _lib.lib()
+    f = lambda s, d, wd=0, od=0: L.hh_embed_tokens_fwd(16, 8, 16, wd, None, 16, od, s, 1, 5, d, 1.0, None)  # noqa: E731
+    assert f(1 << 26, 768) == -1 and b"too many tokens" in L.hh_last_error_string()
+    assert f(1 << 26, 129, 0, 1) == -1 and f(1 << 26, 129, 1, 0) == -1 and f(1 << 26, 257, 1, 1) == -1 and f(1 << 27, 129, 1, 1) == -1 and f(1 << 29, 30) == -1
+
+    def norm(rows, cols):
+        d = _lib.ResidualNorm()
+        d.rows, d.groups, d.cols, d.res_scale = rows, 1, cols, 1.0
+        d.x = d.y = d.x_new = 16
+        return L.hh_residual_norm_fwd(ctypes.byref(d), None)
+    assert norm(1 << 28, 8) == -1 and b"too many rows" in L.hh_last_error_string()
+    assert norm(1 << 24, 4096) == -1 and norm((1 << 31) - 1, 256) == -1 and norm(1 << 40, 1) == -1 and norm((1 << 63) - 1, 1) == -1
+    for fn, args in ((L.hh_act8_fwd, lambda r, c: (16, 1, None, 16, 16, r, c, 0, None)), (L.hh_act8_bwd, lambda r, c: (16, 16, 16, 16, None, 1, r, c, 0, None))):
+        for rows, cols in ((1 << 28, 128), (1 << 28, 1), (1 << 24, 2047), (1 << 23, 2049), ((1 << 63) - 1, 4096)):
+            assert fn(*args(rows, cols)) == -1, (rows, cols)
+            assert b"too many rows" in L.hh_last_error_string()
