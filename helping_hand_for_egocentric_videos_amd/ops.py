@@ -1038,6 +1038,13 @@ def _bytes(nbytes, what, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _ints(what, *sizes):
+    """Sizes that the library takes as 32-bit integers: ctypes would cut larger ones off without a word."""
+    for n in sizes:
+        if n > 0x7fffffff:
+            raise ValueError("%s: a size of %d is over 2^31 - 1" % (what, n))
+
+
 def _ids_of(ids, what):
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError("%s: ids must be int64 or int32, got %s" % (what, ids.dtype))
@@ -1058,6 +1065,7 @@ def embed_tokens(ids, weight, scale=1.0, pos=None, out_dtype=None):
     if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError("embed_tokens: weight must be [V, D], got %s" % (tuple(weight.shape),))
     V, D = weight.shape
+    _ints("embed_tokens", length, D)
     if pos is not None and (pos.dtype != torch.float32 or pos.dim() != 2 or pos.shape[1] != D or pos.shape[0] < length):
         raise ValueError("embed_tokens: pos must be fp32 [>= %d, %d], got %s %s" % (length, D, pos.dtype, tuple(pos.shape)))
     out = weight.new_empty((*ids.shape, D), dtype=out_dtype)
@@ -1084,6 +1092,7 @@ def embed_tokens_bwd(ids, dy, num_rows, scale=1.0, skip_id=None, pos_grad=False,
     if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] == 0:
         raise ValueError("embed_tokens_bwd: dy must be ids' shape and a last dimension D, got %s for ids %s" % (tuple(dy.shape), tuple(ids.shape)))
     V, D = int(num_rows), dy.shape[-1]
+    _ints("embed_tokens_bwd", length, D)
     if out is not None and (out.dtype != torch.float32 or tuple(out.shape) != (V, D)):
         raise ValueError("embed_tokens_bwd: out must be fp32 [%d, %d]" % (V, D))
     dd = _dt(dy)
@@ -1109,6 +1118,7 @@ def _residual_norm_desc(what, x, y, gate, gate_tanh, res_scale, post, pre, rms):
     cols = shape[-1] if shape else 0
     if cols == 0 or y.shape != shape:
         raise ValueError("%s: stream and branch must have one shape [..., cols], got %s and %s" % (what, tuple(shape), tuple(y.shape)))
+    _ints(what, cols)
     rows, groups, kind, gate_at = x.numel() // cols, 1, GATE_NONE, None
     if gate is not None:
         if gate.dtype != torch.float32:
@@ -1196,6 +1206,7 @@ def _chk_act8(q, scale, what):
         raise TypeError("%s: q must be float8_e4m3fn [rows, cols] (act8's), got %s %s" % (what, q.dtype, tuple(q.shape)))
     if scale.dtype != torch.float32 or scale.shape != (shape[0], -(-shape[1] // ACT8_GROUP)):
         raise TypeError("%s: scale must be fp32 [rows, ceil(cols / 128)] (act8's), got %s %s" % (what, scale.dtype, tuple(scale.shape)))
+    _ints(what, shape[1])
 
 
 def act8(u, act=ACT_NONE, want_out=True):
@@ -1207,6 +1218,7 @@ def act8(u, act=ACT_NONE, want_out=True):
         raise ValueError("act8: u must be [rows, cols], got %s" % (tuple(u.shape),))
     dt = _dt(u)
     rows, cols = u.shape
+    _ints("act8", cols)
     a = torch.empty_like(u) if want_out else None
     q = u.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
     scale = u.new_empty((rows, -(-cols // ACT8_GROUP)), dtype=torch.float32)
@@ -1245,6 +1257,7 @@ def gemm_tn_act8(dy, q, scale, colsum=False, out=None):
     N = q.shape[1]
     if dy.dtype != torch.bfloat16 or q.shape[0] != K or M == 0:
         raise ValueError("gemm_tn_act8: dy must be bf16 [%d, M], got %s %s" % (q.shape[0], dy.dtype, tuple(dy.shape)))
+    _ints("gemm_tn_act8", M)
     if out is None:
         out = torch.empty((M, N), dtype=torch.float32, device=dy.device)
     elif out.dtype != torch.float32 or tuple(out.shape) != (M, N):

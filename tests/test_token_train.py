@@ -296,3 +296,23 @@ def test_calls_that_a_launch_has_no_room_for_are_refused_as_shapes():
         for rows, cols in ((1 << 28, 128), (1 << 28, 1), (1 << 24, 2047), (1 << 23, 2049), ((1 << 63) - 1, 4096)):
             assert fn(*args(rows, cols)) == -1, (rows, cols)
             assert b"too many rows" in L.hh_last_error_string()
+
+
+def test_sizes_over_32_bits_are_refused_before_they_are_cut_off(monkeypatch):
+    """The library takes widths and lengths as 32-bit integers, of which ctypes keeps the lowest bits: 2^32 + 64 channels would be worked on as 64."""
+    monkeypatch.setattr(ops, "_here", lambda *t: 0)
+    monkeypatch.setattr(_lib, "lib", lambda: pytest.fail("reached the library"))
+    wide = lambda dtype, *shape: torch.zeros((), dtype=dtype).expand(shape)  # noqa: E731
+    n = (1 << 32) + 64
+    ids, f, b, q, i64 = torch.zeros(1, 1, dtype=torch.int64), torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.int64
+    calls = [lambda: ops.embed_tokens(wide(i64, 1, n), wide(b, 4, 1)), lambda: ops.embed_tokens(ids, wide(b, 4, n)),
+             lambda: ops.embed_tokens_bwd(wide(i64, 1, n), wide(b, 1, n, 1), 4), lambda: ops.embed_tokens_bwd(ids, wide(b, 1, 1, n), 4),
+             lambda: ops.residual_norm(wide(b, 1, n), wide(b, 1, n)), lambda: ops.residual_norm_bwd(wide(b, 1, n), wide(b, 1, n), wide(b, 1, n)),
+             lambda: ops.act8(wide(b, 1, n)), lambda: ops.act8_bwd(wide(q, 1, n), wide(f, 1, n // 128 + 1), wide(b, 1, n), 0)]
+    for call in calls:
+        with pytest.raises(ValueError, match="over 2"):
+            call()
+    # (an expanded row has no unit inner stride: a storage that nothing touches)
+    dy = torch.empty(1, n, dtype=b)
+    with pytest.raises(ValueError, match="over 2"):
+        ops.gemm_tn_act8(dy, torch.zeros(1, 8).to(q), torch.ones(1, 1))
