@@ -24,6 +24,7 @@ void hh_set_error(const char* fmt, ...);
 int hh_check_launch(const char* what);
 int hh_stream_cu_count(hipStream_t s);
 int hh_stream_slot(hipStream_t s);          // 0..31, or -1 when more than 32 streams have launched persistent GEMMs      // CUs the stream may use (runtime.cpp)
+bool hh_stream_capturing(hipStream_t s);    // the launch goes into a graph, which runs on other streams than this one, and beside its later work (runtime.cpp)
 
 // device timing of one kernel launch (runtime.cpp: hh_prof_enable / hh_prof_read); `work` = algorithmic flops or bytes of the launch
 struct HHProfScope {

@@ -713,7 +713,8 @@ int hh_gemm256_launch(const GemmParams& pin, hipStream_t s, bool* tail_done) {
             HHProfScope prof(HH_PROF_GEMM256, 2.0 * (double)p.M * p.N * p.K, s);
             if (g_debug_ts > 1) p.debug_ts = (++g_ts_count == g_debug_ts);
             if (g_mode == 5 && p.K >= 384 && p.K % 128 == 0 && p.N <= 4096) {
-                const int slot = g_dynamic ? hh_stream_slot(s) : -1;
+                // (a captured launch takes its tiles by static stride: two graphs that were captured on one stream may run at once, and would share its counters)
+                const int slot = g_dynamic && !hh_stream_capturing(s) ? hh_stream_slot(s) : -1;
                 p.dynamic = slot >= 0;
                 p.tile_slot = slot >= 0 ? slot : 0;      // (N: bias vector + epilogue scratch share the 32 KB of LDS the ring leaves)
                 static const char* const w4p_names[18] = {"gemm256w4p_kernel<false, 0, 256>", "gemm256w4p_kernel<true, 0, 256>", "gemm256w4p_kernel<false, 1, 256>", "gemm256w4p_kernel<true, 1, 256>",

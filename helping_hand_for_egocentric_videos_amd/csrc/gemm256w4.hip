@@ -659,7 +659,8 @@ __device__ __forceinline__ void w4p_store_tile_z(const GemmParams& p, bf16_t* cw
 }
 
 // Dynamic tile walk: per stream slot (runtime.cpp: hh_stream_slot) 8 per-XCD tile counters + the count of finished workgroups; the last
-// workgroup of a launch zeroes them again (kernels of one stream never overlap).  Zero-initialised device memory, no allocation.
+// workgroup of a launch zeroes them again (kernels of one stream never overlap; launches into a graph, which may run beside that stream's work, take no slot).
+// Zero-initialised device memory, no allocation.
 __device__ unsigned g_w4_tile_cnt[32][16];
 
 //

@@ -93,6 +93,13 @@ int hh_stream_slot(hipStream_t s) {
     return g_slot_n++;
 }
 
+bool hh_stream_capturing(hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &status) == hipSuccess) return status != hipStreamCaptureStatusNone;
+    (void)hipGetLastError();
+    return false;
+}
+
 extern "C" int hh_stream_set_cu_budget(hh_stream_t stream, int n_cus) {
     const int ncu = device_cus();
     if (n_cus == 0) n_cus = ncu;

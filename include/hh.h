@@ -49,7 +49,7 @@ int hh_abi_sizeof(const char* name);
  *   "gemm_tail"     1 (default) = row tails of <= 64 rows (M - 256*floor(M/256), K % 512 == 0) inside the persistent kernel where it
  *                   runs (pieces of <= 32 rows x 32 columns per workgroup), else as 2; 2 = tails of <= 64 rows always on the separate
  *                   split-K-in-workgroup kernel; 0 = on the 128x128 kernel.  Same results in all three.
- *   "gemm256_dynamic" 1 (default) = the persistent 4-wave kernel takes every tile after a workgroup's first from per-XCD atomic counters
+ *   "gemm256_dynamic" 1 (default) = the persistent 4-wave kernel takes every tile after a workgroup's first from per-XCD atomic counters (never in a captured graph)
  *                   (per launch stream, zeroed again by the launch's last workgroup), 0 = static stride
  *   "gemm256_min_tiles" fewest 256x256 tiles for which the 256x256 kernels are used (default 192; the persistent 4-wave kernel takes
  *                   its shapes from 128 tiles on); smaller GEMMs run on the 128x128 kernel

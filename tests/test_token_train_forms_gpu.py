@@ -298,3 +298,53 @@ def test_mlp_act8_of_every_form(rows, act, biases, xt):
         err, size = float((t.double() - ref).norm()), float(ref.norm())
         T.record("test_token_train_forms_gpu", "mlp " + what, err / (size + 1e-300), 2.0 ** -7)
         assert err <= 2.0 ** -7 * size, (what, err, size)
+
+
+# ---- graphs that run at once -----------------------------------------------------------------------------------------------------------
+def mlp_pass(rows, seed):
+    """An MLP's forward and backward pass over fresh inputs of its own -> (what runs it, the tensors that it reads)."""
+    D, H = 512, 1024
+    torch.manual_seed(seed)
+    fc1, fc2 = nn.Linear(D, H).to(DEV), nn.Linear(H, D).to(DEV)
+    x, dy = rnd(rows, D, seed=seed, dtype=BF16).requires_grad_(True), rnd(rows, D, seed=seed + 1)
+
+    def run():
+        y = ts.mlp_act8(x, fc1, fc2)
+        return [y.detach(), *torch.autograd.grad(y, [x, fc1.weight, fc1.bias, fc2.weight, fc2.bias], dy)]
+    return run, (x, dy)
+
+
+def captured(run):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    return graph, outs
+
+
+@pytest.mark.parametrize("rows", [640, 65536])
+def test_captured_mlps_that_run_at_once(rows):
+    """Two graphs, captured one after the other on torch's one capture stream and replayed side by side on two others (65 536 rows: products of 1024 tiles, more than there are
+    workgroups), with eager passes between: each replay gives the eager results' bits."""
+    runs = [mlp_pass(rows, seed) for seed in (1, 5)]
+    graphs = [captured(run) for run, _ in runs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(4):
+        for k, (_, (x, dy)) in enumerate(runs):
+            with torch.no_grad():
+                x.copy_(rnd(rows, x.shape[1], seed=10 * turn + k, dtype=BF16))
+                dy.copy_(rnd(rows, dy.shape[1], seed=10 * turn + k + 5))
+            for o in graphs[k][1]:
+                o.zero_()
+        torch.cuda.synchronize()
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (run, _), (_, outs) in zip(runs, graphs):
+            for i, (got, want) in enumerate(zip(outs, run())):
+                assert torch.equal(got, want), (turn, i)
