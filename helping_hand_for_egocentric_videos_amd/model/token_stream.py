@@ -72,7 +72,7 @@ class _ResidualNorm(torch.autograd.Function):
 def _norm_of(m, rms, which):
     if m is None:
         return None, None, 0.0
-    if isinstance(m, nn.RMSNorm) != rms:
+    if not isinstance(m, nn.RMSNorm if rms else nn.LayerNorm):
         raise TypeError("residual_norm: %s is a %s, with rms=%s" % (which, type(m).__name__, rms))
     if m.weight is None:
         raise ValueError("residual_norm: %s has no weight (elementwise_affine=False)" % which)
@@ -117,6 +117,9 @@ def mlp_act8(x, fc1, fc2, act=ops.ACT_QUICKGELU):
     bytes for a value of either; fc2's input, which has the width of fc1's output, is taken again from that and not kept).  fc1, fc2: nn.Linear whose widths are multiples of 128 (ops.gemm, ops.gemm_tn)."""
     if x.dim() != 2:
         raise ValueError("mlp_act8: x must be [rows, D]")
+    for m in (fc1, fc2):                             # (its weight and bias are used, and nothing else that it may do)
+        if not isinstance(m, nn.Linear) or type(m).forward is not nn.Linear.forward:
+            raise TypeError("mlp_act8: fc1 and fc2 must be nn.Linear, got %s" % type(m).__name__)
     return _MlpAct8.apply(x, fc1.weight, fc1.bias, fc2.weight, fc2.bias, act)
 
 

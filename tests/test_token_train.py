@@ -316,3 +316,34 @@ def test_sizes_over_32_bits_are_refused_before_they_are_cut_off(monkeypatch):
     dy = torch.empty(1, n, dtype=b)
     with pytest.raises(ValueError, match="over 2"):
         ops.gemm_tn_act8(dy, torch.zeros(1, 8).to(q), torch.ones(1, 1))
+
+
+def test_modules_that_are_not_what_the_autograd_forms_compute_are_refused():
+    """Their weights have the right sizes and names: they were taken for a LayerNorm, or for a plain Linear."""
+    from torch import nn
+    from helping_hand_for_egocentric_videos_amd.model import token_stream as ts
+
+    class OwnNorm(nn.Module):                                        # a root-mean-square norm of the user's
+        def __init__(self):
+            super().__init__()
+            self.weight, self.eps = nn.Parameter(torch.ones(8)), 1e-6
+    x = torch.zeros(2, 8)
+    for norm in (nn.BatchNorm1d(8), nn.GroupNorm(2, 8), OwnNorm()):
+        for rms in (False, True):
+            with pytest.raises(TypeError, match="post"):
+                ts.residual_norm(x, x, post=norm, rms=rms)
+
+    class LowRank(nn.Linear):
+        def forward(self, x):
+            return super().forward(x) + 1
+
+    class Wrapper(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.base = nn.Linear(128, 128)
+            self.weight, self.bias = self.base.weight, self.base.bias
+    plain = nn.Linear(128, 128)
+    for other in (LowRank(128, 128), Wrapper()):
+        for fcs in ((plain, other), (other, plain)):
+            with pytest.raises(TypeError, match="must be nn.Linear"):
+                ts.mlp_act8(torch.zeros(2, 128), *fcs)
