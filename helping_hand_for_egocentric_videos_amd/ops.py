@@ -418,7 +418,7 @@ def _set_ln(e, ln, M, N, bias):
 
 def to_bf16(x):
     _chk(x)
-    if x.dtype == torch.bfloat16:
+    if _dt(x) == BF16:                               # (fp32 or an error: the kernel reads four bytes for a value)
         return x
     y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
     _lib.check(_lib.lib().hh_cast_f32_to_bf16(_p(x), _p(y), x.numel(), _stream()), "hh_cast_f32_to_bf16")
@@ -427,7 +427,7 @@ def to_bf16(x):
 
 def to_f32(x):
     _chk(x)
-    if x.dtype == torch.float32:
+    if _dt(x) == F32:
         return x
     y = torch.empty(x.shape, dtype=torch.float32, device=x.device)
     _lib.check(_lib.lib().hh_cast_bf16_to_f32(_p(x), _p(y), x.numel(), _stream()), "hh_cast_bf16_to_f32")
