@@ -10,8 +10,8 @@
 //              Infinities and NaN do not count for the scale; both are stored as e4m3's NaN, so that a gradient that uses them shows it.
 //   backward:  v = q * s;  du = da * act'(v), and on request act(v), the operand of the next product's weight gradient.
 //
-// Both are bound by HBM: a lane takes 8 channels (16 B of bf16), 16 lanes share a scale, one exchange over them.  32 776 x 4096 bf16 (QuickGELU): forward 111 us = 6.1
-// TB/s, backward 106 us = 6.4 TB/s with outputs past the caches (a copy of 2 GiB: 4.9 TB/s).  A row that no 16 bytes divide is read and written in the same pieces, the
+// Both are bound by HBM: a lane takes 8 channels (16 B of bf16), 16 lanes share a scale, one exchange over them.  32 776 x 4096 bf16 (QuickGELU): forward 112 us = 6.0
+// TB/s, backward 106-107 us = 6.3 TB/s with outputs past the caches (a copy of 2 GiB: 4.9 TB/s).  A row that no 16 bytes divide is read and written in the same pieces, the
 // last one moved back to end with the row (24 640 x 767: 20.7 us, one element at a time 52.7).
 #include "common.h"
 

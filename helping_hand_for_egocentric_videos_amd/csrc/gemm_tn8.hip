@@ -41,11 +41,14 @@ struct Tn8Params {
 // A step is 32 tokens: WT^2 matrix instructions for each wave.  LDS holds four tiles of 32 tokens and the registers are on their way with two more, so that a
 // request has two steps' time before its data are put into LDS, and a tile stands there a step before its first fragment is read: one barrier a step.
 // WT = 8 (256 x 256, one wave to a SIMD, 256 accumulators): 16 KB of fragments feed 64 instructions of 16 cycles; the four waves' reads take 512 of those
-//   1024 cycles of LDS, the writes 256.  Bound by the matrix core and the power that it may draw: 65 552 tokens x 1024 x 4096 with db 449 us = 1224 TFLOP/s, where a
-//   library product of 8192^3 in bf16 reaches 1263 on the same card, and its product of this shape and layout, from operands that are bf16 already, 818.
+//   1024 cycles of LDS, the writes 256.  Bound by the matrix core and the power that it may draw: 65 552 tokens x 1024 x 4096 with db 449-461 us = 1190-1224 TFLOP/s (442, and
+//   13 to join its slices, among 200 passes; 530 among the first twelve, before the clock has settled), where a library product of 8192^3 in bf16 reaches 1263 on the same card,
+//   and its product of this shape and layout, from operands that are bf16 already, 818.
 // WT = 4 (128 x 128) for outputs and lengths that give the other too few workgroups: bound by a step's latencies (0.3 us with one wave to a SIMD, where its products take
-//   0.1), so that two groups of four waves take every second tile each and add their sums at the end (12 320 x 768 x 768 35.9 -> 31.5 us).  2464 x 768 x 768 takes
-//   19 us with the launch that joins its five slices.
+//   0.1), so that two groups of four waves take every second tile each and add their sums at the end (12 320 x 768 x 768 35.9 -> 31.5 us).  A step of both, 64 tokens, takes 0.5 us.
+//   A short call is bound by its start and end: of the 16.1 us of 2464 x 768 x 768, five slices of eight steps, the steps are 4.0;  launch, three rounds of loads that wait for each
+//   other, the groups' exchange and one slice's store 6.9;  the four more slices, 2.4 MB to write each, 5.2;  and another launch joins them in 4.0.  (768 x 768, one slice: 1 token, four
+//   steps with those that fill up, 8.9 us, 512 tokens 10.9;  2, 3, 4, 5 slices of 512 12.9, 14.0, 15.0, 16.1;  seven slices, 7168, 14 336, 28 672 tokens: 19.2, 27.8, 45.2.)
 template <int WT, bool VEC>
 __global__ __launch_bounds__(WT == 8 ? 256 : 512) void gemm_tn8_kernel(Tn8Params p) {
     constexpr int G = WT == 8 ? 1 : 2;                                                    // groups of four waves: every G-th tile of the slice to each

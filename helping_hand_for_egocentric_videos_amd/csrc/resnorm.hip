@@ -16,7 +16,8 @@
 // parameters are read once for them, R rows of loads are in flight, and one exchange through LDS (one barrier) serves the sums of R rows.  A wave per row, the
 // obvious form, holds 16 channels of five sums in a lane at 1024 channels: 256 registers, one wave to a SIMD, 1168 us for the backward pass of 131 104 rows.
 // Measured, both norms: forward 131 104 x 1024 (fp32 stream, bf16 branch) 268 us = 6.0 TB/s, bound by HBM; backward of it 472 us = 5.1 TB/s, near HBM's rate for two thirds
-// reads; backward 12 320 x 768 bf16 32 us for both launches, where the arithmetic (VALU 84 % busy) is as long as the traffic.
+// reads; backward 12 320 x 768 bf16 24.5 us and 5.5 for the second launch over the same inputs again and again, 31.0 and 7.0 over a few first ones, 32-33 for both with three sets of
+// inputs in turn; its arithmetic (VALU 82 % busy) is as long as the traffic.
 #include "common.h"
 
 struct Q4 { float v[4]; };

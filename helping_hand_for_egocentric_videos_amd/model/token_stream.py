@@ -1,7 +1,8 @@
 """Autograd of the operators that a trainable token tower needs around its matrix products and attention cores (ops.embed_tokens, ops.residual_norm,
 ops.act8): the embedding with the gradient of its table by sorted tokens, the end of a residual block, and an MLP that keeps its activations in 8
-bits.  The reference trains none of its towers (run/train.py:89 freezes the backbone); these are the pieces with which a user of this
-package would: `CLIP.encode_text`'s lookup (LaviLa.py:660-663), the tanh-gated residual of `SpaceTimeBlock` (LaviLa.py:305-390), `Mlp` (LaviLa.py:175-190).
+bits.  The reference trains none of its towers (run/train.py:89 freezes the backbone), and this package's towers stay frozen: their attention cores have no backward
+pass here.  These are pieces for a user's own trained tower or block, next to the decoder's attention and products: `CLIP.encode_text`'s lookup (LaviLa.py:660-663), the
+residual of `SpaceTimeBlock` with the tanh gate that the reference has there (LaviLa.py:305-390), `Mlp` (LaviLa.py:175-190).
 
 Once differentiable.  Under graph capture, as for any autograd function: no eager graph of the same parameters may be alive when a backward pass is captured (drop
 earlier outputs and losses first), and gradients should be None or already allocated outside the capture."""

@@ -1157,7 +1157,8 @@ def residual_norm(x, y, *, gate=None, gate_tanh=False, res_scale=1.0, post=None,
 
     x, y fp32 / bf16 [..., cols], x_new like x, h of out_dtype.  post / pre: (gamma, beta or None, eps) of a norm (fp32 [cols]) or None; rms: root-mean-square norms
     instead of LayerNorms.  gate fp32, through tanh with gate_tanh: one value, [cols], or [groups, cols] for `groups` groups of consecutive rows (a
-    clip's, a caption's).  out: x_new's buffer, may be x itself (the stream updated in place)."""
+    clip's, a caption's).  out: x_new's buffer, may be x itself (the stream updated in place).  add_layernorm is the form for a frozen block's fp32 stream with bf16 branches
+    (two at once, or without writing the sum); this one keeps what residual_norm_bwd needs and takes every other type."""
     stream = _here(x, y, gate, out, *_norm_tensors(post, pre))
     d = _residual_norm_desc("residual_norm", x, y, gate, gate_tanh, res_scale, post, pre, rms)
     if out is not None and (out.dtype != x.dtype or out.shape != x.shape):
